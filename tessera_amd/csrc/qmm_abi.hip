@@ -16,6 +16,7 @@
 
 #include "qmm_kernels.hpp"
 #include "stream_scratch.hpp"
+#include "tree_args.hpp"
 
 namespace {
 
@@ -1445,6 +1446,77 @@ qmm_status run_moe_ffn_rows(const LaunchCtx& c) {
                                          static_cast<uint32_t>(rows), acc != 0, c.stream));
 }
 
+// ---- a tree of drafted tokens (none of these is a reference id) -------------------------------------------
+// What they refuse: tree_args.hpp.
+qmm::LaunchArgs args_of(const LaunchCtx& c) { return qmm::LaunchArgs{c.buf, c.bytes, c.nbuf, c.sc, c.nsc}; }
+
+// "tree_mask": buffers Parents (u32, one a node; 0xFFFFFFFF: follows the cache's last token), Mask (nodes x ceil(nodes / 32)
+// u32: bit j % 32 of word j / 32, node j is seen), Positions (nodes x 3 u64, as "mrope" takes them); scalars nodes (at most
+// 1024), base (the position of a node that follows the cache).  A parent that is no earlier node marks padding.
+qmm_status run_tree_mask(const LaunchCtx& c) {
+  if (const char* why = qmm::check_tree_mask(args_of(c))) return bad(why);
+  return map_hip(qmm::launch_tree_mask(c.ptr<const uint32_t>(0), c.ptr<uint32_t>(1), c.ptr<uint64_t>(2), static_cast<uint32_t>(c.sc[0]), c.sc[1], c.stream));
+}
+
+// "qk_norm_rope": buffers Q (rows of q_stride floats: heads x head_dim, or with a gate heads x (query, gate)), K (rows of
+// k_stride: kv_heads x head_dim), Wq, Wk (head_dim each), Qout (rows x heads*head_dim), Kout (k_row + rows rows of
+// kv_heads*head_dim, fp32 or fp16, nearest even), optionally Gate (as Qout); scalars rows, heads, kv_heads, head_dim,
+// rope_dim, pos_base, fp32 bits of theta and of epsilon, q_stride, k_stride (0: rows side by side), k_f16, k_row.
+// "qk_norm_mrope": Pos (rows x 3 u64) after Wk, no pos_base, then sec_t, sec_h, sec_w as "mrope".  The arithmetic is that of
+// "rmsnorm" over every head, then "rope" / "mrope".
+qmm_status run_qk_norm(const LaunchCtx& c, bool axes) {
+  qmm::QkNormCall call;
+  if (const char* why = qmm::check_qk_norm(args_of(c), axes, &call)) return bad(why);
+  const size_t o = call.q_out;
+  return map_hip(qmm::launch_qk_norm_rope(call, c.ptr<const float>(0), c.ptr<const float>(1), c.ptr<const float>(2), c.ptr<const float>(3),
+                                          axes ? c.ptr<const uint64_t>(4) : nullptr, c.ptr<float>(o), c.ptr<void>(o + 1),
+                                          call.gated ? c.ptr<float>(o + 2) : nullptr, c.stream));
+}
+qmm_status run_qk_norm_rope(const LaunchCtx& c) { return run_qk_norm(c, false); }
+qmm_status run_qk_norm_mrope(const LaunchCtx& c) { return run_qk_norm(c, true); }
+
+// "attention_tree": buffers Q (m x heads*head_dim fp32), K, V (n x kv_heads*head_dim, fp32 or fp16), Mask (m x ceil(tree /
+// 32) u32), Out (as Q); scalars m, n, heads, kv_heads, head_dim, tree, window, kv_f16.  Every row sees the first n - tree
+// keys and those of the last `tree` that its bits name (bit j % 32 of word j / 32: key n - tree + j), of all these the last
+// `window` (0: all); a row that sees nothing becomes zeros.  "attention_tree_q8", "_q4", "_fp8": the caches of
+// "attention_q8", ..: Q, K and V codes, one scale a key row for K and for V, Mask, Out; without kv_f16.
+qmm_status run_attention_tree_kind(const LaunchCtx& c, bool quantized, uint32_t kind) {
+  if (const char* why = qmm::check_attention_tree(args_of(c), quantized, kind)) return bad(why);
+  if (!quantized) kind = static_cast<uint32_t>(c.sc[7]);
+  const uint64_t m = c.sc[0], n = c.sc[1], heads = c.sc[2], kv_heads = c.sc[3], head_dim = c.sc[4], tree = c.sc[5], window = c.sc[6];
+  const size_t at = quantized ? 5 : 3;
+  auto go = [&](uint64_t parts, void* scratch) {
+    return map_hip(qmm::launch_attention_tree(kind, c.ptr<const float>(0), c.ptr<const void>(1), c.ptr<const void>(2),
+                                              quantized ? c.ptr<const float>(3) : nullptr, quantized ? c.ptr<const float>(4) : nullptr,
+                                              c.ptr<const uint32_t>(at), c.ptr<float>(at + 1), m, n, heads, kv_heads, head_dim, tree, window,
+                                              parts, scratch, c.stream));
+  };
+  const uint64_t parts = qmm::attention_tree_parts(kind, m, n, heads, kv_heads, head_dim, window, 64);
+  if (parts > 1) {
+    const StreamBlock block(c, qmm::attention_parts_bytes(m, heads, head_dim, parts), g_parts_scratch);
+    if (block.get() != nullptr) return go(parts, block.get());
+  }
+  return go(1, nullptr);
+}
+qmm_status run_attention_tree(const LaunchCtx& c) { return run_attention_tree_kind(c, false, 0); }
+qmm_status run_attention_tree_q8(const LaunchCtx& c) { return run_attention_tree_kind(c, true, 2); }
+qmm_status run_attention_tree_q4(const LaunchCtx& c) { return run_attention_tree_kind(c, true, 3); }
+qmm_status run_attention_tree_fp8(const LaunchCtx& c) { return run_attention_tree_kind(c, true, 4); }
+
+// "token_logprobs": buffers Logits (row_base + rows rows of vocab fp32), Tokens (rows x tokens u32), Logprobs (rows x tokens),
+// Entropy (rows) and, with top_k, TopTokens (rows x top_k u32), TopLogprobs (rows x top_k); scalars rows, vocab, tokens, top_k
+// (at most 32), row_base.  The largest entries in descending order, equal ones by their column; -infinity has probability 0.
+qmm_status run_token_logprobs(const LaunchCtx& c) {
+  if (const char* why = qmm::check_token_logprobs(args_of(c))) return bad(why);
+  const uint64_t rows = c.sc[0], vocab = c.sc[1], row_base = c.sc[4];
+  const uint32_t count = static_cast<uint32_t>(c.sc[2]), top_k = static_cast<uint32_t>(c.sc[3]);
+  const size_t need = qmm::token_logprobs_scratch_bytes(rows, vocab, top_k, kPartsLimits.small - 16);
+  const StreamBlock block(c, need, g_parts_scratch);
+  return map_hip(qmm::launch_token_logprobs(c.ptr<const float>(0), c.ptr<const uint32_t>(1), c.ptr<float>(2), c.ptr<float>(3),
+                                            top_k == 0 ? nullptr : c.ptr<uint32_t>(4), top_k == 0 ? nullptr : c.ptr<float>(5), rows, vocab, count,
+                                            top_k, row_base, need == 0 ? nullptr : block.get(), need, c.stream));
+}
+
 struct Entry {
   const char* id;
   qmm_fn fn;
@@ -1532,6 +1604,14 @@ const Entry kTable[] = {
     {"permute_mxfp4_wmma", run_permute_mxfp4_wmma},
     {"permute_q4k_rowgroup", run_permute_q4k_rowgroup},
     {"quantize_fp8_pack_a16", run_quantize_fp8_pack_a16},
+    {"tree_mask", run_tree_mask},
+    {"qk_norm_rope", run_qk_norm_rope},
+    {"qk_norm_mrope", run_qk_norm_mrope},
+    {"attention_tree", run_attention_tree},
+    {"attention_tree_q8", run_attention_tree_q8},
+    {"attention_tree_q4", run_attention_tree_q4},
+    {"attention_tree_fp8", run_attention_tree_fp8},
+    {"token_logprobs", run_token_logprobs},
 };
 constexpr size_t kTableSize = sizeof(kTable) / sizeof(kTable[0]);
 

@@ -261,6 +261,23 @@ hipError_t launch_attention_split(const float* q, const void* k, const void* v, 
                                   bool causal, uint64_t split, hipStream_t stream);
 hipError_t launch_attention_combine(const float* pacc, const float* pmax, const float* psum, float* out, uint64_t m,
                                     uint64_t heads, uint64_t head_dim, uint64_t split, hipStream_t stream);
+// The tree forms (tree_args.hpp: their calls).  attention_tree_parts: the parts of the keys, at most `most_parts`, whose sums
+// attention_parts_bytes of `scratch` hold where there are two or more.
+struct QkNormCall;
+uint64_t attention_tree_parts(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                              uint64_t window, uint64_t most_parts);
+hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
+                                 const uint32_t* mask, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
+                                 uint64_t head_dim, uint64_t tree, uint64_t window, uint64_t parts, void* scratch, hipStream_t stream);
+hipError_t launch_tree_mask(const uint32_t* parents, uint32_t* mask, uint64_t* positions, uint32_t nodes, uint64_t base, hipStream_t stream);
+// pos3 null: positions pos_base + row; gate null: none.
+hipError_t launch_qk_norm_rope(const QkNormCall& call, const float* q, const float* k, const float* wq, const float* wk, const uint64_t* pos3,
+                               float* q_out, void* k_out, float* gate, hipStream_t stream);
+// token_logprobs_scratch_bytes: what the shares of rows take of `scratch`, at most `most`; null: rows are not shared.
+size_t token_logprobs_scratch_bytes(uint64_t rows, uint64_t vocab, uint32_t top_k, size_t most);
+hipError_t launch_token_logprobs(const float* logits, const uint32_t* tokens, float* logprobs, float* entropy, uint32_t* top_tokens,
+                                 float* top_logprobs, uint64_t rows, uint64_t vocab, uint32_t count, uint32_t top_k, uint64_t row_base,
+                                 void* scratch, size_t scratch_bytes, hipStream_t stream);
 hipError_t launch_quantize_kv(const float* in, uint8_t* out, float* scale, uint64_t rows, uint64_t cols, uint32_t bits,
                               hipStream_t stream);
 hipError_t launch_cast_f32_f16(const float* in, void* out, uint64_t n, hipStream_t stream);
