@@ -1106,6 +1106,23 @@ __global__ __launch_bounds__(512, 2) void attention_tile_kernel(AttentionArgs a)
   }
 }
 
+// Element idx of a cache's rows, one of key `key`.
+template <KvKind KV>
+__device__ __forceinline__ float cache_element(const void* base, const float* row_scale, uint64_t key, uint64_t idx) {
+  if constexpr (KV == KvKind::F16) {
+    return half_bits_to_float(static_cast<const uint16_t*>(base)[idx]);
+  } else if constexpr (KV == KvKind::F32) {
+    return static_cast<const float*>(base)[idx];
+  } else if constexpr (KV == KvKind::Q8) {
+    return static_cast<float>(static_cast<const int8_t*>(base)[idx]) * row_scale[key];
+  } else if constexpr (KV == KvKind::Q4) {
+    const int nib = (static_cast<const uint8_t*>(base)[idx >> 1] >> ((idx & 1u) * 4u)) & 0xF;
+    return static_cast<float>((nib & 8) ? nib - 16 : nib) * row_scale[key];
+  } else {
+    return e4m3_to_float(static_cast<const uint8_t*>(base)[idx]) * row_scale[key];
+  }
+}
+
 // ---- head sizes that the matrix kernels' 16-byte runs do not divide ------------------------------
 //
 // One workgroup of four wavefronts per (query row, head[, chunk]).  Keys are taken 64 at a time: a
@@ -1128,20 +1145,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionArgs a) {
   }
   const float scale = 1.0f / sqrtf(static_cast<float>(D));
   const uint64_t qb = ((a.row_base + i) * a.heads + h) * D;
-  auto kv_at = [&](const void* base, const float* row_scale, uint64_t key, uint64_t idx) {
-    if constexpr (KV == KvKind::F16) {
-      return half_bits_to_float(static_cast<const uint16_t*>(base)[idx]);
-    } else if constexpr (KV == KvKind::F32) {
-      return static_cast<const float*>(base)[idx];
-    } else if constexpr (KV == KvKind::Q8) {
-      return static_cast<float>(static_cast<const int8_t*>(base)[idx]) * row_scale[key];
-    } else if constexpr (KV == KvKind::Q4) {
-      const int nib = (static_cast<const uint8_t*>(base)[idx >> 1] >> ((idx & 1u) * 4u)) & 0xF;
-      return static_cast<float>((nib & 8) ? nib - 16 : nib) * row_scale[key];
-    } else {
-      return e4m3_to_float(static_cast<const uint8_t*>(base)[idx]) * row_scale[key];
-    }
-  };
+  auto kv_at = [&](const void* base, const float* row_scale, uint64_t key, uint64_t idx) { return cache_element<KV>(base, row_scale, key, idx); };
   float qr[4];                       // head_dim <= 256: up to four elements a lane
 #pragma unroll
   for (int cc = 0; cc < 4; ++cc) qr[cc] = lane + 64u * cc < D ? a.q[qb + lane + 64u * cc] : 0.0f;

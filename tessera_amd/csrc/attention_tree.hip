@@ -4,21 +4,518 @@
 #include "attention_kernels.hpp"
 
 namespace qmm {
+namespace {
 
-uint64_t attention_tree_parts(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
-                              uint64_t window, uint64_t most_parts) {
+// ---- a workgroup shares its keys among 64 (row, head) pairs ---------------------------------------
+//
+// The pairs of a key head, `group` to a row, are the columns of the contractions S^T = K Q^T and O^T = V^T P^T on
+// v_mfma_f32_16x16x32_f16; the fp32 side (queries, weights) enters as two fp16 terms of a value x, hi = RN16(x) and lo =
+// RN16(x - hi), into the same sums: off by at most 2^-23 of x, or 2^-40 of the largest that x is scaled under.  Eight
+// wavefronts, two a SIMD: four groups of 16 columns times two halves of a tile of 64 keys.  A tile is made fp16 (exactly: fp16
+// numbers or codes) once, on its way into LDS, keys row by row, values transposed; all columns read the same operands.
+//
+// Bound by the matrix instructions and what does not go on beside them, as all wavefronts are at the same place.  So nothing
+// is done to the running sums but by the matrix instructions: weights are taken relative to a reference that follows the
+// largest score only where it would leave 2^kSlack of it, and just then the sums are scaled; and the next tile goes to LDS a
+// piece at a time between them.  64 rows of 24 heads of 256 over 4 on 32832 fp16 keys in ten parts: 115 us (702 with a
+// workgroup a row and key head); a tile of 64 keys 1.47 us, 1.79 with the next one's way to LDS in one go, 2.57 with every
+// tile's sums added to the running ones by the vector unit.
+constexpr float kSlack = 4.0f;                    // in powers of two
+
+template <int DP>
+struct TreeTile {
+  static constexpr uint32_t kKeyBytes = 64 * DP * 2, kStage = 2 * kKeyBytes;
+  alignas(16) uint8_t stage[2][kStage];           // 64 keys, then two times 32 keys' values transposed
+  float scales[2][2][64];                         // keys', values'
+  float ref[64], sum[64], up[64];                 // the second half's
+  uint32_t low[4], high[4], special;
+};
+
+// BYTES (1 to 16) at `offset` of a buffer whose end the hardware checks: what lies past it reads as 0.
+template <int BYTES>
+__device__ __forceinline__ void load_run(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t (&r)[(BYTES + 3) / 4]) {
+  if constexpr (BYTES == 1) {
+    r[0] = __builtin_amdgcn_raw_buffer_load_b8(from, offset, 0, 0);
+  } else if constexpr (BYTES == 2) {
+    r[0] = __builtin_amdgcn_raw_buffer_load_b16(from, offset, 0, 0);
+  } else if constexpr (BYTES == 4) {
+    r[0] = __builtin_amdgcn_raw_buffer_load_b32(from, offset, 0, 0);
+  } else if constexpr (BYTES == 8) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0);
+    r[0] = v[0], r[1] = v[1];
+  } else {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0);
+    r[0] = v[0], r[1] = v[1], r[2] = v[2], r[3] = v[3];
+  }
+}
+
+// One (row, head) pair over keys start .. last, in fp32 by 512 threads: where infinities or NaN keep the matrix instructions
+// from it.  Keys 64 at a time, a wavefront's lanes along head_dim for a score, two threads an element of the sum.
+struct PairShared {
+  float score[64], weight[64], sum[512];
+};
+template <KvKind KV>
+__device__ __forceinline__ void attend_pair(const AttentionArgs& a, uint32_t row, uint32_t head, uint32_t kv, uint64_t start, uint64_t last,
+                                            uint32_t s_part, PairShared& sh) {
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, D = a.head_dim, e = t & 255u, half = t >> 8;
+  const uint64_t pair = static_cast<uint64_t>(row) * a.heads + head;
+  const uint32_t* bits = a.mask + static_cast<uint64_t>(row) * a.words;
+  const float scale = 1.0f / sqrtf(static_cast<float>(D));
+  float run_max = -INFINITY, run_sum = 0.0f, acc = 0.0f;
+  for (uint64_t j0 = start; j0 <= last; j0 += 64u) {
+    const uint32_t count = last - j0 < 63u ? static_cast<uint32_t>(last - j0) + 1u : 64u;
+    const uint32_t low = tree_keys(a, bits, j0), high = count > 32u ? tree_keys(a, bits, j0 + 32u) : 0u;
+    auto sees = [&](uint32_t k) { return k < count && ((k < 32u ? low >> k : high >> (k - 32u)) & 1u) != 0u; };
+    for (uint32_t k = wave; k < 64u; k += 8u) {
+      float dot = 0.0f;
+      if (sees(k)) {
+        for (uint32_t d = lane; d < D; d += 64u) dot = fmaf(a.q[pair * D + d], cache_element<KV>(a.k, a.k_scale, j0 + k, ((j0 + k) * a.kv_heads + kv) * D + d), dot);
+      }
+      dot = wave_sum(dot);
+      if (lane == 0u) sh.score[k] = sees(k) ? dot * scale : -INFINITY;
+    }
+    __syncthreads();
+    const float s = sh.score[lane], most = fmaxf(run_max, wave_max(s)), to = reference_score(most);
+    const float w = sees(lane) ? expf(s - to) : 0.0f, corr = expf(run_max - to);      // (the same in every wavefront)
+    if (wave == 0u) sh.weight[lane] = w;
+    run_sum = fmaf(corr, run_sum, wave_sum(w));
+    run_max = most;
+    __syncthreads();
+    float x = 0.0f;
+    for (uint32_t k = half; k < count && e < D; k += 2u) {
+      if (sees(k)) x = fmaf(sh.weight[k], cache_element<KV>(a.v, a.v_scale, j0 + k, ((j0 + k) * a.kv_heads + kv) * D + e), x);
+    }
+    acc = fmaf(corr, acc, x);
+  }
+  sh.sum[t] = acc;
+  __syncthreads();
+  if (t < D) {
+    const float x = acc + sh.sum[t + 256u];
+    if (a.part.split != 0) a.part.pacc[(pair * a.part.split + s_part) * D + t] = x;
+    else a.out[pair * D + t] = run_sum == 0.0f ? 0.0f : x / run_sum;
+  }
+  if (t == 0u && a.part.split != 0) a.part.pmax[pair * a.part.split + s_part] = run_max, a.part.psum[pair * a.part.split + s_part] = run_sum;
+  __syncthreads();
+}
+
+template <KvKind KV, int DP>
+__global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a) {
+  constexpr bool QUANT = kv_quantized(KV);
+  constexpr int BITS = kv_bits(KV);
+  constexpr int STEPS = DP / 32;                                   // matrix instructions of a score, in two sums
+  constexpr int VE = DP / 16, RE = DP / 32;                        // elements of a row of the result, of a value run
+  constexpr int CHUNKS = DP / 8;                                   // runs of eight elements of a key
+  constexpr int KLOADS = 64 * CHUNKS / 512;
+  constexpr int KDW = 8 * BITS / 32, VDW = (RE * BITS + 31) / 32;
+  using Shared = TreeTile<DP>;
+  __shared__ Shared sh;
+
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const uint32_t r = lane & 15u, g = lane >> 4, col_group = wave & 3u, half = wave >> 2;
+  const uint32_t D = a.head_dim, group = a.heads / a.kv_heads;
+  const uint32_t split = a.part.split == 0 ? 1u : static_cast<uint32_t>(a.part.split);
+  const uint32_t kv = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads, s_part = unit % split;
+  const uint32_t columns = static_cast<uint32_t>(a.rows * group);
+  const uint32_t c0 = unit / split * 64u;
+  const uint32_t c_end = c0 + 64u < columns ? c0 + 64u : columns;
+  // A value the compiler takes for a new one: what is needed only now and then or after the walk over the keys is formed
+  // from the thread's number again, not held, where the registers are just enough.
+  auto again = [](uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  // A lane's column of the workgroup's, past the last one the last.
+  struct Column {
+    uint32_t row, head;
+  };
+  auto column = [&](uint32_t thread) {
+    const uint32_t at = c0 + col_group * 16u + (thread & 15u), col = at < c_end ? at : c_end - 1u;
+    return Column{col / group, kv * group + col % group};
+  };
+
+  // The keys that the columns' rows see begin in no order: the earliest start and the latest.  Past the prefix a tile goes by
+  // the rows' bits.
+  const uint32_t prefix = static_cast<uint32_t>(a.n - a.tree);
+  uint32_t start, wg_start, latest_start, wg_last = static_cast<uint32_t>(a.n - 1);
+  {
+    uint64_t first_key, last_key;
+    key_range<true>(a, column(t).row, first_key, last_key);
+    start = static_cast<uint32_t>(first_key);
+    uint32_t low = start, high = start;
+    if (a.window != 0 || prefix == 0u) {
+#pragma unroll
+      for (uint32_t off = 8u; off > 0u; off >>= 1) {
+        const uint32_t l = __shfl_xor(low, off, kWave), h = __shfl_xor(high, off, kWave);
+        low = l < low ? l : low, high = h > high ? h : high;
+      }
+      if (lane == 0u && half == 0u) sh.low[col_group] = low, sh.high[col_group] = high;
+      __syncthreads();
+      low = ~0u, high = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) low = sh.low[i] < low ? sh.low[i] : low, high = sh.high[i] > high ? sh.high[i] : high;
+    }
+    wg_start = __builtin_amdgcn_readfirstlane(low < wg_last ? low : wg_last);
+    latest_start = __builtin_amdgcn_readfirstlane(high);
+  }
+  if (split > 1u) {                                                // whole tiles of the workgroup's keys a part
+    const uint32_t chunk = ((wg_last - wg_start + split) / split + 63u) / 64u * 64u;
+    if (static_cast<uint64_t>(s_part) * chunk > wg_last - wg_start) {
+      for (uint32_t c = c0; c < c_end; ++c) empty_part<512>(a, c / group, kv * group + c % group, 1, s_part);
+      return;
+    }
+    wg_start += s_part * chunk;
+    if (wg_last - wg_start >= chunk) wg_last = wg_start + chunk - 1u;
+  }
+
+  const uint32_t stride = a.kv_heads * D * BITS / 8;               // (times 64 below 2^31: the caller)
+  // This thread's share of a tile's loads: chunk k_chunk of keys k_key + (512 / CHUNKS) i, elements RE v_run.. of keys
+  // 4 v_four.. (lanes l and l + 16 write the halves of a chunk).  Elements past head_dim are read as the row's first: the
+  // queries are 0 there, of the result they are not stored.  Keys past the last read as 0; no column sees them.
+  const uint32_t k_key = t / CHUNKS, k_chunk = t % CHUNKS;
+  const uint32_t v_run = (t & 15u) * 2u + (t >> 5 & 1u), v_four = half * 8u + (t >> 4 & 1u) * 4u + col_group;
+  const uint32_t head_at = kv * D * BITS / 8;
+  const uint32_t k_off = k_key * stride + head_at + (k_chunk * 8u < D ? k_chunk * BITS : 0u);
+  const uint32_t v_off = v_four * 4u * stride + head_at + (v_run * RE < D ? v_run * RE * BITS / 8 : 0u);
+  auto tile_of = [&](const void* base, uint32_t j0, uint32_t row_bytes) {
+    const uint32_t rows = j0 > wg_last ? 0u : wg_last - j0 < 64u ? wg_last - j0 + 1u : 64u;
+    const uint64_t at = reinterpret_cast<uint64_t>(base) + static_cast<uint64_t>(j0) * row_bytes;
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at)), high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(high) << 32 | low), 0,
+                                             static_cast<int>(__builtin_amdgcn_readfirstlane(rows * row_bytes)), 0x00020000);
+  };
+  uint32_t kr[KLOADS][KDW], vr[4][VDW], sr = 0u;
+  auto fetch_keys = [&](uint32_t j0, int i) { load_run<BITS>(tile_of(a.k, j0, stride), k_off + i * (512u / CHUNKS) * stride, kr[i]); };
+  auto fetch_values = [&](uint32_t j0) {
+    const auto tile = tile_of(a.v, j0, stride);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load_run<RE * BITS / 8>(tile, v_off + e * stride, vr[e]);
+  };
+  auto fetch_scales = [&](uint32_t j0) {
+    if constexpr (QUANT) {
+      if (wave < 2u) sr = __builtin_amdgcn_raw_buffer_load_b32(tile_of(wave == 0u ? a.k_scale : a.v_scale, j0, 4u), lane * 4u, 0, 0);
+    }
+  };
+  // A key's row in LDS: its chunks of sixteen bytes at c ^ swizzle, so that neighbouring keys' chunks fall on
+  // different banks; 256 bytes hold 16 chunks.
+  auto key_swizzle = [](uint32_t key) { return CHUNKS >= 16 ? key & 15u : (key >> 1) & 7u; };
+  // Row `row` of a block of 16 rows of 32 keys' values: four chunks of sixteen bytes, chunk c of keys 4c.. and 16 + 4c.. at
+  // c ^ row % 4; the rows in the order 0, 4, 8, 12, 1, .., which with that puts sixteen lanes on sixteen bank groups.
+  auto value_place = [](uint32_t row, uint32_t chunk) { return (row & 3u) * 256u + (row >> 2) * 64u + ((chunk ^ (row & 3u)) * 16u); };
+  auto stash_keys = [&](uint32_t b, int i) {
+    const uint32_t key = k_key + i * (512u / CHUNKS);
+    *reinterpret_cast<half8_t*>(sh.stage[b] + key * (DP * 2u) + ((k_chunk ^ key_swizzle(key)) * 16u)) = key_operand<KV>(kr[i]);
+  };
+  const uint32_t v_to = Shared::kKeyBytes + half * (DP * 64u) + (v_run & 1u) * (RE * 1024u) + value_place(v_run >> 1, v_four & 3u) + (v_four >> 2 & 1u) * 8u;
+  auto stash_values = [&](uint32_t b, int j) {
+    *reinterpret_cast<uint2*>(sh.stage[b] + v_to + j * 1024u) = uint2{value_pair<KV>(vr[0], vr[1], j), value_pair<KV>(vr[2], vr[3], j)};
+  };
+  auto stash_scales = [&](uint32_t b) {
+    if constexpr (QUANT) {
+      if (wave < 2u) {
+        const float x = bit_cast<float>(sr);
+        sh.scales[b][wave][lane] = x;
+        if (wave == 0u && !(fabsf(x) < INFINITY)) sh.special = 1u;   // such a key's score says nothing of its weight here
+      }
+    }
+  };
+
+  if (t == 0) sh.special = 0u;
+  fetch_scales(wg_start);
+#pragma unroll
+  for (int i = 0; i < KLOADS; ++i) fetch_keys(wg_start, i);
+  fetch_values(wg_start);
+
+  // The queries' terms.
+  half8_t q_hi[STEPS], q_lo[STEPS];
+  float score_scale = kLog2E / sqrtf(static_cast<float>(D));
+  {
+    const Column mine = column(t);
+    const float* qp = a.q + (static_cast<uint64_t>(mine.row) * a.heads + mine.head) * D;
+    float raw[STEPS][8], most = 0.0f;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const uint32_t d = i * 32u + g * 8u;
+      const float4 x = d < D ? *reinterpret_cast<const float4*>(qp + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+      const float4 y = d < D ? *reinterpret_cast<const float4*>(qp + d + 4) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+      raw[i][0] = x.x, raw[i][1] = x.y, raw[i][2] = x.z, raw[i][3] = x.w;
+      raw[i][4] = y.x, raw[i][5] = y.y, raw[i][6] = y.z, raw[i][7] = y.w;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(raw[i][e]));
+    }
+    most = groups_max(most);
+    const float up = most == 0.0f ? 1.0f : power_of_two_to(most, 14);
+    score_scale /= up;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = raw[i][kq_dim<KV>(e)] * up;
+        const _Float16 hi = static_cast<_Float16>(v);
+        q_hi[i][e] = hi;
+        q_lo[i][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+      }
+    }
+  }
+  __syncthreads();                                                 // `special` is set up
+  stash_scales(0);
+  fetch_scales(wg_start + 64u);
+#pragma unroll
+  for (int i = 0; i < KLOADS; ++i) stash_keys(0, i), fetch_keys(wg_start + 64u, i);
+#pragma unroll
+  for (int j = 0; j < RE; ++j) stash_values(0, j);
+  fetch_values(wg_start + 64u);
+  lds_barrier();
+
+  float4_t o[VE];
+#pragma unroll
+  for (int j = 0; j < VE; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float ref = -INFINITY, shift = 0.0f, run_sum = 0.0f;             // shift: ref in units of log2, 0 while there is none
+  float lane_most = 0.0f, value_up = QUANT ? power_of_two_to(0.0f, 14) : 0x1p10f;
+  const uint32_t key_row = (half * 32u + r) * (DP * 2u), key_swz = key_swizzle(r);
+  const uint32_t value_row = Shared::kKeyBytes + half * (DP * 64u) + value_place(r, g);
+  // While a tile is multiplied the next one goes to LDS, a piece at a time between the matrix instructions, and the registers
+  // of every piece take the tile after that one's.
+  for (uint32_t j0 = wg_start, b = 0; j0 <= wg_last; j0 += 64u, b ^= 1u) {
+    const uint8_t* stage = sh.stage[b];
+
+    // Element 4 h + e of a lane: key 16 h + 4 g + e of the wavefront's 32.  Operands are read DEEP steps ahead of
+    // their matrix instructions; the barriers keep the compiler from moving each read to its use.
+    float4_t acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int DEEP = 2;
+    half8_t kf[DEEP + 1][2];
+    auto read_keys = [&](int step) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        kf[step % (DEEP + 1)][h] = *reinterpret_cast<const half8_t*>(stage + key_row + h * (16u * DP * 2u) + (((4u * step + g) ^ key_swz) * 16u));
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) read_keys(i);
+    stash_scales(b ^ 1u);
+    fetch_scales(j0 + 128u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+      if (step + DEEP < STEPS) read_keys(step + DEEP);
+#pragma unroll
+      for (int term = 0; term < 2; ++term) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float4_t& x = acc[h][step % 2];
+          x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % (DEEP + 1)][h], term == 0 ? q_hi[step] : q_lo[step], x, 0, 0, 0);
+        }
+      }
+      if (step % 2 == 1) stash_keys(b ^ 1u, step / 2), fetch_keys(j0 + 128u, step / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // The values' operands, read AHEAD blocks ahead of their matrix instructions, two blocks at a time.
+    constexpr int AHEAD = 2;
+    half8_t vf[AHEAD + 2];
+    auto read_values = [&](int j) { vf[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(stage + value_row + j * 1024u); };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) read_values(j);
+
+    float s[8];
+    float4 vsv[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float4_t x = acc[h][0] + acc[h][1];
+      if constexpr (QUANT) {
+        const uint32_t at = half * 32u + h * 16u + g * 4u;
+        const float4 ks = *reinterpret_cast<const float4*>(&sh.scales[b][0][at]);
+        vsv[h] = *reinterpret_cast<const float4*>(&sh.scales[b][1][at]);
+        s[4 * h] = x[0] * ks.x, s[4 * h + 1] = x[1] * ks.y, s[4 * h + 2] = x[2] * ks.z, s[4 * h + 3] = x[3] * ks.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[4 * h + e] = x[e];
+      }
+    }
+    if (j0 + 64u > prefix || j0 < latest_start || wg_last - j0 < 64u) {   // some column does not see some key of the tile
+      const uint32_t now = again(t), key0 = j0 + half * 32u, from = 4u * (now >> 4 & 3u);
+      uint32_t shown = key0 <= wg_last ? tree_keys(a, a.mask + static_cast<uint64_t>(column(now).row) * a.words, key0) : 0u;
+      if (start > key0) shown = start - key0 < 32u ? shown & ~0u << (start - key0) : 0u;
+      if (wg_last - key0 < 31u) shown &= (2u << (wg_last - key0)) - 1u;
+      shown >>= from;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = (shown >> (16 * (e / 4) + e % 4) & 1u) != 0u ? s[e] : -INFINITY;
+    }
+    float most = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
+    float corr = 1.0f;
+    if (__any(most > ref && (ref == -INFINITY || fmaf(most, score_scale, -shift) > kSlack))) {
+      const bool none = ref == -INFINITY;                          // the same in all lanes of the column, as ref is
+      ref = fmaxf(ref, groups_max(most));
+      const float to = ref == -INFINITY ? 0.0f : ref * score_scale;
+      corr = none ? 1.0f : __builtin_amdgcn_exp2f(shift - to);
+      shift = to;
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], score_scale, -shift));
+      sum += s[e];
+    }
+    run_sum = fmaf(corr, run_sum, sum);
+    if constexpr (QUANT) {
+      // The values' scales enter the weights, under a power of two that keeps the largest contribution so far
+      // between 2^9 and 2^15.
+      lane_most *= corr;
+      float here = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        s[e] *= (&vsv[e / 4].x)[e % 4];
+        here = fmaxf(here, fabsf(s[e]));
+      }
+      lane_most = fmaxf(lane_most, here);
+      if (__any(corr != 1.0f || !(here * value_up < 0x1p15f))) {
+        const float largest = groups_max(lane_most), scaled = largest * value_up;
+        if (largest > 0.0f && !(scaled >= 0x1p9f && scaled < 0x1p15f)) {
+          const float up = power_of_two_to(largest, 13);
+          corr *= up / value_up;
+          value_up = up;
+        }
+      }
+    }
+    if (__any(corr != 1.0f)) {
+#pragma unroll
+      for (int j = 0; j < VE; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] *= corr;
+      }
+    }
+    half8_t p_hi, p_lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x = s[e] * value_up;
+      const _Float16 hi = static_cast<_Float16>(x);
+      p_hi[e] = hi;
+      p_lo[e] = static_cast<_Float16>(x - static_cast<float>(hi));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < VE; j += 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (j + AHEAD + i < VE) read_values(j + AHEAD + i);
+      }
+#pragma unroll
+      for (int term = 0; term < 2; ++term) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          o[j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[(j + i) % (AHEAD + 2)], term == 0 ? p_lo : p_hi, o[j + i], 0, 0, 0);
+        }
+      }
+      stash_values(b ^ 1u, j / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    fetch_values(j0 + 128u);
+    lds_barrier();                                                 // (the loads stay under way)
+  }
+  __syncthreads();
+
+  // Merge of the halves under the larger reference; the lanes' shares of the sums of weights first.
+  run_sum = groups_sum(run_sum);
+  const uint32_t late = again(t), late_g = late >> 4 & 3u, own_at = col_group * 16u + (late & 15u);
+  float* piece = reinterpret_cast<float*>(sh.stage[0]) + col_group * (VE * 256u) + (late & 63u);
+  if (half == 1u) {
+    if (late_g == 0u) sh.ref[own_at] = ref, sh.sum[own_at] = run_sum, sh.up[own_at] = value_up;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) piece[(j * 4 + e) * 64] = o[j][e];
+    }
+  }
+  __syncthreads();
+  float total = 0.0f, top = ref;
+  if (half == 0u) {
+    const float other = sh.ref[own_at];
+    top = fmaxf(ref, other);
+    const float to = top == -INFINITY ? 0.0f : top * score_scale;
+    const float w0 = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - to);
+    const float w1 = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(other * score_scale - to);
+    total = fmaf(w1, sh.sum[own_at], w0 * run_sum);
+    const float f0 = w0 / value_up, f1 = w1 / sh.up[own_at];
+    bool finite = fabsf(total) < INFINITY;
+#pragma unroll
+    for (int j = 0; j < VE; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[j][e] = fmaf(piece[(j * 4 + e) * 64], f1, o[j][e] * f0);
+        finite = finite && fabsf(o[j][e]) < INFINITY;
+      }
+    }
+    if (!finite) sh.special = 1u;
+  }
+  __syncthreads();
+  // Infinities and NaN were not kept apart: whatever met one has left a sum that is not finite, or set `special`, and the
+  // workgroup's columns are done again one by one.
+  if (__builtin_amdgcn_readfirstlane(sh.special) != 0u) {          // workgroup-uniform
+    __syncthreads();
+    for (uint32_t c = c0; c < c_end; ++c) {
+      uint64_t row_start, row_last;
+      key_range<true>(a, c / group, row_start, row_last);
+      row_start = row_start > wg_start ? row_start : wg_start, row_last = row_last < wg_last ? row_last : wg_last;
+      attend_pair<KV>(a, c / group, kv * group + c % group, kv, row_start, row_last, s_part, *reinterpret_cast<PairShared*>(sh.stage[0]));
+    }
+    return;
+  }
+  if (half != 0u || c0 + own_at >= c_end) return;
+  const Column mine = column(late);
+  const uint64_t pair = static_cast<uint64_t>(mine.row) * a.heads + mine.head;
+  float* out = a.out + pair * D;
+  float factor = total == 0.0f ? 0.0f : 1.0f / total;
+  if (split > 1u) {
+    const uint64_t part = pair * split + s_part;
+    out = a.part.pacc + part * D;
+    // The part's largest score in natural units is rounded; the sums move by what that took from it.
+    const float natural = score_scale * kLn2, largest = top * natural;
+    factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(top, natural, -largest) * kLog2E);
+    if (late_g == 0u) a.part.pmax[part] = fmaxf(largest, -1e30f), a.part.psum[part] = total * factor;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t d = (late_g * 4u + e) * VE;
+#pragma unroll
+    for (int j = 0; j < VE; j += 4) {
+      if (d + j < D) *reinterpret_cast<float4*>(out + d + j) = float4{o[j][e] * factor, o[j + 1][e] * factor, o[j + 2][e] * factor, o[j + 3][e] * factor};
+    }
+  }
+}
+
+template <KvKind KV>
+hipError_t launch_tree_tiles(const AttentionArgs& a, hipStream_t stream) {
+  const uint64_t split = a.part.split == 0 ? 1 : a.part.split;
+  const AttentionCall call{a.rows, a.n, a.heads, a.kv_heads, a.head_dim, 0, false};
+  const dim3 grid(static_cast<uint32_t>(attention_pairs64(call) * split));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, stream, a); };
+  a.head_dim <= 64 ? go(attention_tree_kernel<KV, 64>) : a.head_dim <= 128 ? go(attention_tree_kernel<KV, 128>) : go(attention_tree_kernel<KV, 256>);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+TreePlan attention_tree_plan(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                             uint64_t window, const void* out, uint64_t most_parts) {
   const uint64_t keys = window != 0 && window < n ? window : n, per = kind == 0 ? 16 : 8;
-  const uint64_t units = m * kv_heads * ((heads / kv_heads + per - 1) / per);
-  uint64_t parts = 2 * static_cast<uint64_t>(num_cus()) / units;
+  const uint32_t dim = static_cast<uint32_t>(head_dim);
+  const bool fits = kind != 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && kv_heads * head_dim * 2 < (1u << 25) && n < (1u << 31) &&
+                    dim % 8 == 0;
+  const bool tile = fits && m * (heads / kv_heads) > 8;
+  const uint64_t units = tile ? (m * (heads / kv_heads) + 63) / 64 * kv_heads : m * kv_heads * ((heads / kv_heads + per - 1) / per);
+  uint64_t parts = (tile ? 1 : 2) * static_cast<uint64_t>(num_cus()) / units;
   if (parts > keys / 128) parts = keys / 128;
   if (parts > most_parts) parts = most_parts;
   while (parts > 1 && attention_parts_size(m, heads, head_dim, parts) > kAttentionPartsMost) --parts;
-  return parts == 0 ? 1 : parts;
+  return TreePlan{tile, parts == 0 ? 1 : parts};
 }
 
 hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                                  const uint32_t* mask, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
-                                 uint64_t head_dim, uint64_t tree, uint64_t window, uint64_t parts, void* scratch, hipStream_t stream) {
+                                 uint64_t head_dim, uint64_t tree, uint64_t window, const TreePlan& plan, void* scratch, hipStream_t stream) {
+  const uint64_t parts = plan.parts;
   AttentionArgs a = args_of(q, k, v, k_scale, v_scale, out, n, heads, kv_heads, head_dim, 0, 0, window, false, m);
   a.mask = mask, a.tree = static_cast<uint32_t>(tree), a.words = static_cast<uint32_t>((tree + 31) / 32);
   if (parts > 1) {
@@ -26,7 +523,10 @@ hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, c
     float* most = acc + m * heads * parts * head_dim;
     a.part = SplitOut{acc, most, most + m * heads * parts, parts};
   }
-  const hipError_t e = launch_attention_as<true>(kind, a, m, stream);
+  const hipError_t e = !plan.tile ? launch_attention_as<true>(kind, a, m, stream) : with_kind(kind, [&](auto tag) {
+    if constexpr (decltype(tag)::value == KvKind::F32) return hipErrorInvalidValue;
+    else return launch_tree_tiles<decltype(tag)::value>(a, stream);
+  });
   if (e != hipSuccess || parts <= 1) return e;
   return launch_combine<true>(a.part.pacc, a.part.pmax, a.part.psum, out, m, heads, head_dim, parts, stream);
 }
