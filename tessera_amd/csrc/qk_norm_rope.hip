@@ -24,7 +24,7 @@ struct QkNormArgs {
 // cos and sin of position * theta^(-2 j / rope_dim), formed in 64 bits and rounded once, as "rope" does.  theta^(-2 j /
 // rope_dim) is the product of the powers turn[b] of j's bits (at most six roundings of 2^-53); the angle is taken modulo
 // pi/2, which three parts hold to more than 2^-150 of it, and the Taylor sums up to x^13 and x^12 miss by less than 2^-40 there.
-__device__ __forceinline__ void cos_sin(const QkNormArgs& a, uint64_t row, uint32_t j, float& c, float& s) {
+__device__ __forceinline__ float2 cos_sin(const QkNormArgs& a, uint64_t row, uint32_t j) {
   uint64_t p = a.pos_base + row;
   if (a.pos3 != nullptr) p = a.pos3[row * 3 + (j < a.sec_t ? 0u : j < a.sec_t + a.sec_h ? 1u : 2u)];
   double f = 1.0;
@@ -44,10 +44,8 @@ __device__ __forceinline__ void cos_sin(const QkNormArgs& a, uint64_t row, uint3
   sn = fma(z, sn, -1.0 / 6.0), cs = fma(z, cs, -0.5);
   sn = fma(x * z, sn, x), cs = fma(z, cs, 1.0);
   const float sin_x = static_cast<float>(sn), cos_x = static_cast<float>(cs);
-  c = (quarter & 1u) != 0u ? sin_x : cos_x;
-  s = (quarter & 1u) != 0u ? cos_x : sin_x;
-  if (quarter == 1u || quarter == 2u) c = -c;
-  if (quarter >= 2u) s = -s;
+  const float c = (quarter & 1u) != 0u ? sin_x : cos_x, s = (quarter & 1u) != 0u ? cos_x : sin_x;
+  return float2{quarter == 1u || quarter == 2u ? -c : c, quarter >= 2u ? -s : s};
 }
 
 // Sum over each run of LANES lanes, in every lane of it.
@@ -82,11 +80,14 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormArgs a) {
   const uint32_t wide = a.gate != nullptr ? 2u * D : D;
   const float *qr = a.q + row * a.q_stride, *kr = a.k + row * a.k_stride;
   auto source = [&](uint32_t h) { return h < a.heads ? qr + static_cast<size_t>(h) * wide : kr + static_cast<size_t>(h - a.heads) * D; };
-  const float4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  auto load = [&](uint32_t h) { return inside && h < all ? *reinterpret_cast<const float4*>(source(h) + e) : zero; };
-  auto load_gate = [&](uint32_t h) { return a.gate != nullptr && inside && h < a.heads ? *reinterpret_cast<const float4*>(source(h) + D + e) : zero; };
+  auto four = [](bool there, const float* from) {
+    if (!there) return float4{0.0f, 0.0f, 0.0f, 0.0f};
+    return *reinterpret_cast<const float4*>(from);
+  };
+  auto load = [&](uint32_t h) { return four(inside && h < all, source(h) + e); };
+  auto load_gate = [&](uint32_t h) { return four(a.gate != nullptr && inside && h < a.heads, source(h) + D + e); };
   float4 next = load(head0), next_gate = load_gate(head0);
-  const float4 wq = inside ? *reinterpret_cast<const float4*>(a.wq + e) : zero, wk = inside ? *reinterpret_cast<const float4*>(a.wk + e) : zero;
+  const float4 wq = four(inside, a.wq + e), wk = four(inside, a.wk + e);
 
   // y' = y cos +- partner sin: the first half of the pairs minus, the second plus, elements past rope_dim as they are.
   float c[4] = {1.0f, 1.0f, 1.0f, 1.0f}, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -94,11 +95,12 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormArgs a) {
   if (e < a.rope_dim) {
     const bool second = e >= pairs;
     partner += second ? -static_cast<int>(pairs / 4u) : static_cast<int>(pairs / 4u);
+    const uint32_t j = second ? e - pairs : e;
+    const float2 t0 = cos_sin(a, row, j), t1 = cos_sin(a, row, j + 1u), t2 = cos_sin(a, row, j + 2u), t3 = cos_sin(a, row, j + 3u);
+    c[0] = t0.x, c[1] = t1.x, c[2] = t2.x, c[3] = t3.x;
+    s[0] = t0.y, s[1] = t1.y, s[2] = t2.y, s[3] = t3.y;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      cos_sin(a, row, second ? e - pairs + i : e + i, c[i], s[i]);
-      s[i] = second ? s[i] : -s[i];
-    }
+    for (uint32_t i = 0; i < 4; ++i) s[i] = second ? s[i] : -s[i];
   }
   const float part = 1.0f / static_cast<float>(D);
   for (uint32_t n = 0; n < a.each; ++n) {
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormArgs a) {
     sum = run_sum<LANES>(sum);
     const float gain = 1.0f / sqrtf(sum * part + a.eps);
     const bool query = h < a.heads;
-    const float4 w = query ? wq : wk;
+    const float4 w = {query ? wq.x : wk.x, query ? wq.y : wk.y, query ? wq.z : wk.z, query ? wq.w : wk.w};
     const float y[4] = {x.x * gain * w.x, x.y * gain * w.y, x.z * gain * w.z, x.w * gain * w.w};
     float z[4];
 #pragma unroll
@@ -125,8 +127,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormArgs a) {
     } else {
       const size_t to = (row * a.kv_heads + (h - a.heads)) * D + e;
       if constexpr (F16) {
-        union { _Float16 h[4]; uint2 u; } v = {{static_cast<_Float16>(z[0]), static_cast<_Float16>(z[1]), static_cast<_Float16>(z[2]), static_cast<_Float16>(z[3])}};
-        *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.k_out) + to) = v.u;
+        const half2_t low = {static_cast<_Float16>(z[0]), static_cast<_Float16>(z[1])}, high = {static_cast<_Float16>(z[2]), static_cast<_Float16>(z[3])};
+        *reinterpret_cast<uint2*>(static_cast<_Float16*>(a.k_out) + to) = uint2{bit_cast<uint32_t>(low), bit_cast<uint32_t>(high)};
       } else {
         *reinterpret_cast<float4*>(static_cast<float*>(a.k_out) + to) = float4{z[0], z[1], z[2], z[3]};
       }
@@ -167,9 +169,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_any_kernel(QkNormArgs a) {
     float z = held[wave][e];
     if (e < a.rope_dim) {
       const bool second = e >= pairs;
-      float c, s;
-      cos_sin(a, row, second ? e - pairs : e, c, s);
-      z = fmaf(z, c, held[wave][second ? e - pairs : e + pairs] * (second ? s : -s));
+      const float2 turned = cos_sin(a, row, second ? e - pairs : e);
+      z = fmaf(z, turned.x, held[wave][second ? e - pairs : e + pairs] * (second ? turned.y : -turned.y));
     }
     if (query) {
       a.q_out[to + e] = z;
@@ -211,7 +212,11 @@ hipError_t launch_qk_norm_rope(const QkNormCall& call, const float* q, const flo
   auto go = [&](auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     const uint64_t groups = (all + 64 / LANES - 1) / (64 / LANES);
-    a.each = 1;
+    // With many heads a wavefront takes several of a row, which share its angles and hide each other's way to memory (us, 1 / 2
+    // / 4 / 7 / 14 at a time: 2048 rows of 28 heads of 256 53 / 38 / 31 / 29 / 31, 512 rows 16 / 11.3 / 10.1 / 9.8 / 11.9, 128 rows
+    // 6.4 / 5.3 / 5.3 / 6.7 / 9.9, one row 4.2 / 4.2 / 4.8 / 6.2 / 9.3).
+    const uint64_t units = call.rows * groups;
+    a.each = units >= 32768 ? 7 : units >= 8192 ? 4 : units >= 2048 ? 2 : 1;
     a.chunks = static_cast<uint32_t>((groups + a.each - 1) / a.each);
     const dim3 g = grid(call.rows * a.chunks);
     if (f16) hipLaunchKernelGGL((qk_norm_rope_kernel<LANES, true>), g, dim3(256), 0, stream, a);
