@@ -27,7 +27,7 @@ struct TreeTile {
   static constexpr uint32_t kKeyBytes = 64 * DP * 2, kStage = 2 * kKeyBytes;
   alignas(16) uint8_t stage[2][kStage];           // 64 keys, then two times 32 keys' values transposed
   float scales[2][2][64];                         // keys', values'
-  float ref[64], sum[64], up[64];                 // the second half's
+  float ref[2][64], sum[2][64], up[2][64];        // the halves'
   uint32_t low[4], high[4], special;
 };
 
@@ -136,12 +136,14 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   // The keys that the columns' rows see begin in no order: the earliest start and the latest.  Past the prefix a tile goes by
   // the rows' bits.
   const uint32_t prefix = static_cast<uint32_t>(a.n - a.tree);
-  uint32_t start, wg_start, latest_start, wg_last = static_cast<uint32_t>(a.n - 1);
-  {
+  auto start_of = [&](uint32_t row) {
     uint64_t first_key, last_key;
-    key_range<true>(a, column(t).row, first_key, last_key);
-    start = static_cast<uint32_t>(first_key);
-    uint32_t low = start, high = start;
+    key_range<true>(a, row, first_key, last_key);
+    return static_cast<uint32_t>(first_key);
+  };
+  uint32_t wg_start, latest_start, wg_last = static_cast<uint32_t>(a.n - 1);
+  {
+    uint32_t low = start_of(column(t).row), high = low;
     if (a.window != 0 || prefix == 0u) {
 #pragma unroll
       for (uint32_t off = 8u; off > 0u; off >>= 1) {
@@ -198,16 +200,18 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   // A key's row in LDS: its chunks of sixteen bytes at c ^ swizzle, so that neighbouring keys' chunks fall on
   // different banks; 256 bytes hold 16 chunks.
   auto key_swizzle = [](uint32_t key) { return CHUNKS >= 16 ? key & 15u : (key >> 1) & 7u; };
-  // Row `row` of a block of 16 rows of 32 keys' values: four chunks of sixteen bytes, chunk c of keys 4c.. and 16 + 4c.. at
-  // c ^ row % 4; the rows in the order 0, 4, 8, 12, 1, .., which with that puts sixteen lanes on sixteen bank groups.
-  auto value_place = [](uint32_t row, uint32_t chunk) { return (row & 3u) * 256u + (row >> 2) * 64u + ((chunk ^ (row & 3u)) * 16u); };
+  // Block j of 32 keys' values holds elements 16 j .. 16 j + 15, a row each of four chunks of sixteen bytes, chunk c of keys 4c..
+  // and 16 + 4c..; chunk c of row r is at place (4 r + c) ^ (r & 12) ^ j of the block, which puts the sixteen blocks or
+  // rows that sixteen lanes write at once on sixteen bank groups.
   auto stash_keys = [&](uint32_t b, int i) {
     const uint32_t key = k_key + i * (512u / CHUNKS);
     *reinterpret_cast<half8_t*>(sh.stage[b] + key * (DP * 2u) + ((k_chunk ^ key_swizzle(key)) * 16u)) = key_operand<KV>(kr[i]);
   };
-  const uint32_t v_to = Shared::kKeyBytes + half * (DP * 64u) + (v_run & 1u) * (RE * 1024u) + value_place(v_run >> 1, v_four & 3u) + (v_four >> 2 & 1u) * 8u;
+  const uint32_t v_row = v_run * RE & 15u, v_block = v_run * RE / 16u;
+  const uint32_t v_to = Shared::kKeyBytes + half * (DP * 64u) + v_block * 1024u + (((v_row * 4u + (v_four & 3u)) ^ (v_row & 12u) ^ v_block) * 16u) + (v_four >> 2 & 1u) * 8u;
   auto stash_values = [&](uint32_t b, int j) {
-    *reinterpret_cast<uint2*>(sh.stage[b] + v_to + j * 1024u) = uint2{value_pair<KV>(vr[0], vr[1], j), value_pair<KV>(vr[2], vr[3], j)};
+    const uint32_t to = v_to ^ static_cast<uint32_t>(((4 * j) ^ (j & 12)) * 16);   // (the bits of v_row + j and of v_row are apart)
+    *reinterpret_cast<uint2*>(sh.stage[b] + to) = uint2{value_pair<KV>(vr[0], vr[1], j), value_pair<KV>(vr[2], vr[3], j)};
   };
   auto stash_scales = [&](uint32_t b) {
     if constexpr (QUANT) {
@@ -225,16 +229,17 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   for (int i = 0; i < KLOADS; ++i) fetch_keys(wg_start, i);
   fetch_values(wg_start);
 
-  // The queries' terms.
+  // The queries' terms: each half makes those of half the steps and takes the others from LDS.
   half8_t q_hi[STEPS], q_lo[STEPS];
   float score_scale = kLog2E / sqrtf(static_cast<float>(D));
   {
+    constexpr int OWN = STEPS / 2;
     const Column mine = column(t);
     const float* qp = a.q + (static_cast<uint64_t>(mine.row) * a.heads + mine.head) * D;
-    float raw[STEPS][8], most = 0.0f;
+    float raw[OWN][8], most = 0.0f;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const uint32_t d = i * 32u + g * 8u;
+    for (int i = 0; i < OWN; ++i) {
+      const uint32_t d = (half * OWN + i) * 32u + g * 8u;
       const float4 x = d < D ? *reinterpret_cast<const float4*>(qp + d) : float4{0.0f, 0.0f, 0.0f, 0.0f};
       const float4 y = d < D ? *reinterpret_cast<const float4*>(qp + d + 4) : float4{0.0f, 0.0f, 0.0f, 0.0f};
       raw[i][0] = x.x, raw[i][1] = x.y, raw[i][2] = x.z, raw[i][3] = x.w;
@@ -243,36 +248,42 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(raw[i][e]));
     }
     most = groups_max(most);
+    if (g == 0u) sh.ref[half][col_group * 16u + r] = most;
+    __syncthreads();                                               // (and `special` is set up)
+    most = fmaxf(sh.ref[0][col_group * 16u + r], sh.ref[1][col_group * 16u + r]);
     const float up = most == 0.0f ? 1.0f : power_of_two_to(most, 14);
     score_scale /= up;
+    half8_t* swap = reinterpret_cast<half8_t*>(sh.stage[1]) + col_group * (STEPS * 128) + lane;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
+    for (int i = 0; i < OWN; ++i) {
+      half8_t hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = raw[i][kq_dim<KV>(e)] * up;
-        const _Float16 hi = static_cast<_Float16>(v);
-        q_hi[i][e] = hi;
-        q_lo[i][e] = static_cast<_Float16>(v - static_cast<float>(hi));
+        hi[e] = static_cast<_Float16>(v);
+        lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
       }
+      swap[(half * OWN + i) * 128u] = hi, swap[(half * OWN + i) * 128u + 64u] = lo;
     }
+    stash_scales(0);
+    fetch_scales(wg_start + 64u);
+#pragma unroll
+    for (int i = 0; i < KLOADS; ++i) stash_keys(0, i), fetch_keys(wg_start + 64u, i);
+#pragma unroll
+    for (int j = 0; j < RE; ++j) stash_values(0, j);
+    fetch_values(wg_start + 64u);
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) q_hi[i] = swap[i * 128], q_lo[i] = swap[i * 128 + 64];
+    lds_barrier();                                                 // the next tile goes where they were
   }
-  __syncthreads();                                                 // `special` is set up
-  stash_scales(0);
-  fetch_scales(wg_start + 64u);
-#pragma unroll
-  for (int i = 0; i < KLOADS; ++i) stash_keys(0, i), fetch_keys(wg_start + 64u, i);
-#pragma unroll
-  for (int j = 0; j < RE; ++j) stash_values(0, j);
-  fetch_values(wg_start + 64u);
-  lds_barrier();
-
   float4_t o[VE];
 #pragma unroll
   for (int j = 0; j < VE; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float ref = -INFINITY, shift = 0.0f, run_sum = 0.0f;             // shift: ref in units of log2, 0 while there is none
   float lane_most = 0.0f, value_up = QUANT ? power_of_two_to(0.0f, 14) : 0x1p10f;
   const uint32_t key_row = (half * 32u + r) * (DP * 2u), key_swz = key_swizzle(r);
-  const uint32_t value_row = Shared::kKeyBytes + half * (DP * 64u) + value_place(r, g);
+  const uint32_t value_row = Shared::kKeyBytes + half * (DP * 64u) + (((r * 4u + g) ^ (r & 12u)) * 16u);
   // While a tile is multiplied the next one goes to LDS, a piece at a time between the matrix instructions, and the registers
   // of every piece take the tile after that one's.
   for (uint32_t j0 = wg_start, b = 0; j0 <= wg_last; j0 += 64u, b ^= 1u) {
@@ -313,7 +324,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     // The values' operands, read AHEAD blocks ahead of their matrix instructions, two blocks at a time.
     constexpr int AHEAD = 2;
     half8_t vf[AHEAD + 2];
-    auto read_values = [&](int j) { vf[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(stage + value_row + j * 1024u); };
+    auto read_values = [&](int j) { vf[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(stage + (value_row ^ static_cast<uint32_t>(j * 16)) + j * 1024u); };
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) read_values(j);
 
@@ -334,7 +345,9 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     }
     if (j0 + 64u > prefix || j0 < latest_start || wg_last - j0 < 64u) {   // some column does not see some key of the tile
       const uint32_t now = again(t), key0 = j0 + half * 32u, from = 4u * (now >> 4 & 3u);
-      uint32_t shown = key0 <= wg_last ? tree_keys(a, a.mask + static_cast<uint64_t>(column(now).row) * a.words, key0) : 0u;
+      const uint32_t row = column(now).row;
+      uint32_t shown = key0 <= wg_last ? tree_keys(a, a.mask + static_cast<uint64_t>(row) * a.words, key0) : 0u;
+      const uint32_t start = a.window == 0 ? 0u : start_of(row);   // (where there is no window, rows that see nothing have no bits)
       if (start > key0) shown = start - key0 < 32u ? shown & ~0u << (start - key0) : 0u;
       if (wg_last - key0 < 31u) shown &= (2u << (wg_last - key0)) - 1u;
       shown >>= from;
@@ -416,39 +429,33 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   }
   __syncthreads();
 
-  // Merge of the halves under the larger reference; the lanes' shares of the sums of weights first.
+  // Merge of the halves under the larger reference, each for half the elements; the lanes' shares of the sums of weights first.
   run_sum = groups_sum(run_sum);
   const uint32_t late = again(t), late_g = late >> 4 & 3u, own_at = col_group * 16u + (late & 15u);
-  float* piece = reinterpret_cast<float*>(sh.stage[0]) + col_group * (VE * 256u) + (late & 63u);
-  if (half == 1u) {
-    if (late_g == 0u) sh.ref[own_at] = ref, sh.sum[own_at] = run_sum, sh.up[own_at] = value_up;
+  constexpr int VH = VE / 2;
+  float4_t* pieces = reinterpret_cast<float4_t*>(sh.stage[0]) + col_group * (VE * 64u) + (late & 63u);
+  if (late_g == 0u) sh.ref[half][own_at] = ref, sh.sum[half][own_at] = run_sum, sh.up[half][own_at] = value_up;
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) piece[(j * 4 + e) * 64] = o[j][e];
-    }
-  }
+  for (int j = 0; j < VH; ++j) pieces[(half * VH + j) * 64u] = half == 0u ? o[VH + j] : o[j];
   __syncthreads();
-  float total = 0.0f, top = ref;
-  if (half == 0u) {
-    const float other = sh.ref[own_at];
-    top = fmaxf(ref, other);
-    const float to = top == -INFINITY ? 0.0f : top * score_scale;
-    const float w0 = ref == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - to);
-    const float w1 = other == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(other * score_scale - to);
-    total = fmaf(w1, sh.sum[own_at], w0 * run_sum);
-    const float f0 = w0 / value_up, f1 = w1 / sh.up[own_at];
-    bool finite = fabsf(total) < INFINITY;
+  const float ref0 = sh.ref[0][own_at], ref1 = sh.ref[1][own_at], top = fmaxf(ref0, ref1);
+  const float to = top == -INFINITY ? 0.0f : top * score_scale;
+  const float w0 = ref0 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref0 * score_scale - to);
+  const float w1 = ref1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref1 * score_scale - to);
+  const float total = fmaf(w1, sh.sum[1][own_at], w0 * sh.sum[0][own_at]);
+  const float f0 = w0 / sh.up[0][own_at], f1 = w1 / sh.up[1][own_at];
+  float4_t merged[VH];                                             // elements 16 (half * VH + j) + 4 g ..
+  bool finite = fabsf(total) < INFINITY;
 #pragma unroll
-    for (int j = 0; j < VE; ++j) {
+  for (int j = 0; j < VH; ++j) {
+    const float4_t own = half == 0u ? o[j] : o[VH + j], other = pieces[((1u - half) * VH + j) * 64u];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        o[j][e] = fmaf(piece[(j * 4 + e) * 64], f1, o[j][e] * f0);
-        finite = finite && fabsf(o[j][e]) < INFINITY;
-      }
+    for (int e = 0; e < 4; ++e) {
+      merged[j][e] = half == 0u ? fmaf(other[e], f1, own[e] * f0) : fmaf(own[e], f1, other[e] * f0);
+      finite = finite && fabsf(merged[j][e]) < INFINITY;
     }
-    if (!finite) sh.special = 1u;
   }
+  if (!finite) sh.special = 1u;
   __syncthreads();
   // Infinities and NaN were not kept apart: whatever met one has left a sum that is not finite, or set `special`, and the
   // workgroup's columns are done again one by one.
@@ -462,7 +469,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     }
     return;
   }
-  if (half != 0u || c0 + own_at >= c_end) return;
+  if (c0 + own_at >= c_end) return;
   const Column mine = column(late);
   const uint64_t pair = static_cast<uint64_t>(mine.row) * a.heads + mine.head;
   float* out = a.out + pair * D;
@@ -473,15 +480,12 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     // The part's largest score in natural units is rounded; the sums move by what that took from it.
     const float natural = score_scale * kLn2, largest = top * natural;
     factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(top, natural, -largest) * kLog2E);
-    if (late_g == 0u) a.part.pmax[part] = fmaxf(largest, -1e30f), a.part.psum[part] = total * factor;
+    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(largest, -1e30f), a.part.psum[part] = total * factor;
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t d = (late_g * 4u + e) * VE;
-#pragma unroll
-    for (int j = 0; j < VE; j += 4) {
-      if (d + j < D) *reinterpret_cast<float4*>(out + d + j) = float4{o[j][e] * factor, o[j + 1][e] * factor, o[j + 2][e] * factor, o[j + 3][e] * factor};
-    }
+  for (int j = 0; j < VH; ++j) {
+    const uint32_t d = (half * VH + j) * 16u + late_g * 4u;
+    if (d < D) *reinterpret_cast<float4_t*>(out + d) = merged[j] * factor;
   }
 }
 
