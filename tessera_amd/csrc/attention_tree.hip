@@ -501,25 +501,25 @@ hipError_t launch_tree_tiles(const AttentionArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-TreePlan attention_tree_plan(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
-                             uint64_t window, const void* out, uint64_t most_parts) {
-  const uint64_t keys = window != 0 && window < n ? window : n, per = kind == 0 ? 16 : 8;
+TreeShape attention_tree_shape(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                               uint64_t window, const void* out, uint64_t most_parts) {
   const uint32_t dim = static_cast<uint32_t>(head_dim);
-  const bool fits = kind != 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && kv_heads * head_dim * 2 < (1u << 25) && n < (1u << 31) &&
-                    dim % 8 == 0;
-  const bool tile = fits && m * (heads / kv_heads) > 8;
-  const uint64_t units = tile ? (m * (heads / kv_heads) + 63) / 64 * kv_heads : m * kv_heads * ((heads / kv_heads + per - 1) / per);
-  uint64_t parts = (tile ? 1 : 2) * static_cast<uint64_t>(num_cus()) / units;
-  if (parts > keys / 128) parts = keys / 128;
+  const bool by_rows = with_kind(kind, [&](auto tag) { return runs_fit<decltype(tag)::value>(dim); });
+  // (a tile's rows lie within 2^31 bytes, its loads are runs of eight elements)
+  const bool shared = kind != 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && kv_heads * head_dim * 2 < (1u << 25) && n < (1u << 31) && dim % 8 == 0;
+  const TreeCall call{m, window != 0 && window < n ? window : n, heads, kv_heads, head_dim, padded_head(dim), kind == 0, kind > 1, by_rows, shared};
+  if (by_rows || shared) return tree_rule(call, static_cast<uint64_t>(num_cus()), most_parts, kAttentionPartsMost);
+  uint64_t parts = 2 * static_cast<uint64_t>(num_cus()) / (m * heads);      // a workgroup a row and head
+  if (parts > call.keys / 128) parts = call.keys / 128;
   if (parts > most_parts) parts = most_parts;
   while (parts > 1 && attention_parts_size(m, heads, head_dim, parts) > kAttentionPartsMost) --parts;
-  return TreePlan{tile, parts == 0 ? 1 : parts};
+  return TreeShape{false, parts < 2 ? 1 : parts};
 }
 
 hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                                  const uint32_t* mask, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
-                                 uint64_t head_dim, uint64_t tree, uint64_t window, const TreePlan& plan, void* scratch, hipStream_t stream) {
-  const uint64_t parts = plan.parts;
+                                 uint64_t head_dim, uint64_t tree, uint64_t window, const TreeShape& shape, void* scratch, hipStream_t stream) {
+  const uint64_t parts = shape.parts;
   AttentionArgs a = args_of(q, k, v, k_scale, v_scale, out, n, heads, kv_heads, head_dim, 0, 0, window, false, m);
   a.mask = mask, a.tree = static_cast<uint32_t>(tree), a.words = static_cast<uint32_t>((tree + 31) / 32);
   if (parts > 1) {
@@ -527,7 +527,7 @@ hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, c
     float* most = acc + m * heads * parts * head_dim;
     a.part = SplitOut{acc, most, most + m * heads * parts, parts};
   }
-  const hipError_t e = !plan.tile ? launch_attention_as<true>(kind, a, m, stream) : with_kind(kind, [&](auto tag) {
+  const hipError_t e = !shape.tile ? launch_attention_as<true>(kind, a, m, stream) : with_kind(kind, [&](auto tag) {
     if constexpr (decltype(tag)::value == KvKind::F32) return hipErrorInvalidValue;
     else return launch_tree_tiles<decltype(tag)::value>(a, stream);
   });

@@ -223,6 +223,60 @@ constexpr uint64_t attention_rule(const AttentionCall& a, uint64_t cus, uint64_t
   return one_us < 0.98 * row_us ? 1 : 0;
 }
 
+// ---- "attention_tree" ------------------------------------------------------------------------------------------------
+// How a call runs: a workgroup a row and key head (`tile` false), or 64 (row, head) pairs of a key head that share their keys, 64
+// at a time; and the parts of the keys.  The shortest of the estimated times, in us: a fixed part, the rounds of workgroups that
+// the chip holds, each with a part of its own and what its keys take, and for parts the second launch and the sums' way through
+// memory.  Fitted to 2780 calls of 320 shapes (1 to 64 rows, 1 to 30000 keys, 1 to 64 heads over 1 to 8 key heads of 64 to 256, all
+// kinds of cache), which they meet within 10 % on average: the way taken is 1 % over the best of those measured on average, 27 % at
+// most.  A workgroup a row and key head / shared keys, each in its best number of parts: 1 row of 48 heads over 8 of 128 on 18168 4-bit
+// keys 15 / 22, 10 rows of 12 heads over 2 of 64 on 62 5.8 / 7.1, 13 rows of 6 over 2 of 256 on 13892 fp16 keys 46 / 22, 59 rows
+// of 24 over 4 of 128 on 11138 113 / 32.
+struct TreeCall {
+  uint64_t rows, keys, heads, kv_heads, head_dim, padded;   // keys: that a row sees at most; padded: the head size, 64, 128 or 256
+  bool fp32, quantized;
+  bool by_rows, shared;                                     // which ways the call can take
+};
+struct TreeShape {
+  bool tile;
+  uint64_t parts;
+};
+constexpr uint64_t tree_units(const TreeCall& a, bool tile) {
+  const uint64_t group = a.heads / a.kv_heads, each = a.fp32 ? 16 : 8;
+  return tile ? (a.rows * group + 63) / 64 * a.kv_heads : a.rows * a.kv_heads * ((group + each - 1) / each);
+}
+constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_parts, size_t most_bytes) {
+  // at_once: workgroups a CU; whole: a round takes its time however few it holds (one workgroup fills the CU), else what it holds
+  struct Times {
+    double fixed, round, keys, quantized, at_once, parts, megabyte;
+    bool whole;
+  };
+  constexpr Times kRows[3] = {{4.7, 0.48, 0.0056, 1.23, 0.81, 2.6, 3.0, false}, {3.5, 2.76, 0.0089, 1.04, 0.76, 2.6, 1.1, false}, {2.35, 6.2, 0.0196, 1.02, 1.0, 3.2, 1.96, true}};
+  constexpr Times kRowsF32[3] = {{4.7, 0.0, 0.013, 1.0, 0.66, 2.6, 2.6, false}, {5.0, 0.9, 0.0242, 1.0, 0.82, 3.6, 3.0, false}, {0.4, 8.6, 0.0511, 1.0, 1.07, 4.1, 3.5, false}};
+  constexpr Times kTiles[3] = {{4.85, 0.27, 0.706, 1.36, 2.0, 3.0, 1.77, true}, {3.42, 2.55, 0.93, 1.35, 1.0, 3.05, 1.08, true}, {2.3, 5.6, 1.41, 1.29, 1.0, 4.3, 0.89, true}};
+  const int size = a.padded == 64 ? 0 : a.padded == 128 ? 1 : 2;
+  TreeShape best{a.shared && !a.by_rows, 1};
+  double least = -1.0;
+  for (int tile = 0; tile < 2; ++tile) {
+    if (tile != 0 ? !a.shared : !a.by_rows) continue;
+    const Times& t = tile != 0 ? kTiles[size] : a.fp32 ? kRowsF32[size] : kRows[size];
+    const uint64_t units = tree_units(a, tile != 0);
+    const double slots = static_cast<double>(cus) * t.at_once;
+    const uint64_t fill = static_cast<uint64_t>(slots) / units;        // parts that fill the chip
+    for (uint64_t parts : {uint64_t{1}, uint64_t{2}, uint64_t{3}, uint64_t{4}, uint64_t{6}, uint64_t{8}, uint64_t{12}, uint64_t{16}, uint64_t{24}, uint64_t{32}, uint64_t{48},
+                           uint64_t{64}, fill}) {
+      if (parts == 0 || (parts > 1 && (parts > most_parts || a.keys / parts < 48 || attention_parts_size(a.rows, a.heads, a.head_dim, parts) > most_bytes))) continue;
+      const uint64_t each = (a.keys + parts - 1) / parts, groups = units * parts;
+      double rounds = static_cast<double>(groups) / slots;
+      if (t.whole) rounds = static_cast<double>((groups + static_cast<uint64_t>(slots) - 1) / static_cast<uint64_t>(slots));
+      double us = t.fixed + (rounds < 1.0 ? 1.0 : rounds) * (t.round + t.keys * (a.quantized ? t.quantized : 1.0) * static_cast<double>(tile != 0 ? (each + 63) / 64 : each));
+      if (parts > 1) us += t.parts + t.megabyte * static_cast<double>(a.rows * a.heads * parts * a.head_dim * 4) * 1e-6;
+      if (least < 0.0 || us < least) least = us, best = TreeShape{tile != 0, parts};
+    }
+  }
+  return best;
+}
+
 // ---- "attention_combine" ---------------------------------------------------------------------------------------------
 // Wavefronts of a (row, head): sixteen where there are few and many parts, four where the rows fill the chip by themselves or
 // sixteen parts are all that there are, one where its four are and that does not make a lane's run long with few rows (us, 1 /

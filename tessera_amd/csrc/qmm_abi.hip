@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "qmm_kernels.hpp"
+#include "launch_rules.hpp"
 #include "stream_scratch.hpp"
 #include "tree_args.hpp"
 
@@ -1485,14 +1486,14 @@ qmm_status run_attention_tree_kind(const LaunchCtx& c, bool quantized, uint32_t 
   if (!quantized) kind = static_cast<uint32_t>(c.sc[7]);
   const uint64_t m = c.sc[0], n = c.sc[1], heads = c.sc[2], kv_heads = c.sc[3], head_dim = c.sc[4], tree = c.sc[5], window = c.sc[6];
   const size_t at = quantized ? 5 : 3;
-  auto go = [&](const qmm::TreePlan& plan, void* scratch) {
+  auto go = [&](const qmm::TreeShape& plan, void* scratch) {
     return map_hip(qmm::launch_attention_tree(kind, c.ptr<const float>(0), c.ptr<const void>(1), c.ptr<const void>(2),
                                               quantized ? c.ptr<const float>(3) : nullptr, quantized ? c.ptr<const float>(4) : nullptr,
                                               c.ptr<const uint32_t>(at), c.ptr<float>(at + 1), m, n, heads, kv_heads, head_dim, tree, window,
                                               plan, scratch, c.stream));
   };
-  auto plan = [&](uint64_t most) { return qmm::attention_tree_plan(kind, m, n, heads, kv_heads, head_dim, window, c.buf[at + 1], most); };
-  const qmm::TreePlan in_parts = plan(64);
+  auto plan = [&](uint64_t most) { return qmm::attention_tree_shape(kind, m, n, heads, kv_heads, head_dim, window, c.buf[at + 1], most); };
+  const qmm::TreeShape in_parts = plan(64);
   if (in_parts.parts > 1) {
     const StreamBlock block(c, qmm::attention_parts_bytes(m, heads, head_dim, in_parts.parts), g_parts_scratch);
     if (block.get() != nullptr) return go(in_parts, block.get());

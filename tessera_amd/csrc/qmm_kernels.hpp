@@ -261,18 +261,15 @@ hipError_t launch_attention_split(const float* q, const void* k, const void* v, 
                                   bool causal, uint64_t split, hipStream_t stream);
 hipError_t launch_attention_combine(const float* pacc, const float* pmax, const float* psum, float* out, uint64_t m,
                                     uint64_t heads, uint64_t head_dim, uint64_t split, hipStream_t stream);
-// The tree forms (tree_args.hpp: their calls).  TreePlan: whether rows share keys, and the parts of the keys, at most
-// `most_parts`, whose sums attention_parts_bytes of `scratch` hold where there are two or more.
+// The tree forms (tree_args.hpp: their calls).  attention_tree_shape: whether rows share keys, and the parts of the keys, at
+// most `most_parts`, whose sums attention_parts_bytes of `scratch` hold where there are two or more (launch_rules.hpp).
 struct QkNormCall;
-struct TreePlan {
-  bool tile;
-  uint64_t parts;
-};
-TreePlan attention_tree_plan(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
-                             uint64_t window, const void* out, uint64_t most_parts);
+struct TreeShape;
+TreeShape attention_tree_shape(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
+                               uint64_t window, const void* out, uint64_t most_parts);
 hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
                                  const uint32_t* mask, float* out, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads,
-                                 uint64_t head_dim, uint64_t tree, uint64_t window, const TreePlan& plan, void* scratch, hipStream_t stream);
+                                 uint64_t head_dim, uint64_t tree, uint64_t window, const TreeShape& shape, void* scratch, hipStream_t stream);
 hipError_t launch_tree_mask(const uint32_t* parents, uint32_t* mask, uint64_t* positions, uint32_t nodes, uint64_t base, hipStream_t stream);
 // pos3 null: positions pos_base + row; gate null: none.
 hipError_t launch_qk_norm_rope(const QkNormCall& call, const float* q, const float* k, const float* wq, const float* wk, const uint64_t* pos3,
