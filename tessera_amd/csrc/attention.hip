@@ -3,6 +3,19 @@
 #include "attention_kernels.hpp"
 
 namespace qmm {
+namespace {
+
+hipError_t launch_attention_as(uint32_t kind, const AttentionArgs& a, uint64_t m, hipStream_t stream) {
+  return with_kind(kind, [&](auto tag) {
+    constexpr KvKind KV = decltype(tag)::value;
+    if (runs_fit<KV>(a.head_dim)) return launch_rows<KV>(a, m, stream);
+    const uint64_t parts = a.part.split == 0 ? 1 : a.part.split;
+    hipLaunchKernelGGL(attention_any_kernel<KV>, dim3(static_cast<uint32_t>(m * a.heads * parts)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+  });
+}
+
+}  // namespace
 
 uint64_t attention_parts(uint32_t kind, uint64_t m, uint64_t n, uint64_t heads, uint64_t kv_heads, uint64_t head_dim,
                          uint64_t q_base, uint64_t window, bool causal, const void* out, uint64_t most_parts) {

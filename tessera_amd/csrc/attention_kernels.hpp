@@ -70,6 +70,19 @@ __device__ __forceinline__ uint32_t tree_keys(const AttentionArgs& a, const uint
   return shift == 0u ? low : low >> shift | high << (32u - shift);
 }
 
+// Pair c of a key head's (row, head) pairs, `group` to a row: its row, and its place among all pairs (fewer than 2^24).
+struct TreePair {
+  uint32_t row, at;
+};
+__device__ __forceinline__ TreePair tree_pair(const AttentionArgs& a, uint32_t kv, uint32_t c) {
+  const uint32_t group = a.heads / a.kv_heads, row = c / group;
+  return TreePair{row, row * a.heads + kv * group + (c - row * group)};
+}
+// What attend_row has besides for pairs: their places, and whether a result is not finite.
+struct TreeRows {
+  uint32_t at[16], special;
+};
+
 // Keys [start, last] that query row i sees (TREE: in which those lie that it sees; start > last: none).
 template <bool TREE = false>
 __device__ __forceinline__ void key_range(const AttentionArgs& a, uint64_t i, uint64_t& start, uint64_t& last) {
@@ -258,9 +271,13 @@ __device__ __forceinline__ void empty_part(const AttentionArgs& a, uint64_t row,
 
 // Heads head0 .. head0 + here - 1 (at most rows_heads, all of key head kv) of query row `row` over keys start .. last:
 // part s_part of the row, or all of it.  KEYS: keys a tile, 16 where the registers of 32 are not to be had.
+// TREE: the pairs row .. row + here - 1 of the (row, head) pairs of key head kv instead, whose rows each see the keys that
+// their bits and the window leave them; infinities and NaN are not kept apart, a result that is not finite sets `special`.  `at` is
+// read behind the barrier of the merge.
 template <KvKind KV, int DP, int NW, int KEYS = KV == KvKind::F32 ? 16 : 32, bool TREE = false>
 __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row, uint32_t kv, uint32_t head0, uint32_t here,
-                                           uint64_t start, uint64_t last, uint64_t s_part, RowsShared<KV, DP, NW>& merge) {
+                                           uint64_t start, uint64_t last, uint64_t s_part, RowsShared<KV, DP, NW>& merge,
+                                           TreeRows* pairs = nullptr) {
   constexpr bool F32 = KV == KvKind::F32, QUANT = kv_quantized(KV);
   constexpr int BITS = kv_bits(KV);
   constexpr int CE = F32 ? 4 : 128 / BITS < DP / 4 ? 128 / BITS : DP / 4;   // elements of a key a lane loads at once
@@ -341,7 +358,20 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
     const half2_t lo = {static_cast<_Float16>(low_x), static_cast<_Float16>(low_y)};
     return bit_cast<half2_t>(second ? bit_cast<uint32_t>(lo) : bit_cast<uint32_t>(hi));
   };
-  const float* qp = a.q + ((a.row_base + row) * a.heads + head0 + (column_head < here ? column_head : here - 1u)) * D;
+  const float* qp = nullptr;
+  const uint32_t* bits = nullptr;
+  uint64_t own_start = 0;
+  if constexpr (TREE) {
+    const TreePair own = tree_pair(a, kv, static_cast<uint32_t>(row) + (column_head < here ? column_head : here - 1u));
+    qp = a.q + static_cast<uint64_t>(own.at) * D;
+    bits = a.mask + static_cast<uint64_t>(own.row) * a.words;
+    if (a.window != 0) {
+      uint64_t own_last;
+      key_range<true>(a, own.row, own_start, own_last);
+    }
+  } else {
+    qp = a.q + ((a.row_base + row) * a.heads + head0 + (column_head < here ? column_head : here - 1u)) * D;
+  }
   float qf[F32 ? STEPS : 1];
   half8_t qh[F32 ? 1 : STEPS];
   // A column's scores are kept as the matrix instructions leave them, s; score_scale s is in units of log2.  Only
@@ -386,6 +416,15 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
   float lane_most = 0.0f, value_up = F32 ? 1.0f : QUANT ? power_of_two_to(0.0f, 14) : 0x1p14f;
   for (uint64_t j0 = first; j0 <= last; j0 += NW * KEYS) {
     const bool more = j0 + NW * KEYS <= last;
+    // TREE: what each row sees of this tile, where that may not be all of it.
+    const bool hides = TREE && (j0 + KEYS > a.n - a.tree || (a.window != 0 && __any(own_start > j0)));
+    uint32_t shown = ~0u;
+    if constexpr (TREE) {
+      if (hides) {
+        shown = tree_keys(a, bits, j0);
+        if (own_start > j0) shown = own_start - j0 < 32u ? shown & ~0u << (own_start - j0) : 0u;
+      }
+    }
     float s[4 * HALVES];
 #pragma unroll
     for (int h = 0; h < HALVES; ++h) {
@@ -439,12 +478,7 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
         }
       }
     }
-    // The range ends inside this tile (TREE: or some of it may be hidden from the row).
-    const bool past = j0 + KEYS - 1 > last || (TREE && j0 + KEYS > a.n - a.tree);
-    uint32_t shown = ~0u;
-    if constexpr (TREE) {
-      if (past) shown = tree_keys(a, a.mask + row * a.words, j0);
-    }
+    const bool past = j0 + KEYS - 1 > last || hides;   // the range ends inside this tile
     if (past) {
 #pragma unroll
       for (int e = 0; e < 4 * HALVES; ++e) {
@@ -502,13 +536,13 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
         for (int e = 0; e < 4; ++e) o[j][e] *= corr;
       }
     }
-    if constexpr (!QUANT || (TREE && KV == KvKind::Fp8)) {
+    if constexpr (!QUANT) {
       // Rows past the range's end stand for no key: infinite elements of the one read in their place would
-      // not vanish under the weight 0 (nor would a hidden key's E4M3 codes that are NaN).
+      // not vanish under the weight 0.
       if (past) {
 #pragma unroll
         for (int e = 0; e < 4 * HALVES; ++e) {
-          const bool none = j0 + 16 * (e / 4) + 4 * g + e % 4 > last || (TREE && (shown >> (16 * (e / 4) + 4 * g + e % 4) & 1u) == 0u);
+          const bool none = j0 + 16 * (e / 4) + 4 * g + e % 4 > last;
 #pragma unroll
           for (int w = 0; w < VW; ++w) vr[e][w] = none ? 0u : vr[e][w];
         }
@@ -578,20 +612,21 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
       sum = fmaf(__builtin_amdgcn_exp2f((merge.m[w][h] - m_ref) * scale), merge.l[w][h], sum);
       acc += merge.o[w][h][d / VE][d % VE];
     }
+    if (TREE && !(fabsf(acc) < INFINITY && fabsf(sum) < INFINITY)) pairs->special = 1u;
     if (a.part.split != 0) {
-      const uint64_t at = (row * a.heads + head0 + h) * split + s_part;
+      const uint64_t at = (TREE ? static_cast<uint64_t>(pairs->at[h]) : row * a.heads + head0 + h) * split + s_part;
       // The part's largest score in natural units is rounded; the sums move by what that took from it.
       const float natural = scale * kLn2, largest = m * natural;
       const float moved = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(m, natural, -largest) * kLog2E);
       a.part.pacc[at * D + d] = acc * moved;
       if (d == 0) a.part.pmax[at] = largest, a.part.psum[at] = sum * moved;
     } else {
-      a.out[((a.row_base + row) * a.heads + head0 + h) * D + d] = TREE && sum == 0.0f ? 0.0f : acc / sum;
+      a.out[(TREE ? static_cast<uint64_t>(pairs->at[h]) : (a.row_base + row) * a.heads + head0 + h) * D + d] = TREE && sum == 0.0f ? 0.0f : acc / sum;
     }
   }
 }
 
-template <KvKind KV, int DP, int NW, bool TREE = false>
+template <KvKind KV, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void attention_rows_kernel(AttentionArgs a) {
   constexpr uint32_t kHeads = rows_heads<KV>();
   __shared__ RowsShared<KV, DP, NW> merge;
@@ -602,12 +637,12 @@ __global__ __launch_bounds__(NW * 64, 1) void attention_rows_kernel(AttentionArg
   const uint32_t head0 = kv * group + first, here = group - first < kHeads ? group - first : kHeads;
   const uint64_t row = row_kv / a.kv_heads, s_part = blockIdx.x % split;
   uint64_t start, last;
-  key_range<TREE>(a, row, start, last);
+  key_range(a, row, start, last);
   if (a.part.split != 0 && !key_chunk(a, s_part, start, last)) {   // workgroup-uniform
     empty_part<NW * 64>(a, row, head0, here, s_part);
     return;
   }
-  attend_row<KV, DP, NW, KV == KvKind::F32 ? 16 : 32, TREE>(a, row, kv, head0, here, start, last, s_part, merge);
+  attend_row<KV, DP, NW>(a, row, kv, head0, here, start, last, s_part, merge);
 }
 
 // ---- many query rows: a workgroup shares its keys among 64 (row, head) pairs ---------------------
@@ -1279,13 +1314,9 @@ __global__ __launch_bounds__(WAVES * 64) void attention_combine_kernel(const flo
 
 // ---- dispatch ------------------------------------------------------------------------------------
 
-template <KvKind KV, bool TREE = false>
-hipError_t launch_rows(const AttentionArgs& a, uint64_t m, hipStream_t stream) {
-  constexpr uint32_t kHeads = KV == KvKind::F32 ? 16 : 8;
-  const uint32_t group = a.heads / a.kv_heads, blocks = (group + kHeads - 1) / kHeads;
+template <KvKind KV, class Go>
+hipError_t with_waves(const AttentionArgs& a, uint64_t workgroups, Go&& go) {
   const uint64_t split = a.part.split == 0 ? 1 : a.part.split;
-  const uint64_t workgroups = m * a.kv_heads * blocks * split;
-  const dim3 grid(static_cast<uint32_t>(workgroups));
   // Four wavefronts a workgroup take 128 keys at once; where a workgroup has more to do and the registers and the size of a
   // grid allow it, eight; with no more workgroups than CUs, five take the 129 to 160 keys that parts of 128 come to where they
   // do not divide the keys, and spare a time round (us, four / five: int8, 1200 keys in 9 parts, 4 key heads of 128 8.6 /
@@ -1295,17 +1326,25 @@ hipError_t launch_rows(const AttentionArgs& a, uint64_t m, hipStream_t stream) {
   const uint64_t each = (a.n + split - 1) / split;
   const bool wide = a.n / split > 160 && workgroups < kMaxGridThreads / 512u;
   const bool five = each > 128 && each <= (KV == KvKind::F32 ? 144 : 160) && workgroups <= static_cast<uint64_t>(num_cus());
-  auto go = [&](auto kernel, uint32_t waves) { hipLaunchKernelGGL(kernel, grid, dim3(waves * 64u), 0, stream, a); };
   auto pick = [&](auto dim) {
     constexpr int DP = decltype(dim)::value;
-    if (DP < 256 && five) go(attention_rows_kernel<KV, DP, DP < 256 ? 5 : 4, TREE>, 5);
-    else if (DP < 256 && wide) go(attention_rows_kernel<KV, DP, DP < 256 ? 8 : 4, TREE>, 8);
-    else go(attention_rows_kernel<KV, DP, 4, TREE>, 4);
+    if (DP < 256 && five) go(dim, std::integral_constant<int, DP < 256 ? 5 : 4>{});
+    else if (DP < 256 && wide) go(dim, std::integral_constant<int, DP < 256 ? 8 : 4>{});
+    else go(dim, std::integral_constant<int, 4>{});
   };
   if (a.head_dim <= 64) pick(std::integral_constant<int, 64>{});
   else if (a.head_dim <= 128) pick(std::integral_constant<int, 128>{});
   else pick(std::integral_constant<int, 256>{});
   return hipGetLastError();
+}
+template <KvKind KV>
+hipError_t launch_rows(const AttentionArgs& a, uint64_t m, hipStream_t stream) {
+  const uint32_t group = a.heads / a.kv_heads, blocks = (group + rows_heads<KV>() - 1) / rows_heads<KV>();
+  const uint64_t workgroups = m * a.kv_heads * blocks * (a.part.split == 0 ? 1 : a.part.split);
+  return with_waves<KV>(a, workgroups, [&](auto dim, auto waves) {
+    hipLaunchKernelGGL((attention_rows_kernel<KV, decltype(dim)::value, decltype(waves)::value>), dim3(static_cast<uint32_t>(workgroups)),
+                       dim3(decltype(waves)::value * 64u), 0, stream, a);
+  });
 }
 
 // The runs that the lanes of the matrix kernels load divide a head's row: 16 bytes of a key (a quarter of the padded
@@ -1339,17 +1378,6 @@ auto with_kind(uint32_t kind, Go&& go) {
     case 3: return go(std::integral_constant<KvKind, KvKind::Q4>{});
     default: return go(std::integral_constant<KvKind, KvKind::Fp8>{});
   }
-}
-
-template <bool TREE = false>
-hipError_t launch_attention_as(uint32_t kind, const AttentionArgs& a, uint64_t m, hipStream_t stream) {
-  return with_kind(kind, [&](auto tag) {
-    constexpr KvKind KV = decltype(tag)::value;
-    if (runs_fit<KV>(a.head_dim)) return launch_rows<KV, TREE>(a, m, stream);
-    const uint64_t parts = a.part.split == 0 ? 1 : a.part.split;
-    hipLaunchKernelGGL((attention_any_kernel<KV, TREE>), dim3(static_cast<uint32_t>(m * a.heads * parts)), dim3(256), 0, stream, a);
-    return hipGetLastError();
-  });
 }
 
 AttentionArgs args_of(const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale, float* out,

@@ -49,24 +49,31 @@ __device__ __forceinline__ void load_run(__amdgpu_buffer_rsrc_t from, uint32_t o
   }
 }
 
-// One (row, head) pair over keys start .. last, in fp32 by 512 threads: where infinities or NaN keep the matrix instructions
-// from it.  Keys 64 at a time, a wavefront's lanes along head_dim for a score, two threads an element of the sum.
+// (row, head) pair `pair` over the keys of start .. last that its row sees, in fp32 by THREADS threads (256 at least): where
+// infinities or NaN keep the matrix instructions from it.  Keys 64 at a time, a wavefront's lanes along head_dim for a score, a
+// thread or two an element of the sum.
 struct PairShared {
   float score[64], weight[64], sum[512];
 };
-template <KvKind KV>
-__device__ __forceinline__ void attend_pair(const AttentionArgs& a, uint32_t row, uint32_t head, uint32_t kv, uint64_t start, uint64_t last,
-                                            uint32_t s_part, PairShared& sh) {
+template <KvKind KV, uint32_t THREADS>
+__device__ __forceinline__ void attend_pair(const AttentionArgs& a, TreePair which, uint32_t kv, uint64_t start, uint64_t last, uint32_t s_part,
+                                            PairShared& sh) {
+  constexpr uint32_t kHalves = THREADS / 256u, kWaves = THREADS / 64u;
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, D = a.head_dim, e = t & 255u, half = t >> 8;
-  const uint64_t pair = static_cast<uint64_t>(row) * a.heads + head;
-  const uint32_t* bits = a.mask + static_cast<uint64_t>(row) * a.words;
+  const uint64_t pair = which.at;
+  const uint32_t* bits = a.mask + static_cast<uint64_t>(which.row) * a.words;
+  {
+    uint64_t row_start, row_last;
+    key_range<true>(a, which.row, row_start, row_last);
+    start = row_start > start ? row_start : start;
+  }
   const float scale = 1.0f / sqrtf(static_cast<float>(D));
   float run_max = -INFINITY, run_sum = 0.0f, acc = 0.0f;
   for (uint64_t j0 = start; j0 <= last; j0 += 64u) {
     const uint32_t count = last - j0 < 63u ? static_cast<uint32_t>(last - j0) + 1u : 64u;
     const uint32_t low = tree_keys(a, bits, j0), high = count > 32u ? tree_keys(a, bits, j0 + 32u) : 0u;
     auto sees = [&](uint32_t k) { return k < count && ((k < 32u ? low >> k : high >> (k - 32u)) & 1u) != 0u; };
-    for (uint32_t k = wave; k < 64u; k += 8u) {
+    for (uint32_t k = wave; k < 64u; k += kWaves) {
       float dot = 0.0f;
       if (sees(k)) {
         for (uint32_t d = lane; d < D; d += 64u) dot = fmaf(a.q[pair * D + d], cache_element<KV>(a.k, a.k_scale, j0 + k, ((j0 + k) * a.kv_heads + kv) * D + d), dot);
@@ -82,15 +89,17 @@ __device__ __forceinline__ void attend_pair(const AttentionArgs& a, uint32_t row
     run_max = most;
     __syncthreads();
     float x = 0.0f;
-    for (uint32_t k = half; k < count && e < D; k += 2u) {
+    for (uint32_t k = half; k < count && e < D && half < kHalves; k += kHalves) {
       if (sees(k)) x = fmaf(sh.weight[k], cache_element<KV>(a.v, a.v_scale, j0 + k, ((j0 + k) * a.kv_heads + kv) * D + e), x);
     }
     acc = fmaf(corr, acc, x);
   }
-  sh.sum[t] = acc;
+  if constexpr (kHalves == 2) {
+    if (half < 2u) sh.sum[t] = acc;
+  }
   __syncthreads();
   if (t < D) {
-    const float x = acc + sh.sum[t + 256u];
+    const float x = kHalves == 2 ? acc + sh.sum[t + 256u] : acc;
     if (a.part.split != 0) a.part.pacc[(pair * a.part.split + s_part) * D + t] = x;
     else a.out[pair * D + t] = run_sum == 0.0f ? 0.0f : x / run_sum;
   }
@@ -461,12 +470,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   // workgroup's columns are done again one by one.
   if (__builtin_amdgcn_readfirstlane(sh.special) != 0u) {          // workgroup-uniform
     __syncthreads();
-    for (uint32_t c = c0; c < c_end; ++c) {
-      uint64_t row_start, row_last;
-      key_range<true>(a, c / group, row_start, row_last);
-      row_start = row_start > wg_start ? row_start : wg_start, row_last = row_last < wg_last ? row_last : wg_last;
-      attend_pair<KV>(a, c / group, kv * group + c % group, kv, row_start, row_last, s_part, *reinterpret_cast<PairShared*>(sh.stage[0]));
-    }
+    for (uint32_t c = c0; c < c_end; ++c) attend_pair<KV, 512>(a, tree_pair(a, kv, c), kv, wg_start, wg_last, s_part, *reinterpret_cast<PairShared*>(sh.stage[0]));
     return;
   }
   if (c0 + own_at >= c_end) return;
@@ -487,6 +491,64 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     const uint32_t d = (half * VH + j) * 16u + late_g * 4u;
     if (d < D) *reinterpret_cast<float4_t*>(out + d) = merged[j] * factor;
   }
+}
+
+// ---- few pairs a workgroup: eight at most, sixteen over an fp32 cache -------------------------------------------------------
+//
+// attend_row with `each` (row, head) pairs in place of a row's heads, so that a key is read once for all of them.  Over fp32 keys,
+// which the kernel above does not take, 64 rows of 24 heads over 4 of 256 on 8192 keys are 220 us by sixteen pairs and 428 by a
+// row's heads, 59 Tflop/s where fp32 matrix instructions do 157 at most; few keys are the other way round, 46 rows
+// of 8 heads over 1 of 128 on 52 9.4 by pairs and 7.6 by rows, as the sums of sixteen are merged.
+// The shortest calls are a launch and its latencies: 10 rows of 12 heads over 2 of 64 on 62 fp16 keys 7.0 us (an empty launch
+// among others 3.5).
+template <KvKind KV, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 1) void attention_pairs_kernel(AttentionArgs a, uint32_t each) {
+  union Lds {
+    RowsShared<KV, DP, NW> merge;
+    PairShared pair;
+    __device__ Lds() {}
+  };
+  __shared__ Lds lds;
+  __shared__ TreeRows rows;
+  const uint32_t t = threadIdx.x, split = a.part.split == 0 ? 1u : static_cast<uint32_t>(a.part.split);
+  const uint32_t kv = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads, s_part = unit % split;
+  const uint32_t pairs = static_cast<uint32_t>(a.rows) * (a.heads / a.kv_heads), first = unit / split * each;
+  const uint32_t here = pairs - first < each ? pairs - first : each;
+  if (t < here) rows.at[t] = tree_pair(a, kv, first + t).at;
+  if (t == 0u) rows.special = 0u;
+  // From the earliest key that a row sees.
+  uint64_t start = 0, last = a.n - 1;
+  if (a.window != 0 || a.n == a.tree) {
+    const uint32_t own = t % 16u;
+    uint64_t row_last;
+    key_range<true>(a, tree_pair(a, kv, first + (own < here ? own : here - 1u)).row, start, row_last);
+#pragma unroll
+    for (uint32_t off = 8u; off > 0u; off >>= 1) {
+      const uint64_t other = __shfl_xor(static_cast<unsigned long long>(start), off, kWave);
+      start = other < start ? other : start;
+    }
+    start = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(start >> 32))) << 32 | __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(start));
+  }
+  if (a.part.split != 0 && !key_chunk(a, s_part, start, last)) {   // workgroup-uniform
+    for (uint32_t i = 0; i < here; ++i) {
+      const TreePair pair = tree_pair(a, kv, first + i);
+      empty_part<NW * 64>(a, pair.row, pair.at - pair.row * a.heads, 1, s_part);
+    }
+    return;
+  }
+  attend_row<KV, DP, NW, KV == KvKind::F32 ? 16 : 32, true>(a, first, kv, 0, here, start, last, s_part, lds.merge, &rows);
+  __syncthreads();
+  if (__builtin_amdgcn_readfirstlane(rows.special) == 0u) return;       // workgroup-uniform
+  for (uint32_t i = 0; i < here; ++i) attend_pair<KV, NW * 64>(a, tree_pair(a, kv, first + i), kv, start, last, s_part, lds.pair);
+}
+
+template <KvKind KV>
+hipError_t launch_pairs(const AttentionArgs& a, uint64_t each, hipStream_t stream) {
+  const uint64_t workgroups = (a.rows * (a.heads / a.kv_heads) + each - 1) / each * a.kv_heads * (a.part.split == 0 ? 1 : a.part.split);
+  return with_waves<KV>(a, workgroups, [&](auto dim, auto waves) {
+    hipLaunchKernelGGL((attention_pairs_kernel<KV, decltype(dim)::value, decltype(waves)::value>), dim3(static_cast<uint32_t>(workgroups)),
+                       dim3(decltype(waves)::value * 64u), 0, stream, a, static_cast<uint32_t>(each));
+  });
 }
 
 template <KvKind KV>
@@ -513,7 +575,7 @@ TreeShape attention_tree_shape(uint32_t kind, uint64_t m, uint64_t n, uint64_t h
   if (parts > call.keys / 128) parts = call.keys / 128;
   if (parts > most_parts) parts = most_parts;
   while (parts > 1 && attention_parts_size(m, heads, head_dim, parts) > kAttentionPartsMost) --parts;
-  return TreeShape{false, parts < 2 ? 1 : parts};
+  return TreeShape{false, 1, parts < 2 ? 1 : parts};
 }
 
 hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, const void* v, const float* k_scale, const float* v_scale,
@@ -527,9 +589,14 @@ hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, c
     float* most = acc + m * heads * parts * head_dim;
     a.part = SplitOut{acc, most, most + m * heads * parts, parts};
   }
-  const hipError_t e = !shape.tile ? launch_attention_as<true>(kind, a, m, stream) : with_kind(kind, [&](auto tag) {
-    if constexpr (decltype(tag)::value == KvKind::F32) return hipErrorInvalidValue;
-    else return launch_tree_tiles<decltype(tag)::value>(a, stream);
+  const hipError_t e = with_kind(kind, [&](auto tag) {
+    constexpr KvKind KV = decltype(tag)::value;
+    if constexpr (KV != KvKind::F32) {
+      if (shape.tile) return launch_tree_tiles<KV>(a, stream);
+    }
+    if (runs_fit<KV>(a.head_dim)) return launch_pairs<KV>(a, shape.pairs, stream);
+    hipLaunchKernelGGL((attention_any_kernel<KV, true>), dim3(static_cast<uint32_t>(m * heads * (parts < 2 ? 1 : parts))), dim3(256), 0, stream, a);
+    return hipGetLastError();
   });
   if (e != hipSuccess || parts <= 1) return e;
   return launch_combine<true>(a.part.pacc, a.part.pmax, a.part.psum, out, m, heads, head_dim, parts, stream);

@@ -224,43 +224,46 @@ constexpr uint64_t attention_rule(const AttentionCall& a, uint64_t cus, uint64_t
 }
 
 // ---- "attention_tree" ------------------------------------------------------------------------------------------------
-// How a call runs: a workgroup a row and key head (`tile` false), or 64 (row, head) pairs of a key head that share their keys, 64
-// at a time; and the parts of the keys.  The shortest of the estimated times, in us: a fixed part, the rounds of workgroups that
-// the chip holds, each with a part of its own and what its keys take, and for parts the second launch and the sums' way through
-// memory.  Fitted to 2780 calls of 320 shapes (1 to 64 rows, 1 to 30000 keys, 1 to 64 heads over 1 to 8 key heads of 64 to 256, all
-// kinds of cache), which they meet within 10 % on average: the way taken is 1 % over the best of those measured on average, 27 % at
-// most.  A workgroup a row and key head / shared keys, each in its best number of parts: 1 row of 48 heads over 8 of 128 on 18168 4-bit
-// keys 15 / 22, 10 rows of 12 heads over 2 of 64 on 62 5.8 / 7.1, 13 rows of 6 over 2 of 256 on 13892 fp16 keys 46 / 22, 59 rows
-// of 24 over 4 of 128 on 11138 113 / 32.
+// How a call runs: a workgroup a row and key head, at most eight heads (sixteen over fp32 keys); or sixteen (row, head) pairs of a
+// key head, fp32 keys only; or 64 that share their keys, 64 at a time (`tile`); and the parts of the keys.  The shortest of the
+// estimated times, in us: a fixed part, the rounds of workgroups that the chip holds, each with a part of its own and what its
+// keys take, and for parts the second launch and the sums' way through memory.  Fitted to 6290 calls of 580 shapes (1 to 64
+// rows, 1 to 30000 keys, 1 to 64 heads over 1 to 8 key heads of 64 to 256, all kinds of cache), which they meet within 10 % on
+// average: the way taken is 1.5 % over the best of those measured on average, 27 % at most.  A workgroup a row and key head /
+// shared keys, each in its best number of parts: 1 row of 48 heads over 8 of 128 on 18168 4-bit keys 15 / 22, 10 rows of 12 heads
+// over 2 of 64 on 62 5.8 / 7.1, 13 rows of 6 over 2 of 256 on 13892 fp16 keys 46 / 22, 59 rows of 24 over 4 of 128 on 11138
+// 113 / 32; / sixteen pairs, fp32 keys: 32 rows of 64 over 8 of 96 on 8224 214 / 113, 24 of 8 over 2 of 256 on 71 15 / 20.
 struct TreeCall {
   uint64_t rows, keys, heads, kv_heads, head_dim, padded;   // keys: that a row sees at most; padded: the head size, 64, 128 or 256
   bool fp32, quantized;
   bool by_rows, shared;                                     // which ways the call can take
 };
 struct TreeShape {
-  bool tile;
-  uint64_t parts;
+  bool tile;                                                // by the kernel of shared keys
+  uint64_t pairs, parts;                                    // (row, head) pairs a workgroup
 };
-constexpr uint64_t tree_units(const TreeCall& a, bool tile) {
-  const uint64_t group = a.heads / a.kv_heads, each = a.fp32 ? 16 : 8;
-  return tile ? (a.rows * group + 63) / 64 * a.kv_heads : a.rows * a.kv_heads * ((group + each - 1) / each);
+constexpr uint64_t tree_units(const TreeCall& a, uint64_t pairs) {
+  return (a.rows * (a.heads / a.kv_heads) + pairs - 1) / pairs * a.kv_heads;
 }
 constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_parts, size_t most_bytes) {
   // at_once: workgroups a CU; whole: a round takes its time however few it holds (one workgroup fills the CU), else what it holds
   struct Times {
     double fixed, round, keys, quantized, at_once, parts, megabyte;
     bool whole;
+    double pair = 0.0;
   };
   constexpr Times kRows[3] = {{4.7, 0.48, 0.0056, 1.23, 0.81, 2.6, 3.0, false}, {3.5, 2.76, 0.0089, 1.04, 0.76, 2.6, 1.1, false}, {2.35, 6.2, 0.0196, 1.02, 1.0, 3.2, 1.96, true}};
-  constexpr Times kRowsF32[3] = {{4.7, 0.0, 0.013, 1.0, 0.66, 2.6, 2.6, false}, {5.0, 0.9, 0.0242, 1.0, 0.82, 3.6, 3.0, false}, {0.4, 8.6, 0.0511, 1.0, 1.07, 4.1, 3.5, false}};
+  constexpr Times kRowsF32[3] = {{4.67, 0.36, 0.0129, 1.0, 0.83, 2.85, 1.43, false, 0.022}, {4.43, 1.74, 0.0247, 1.0, 0.81, 3.36, 1.86, false, 0.045}, {3.85, 4.78, 0.0515, 1.0, 0.71, 3.97, 1.55, false, 0.24}};
   constexpr Times kTiles[3] = {{4.85, 0.27, 0.706, 1.36, 2.0, 3.0, 1.77, true}, {3.42, 2.55, 0.93, 1.35, 1.0, 3.05, 1.08, true}, {2.3, 5.6, 1.41, 1.29, 1.0, 4.3, 0.89, true}};
   const int size = a.padded == 64 ? 0 : a.padded == 128 ? 1 : 2;
-  TreeShape best{a.shared && !a.by_rows, 1};
+  const uint64_t group = a.heads / a.kv_heads, fit = a.fp32 ? 16 : 8, own = group < fit ? group : fit;
+  TreeShape best{false, own, 1};
   double least = -1.0;
-  for (int tile = 0; tile < 2; ++tile) {
-    if (tile != 0 ? !a.shared : !a.by_rows) continue;
-    const Times& t = tile != 0 ? kTiles[size] : a.fp32 ? kRowsF32[size] : kRows[size];
-    const uint64_t units = tree_units(a, tile != 0);
+  for (uint64_t pairs : {own, uint64_t{16}, uint64_t{64}}) {
+    const bool tile = pairs == 64;
+    if (tile ? !a.shared : !a.by_rows || (pairs != own && (!a.fp32 || a.rows * group <= own))) continue;
+    const Times& t = tile ? kTiles[size] : a.fp32 ? kRowsF32[size] : kRows[size];
+    const uint64_t units = tree_units(a, pairs);
     const double slots = static_cast<double>(cus) * t.at_once;
     const uint64_t fill = static_cast<uint64_t>(slots) / units;        // parts that fill the chip
     for (uint64_t parts : {uint64_t{1}, uint64_t{2}, uint64_t{3}, uint64_t{4}, uint64_t{6}, uint64_t{8}, uint64_t{12}, uint64_t{16}, uint64_t{24}, uint64_t{32}, uint64_t{48},
@@ -269,9 +272,9 @@ constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_par
       const uint64_t each = (a.keys + parts - 1) / parts, groups = units * parts;
       double rounds = static_cast<double>(groups) / slots;
       if (t.whole) rounds = static_cast<double>((groups + static_cast<uint64_t>(slots) - 1) / static_cast<uint64_t>(slots));
-      double us = t.fixed + (rounds < 1.0 ? 1.0 : rounds) * (t.round + t.keys * (a.quantized ? t.quantized : 1.0) * static_cast<double>(tile != 0 ? (each + 63) / 64 : each));
+      double us = t.fixed + (rounds < 1.0 ? 1.0 : rounds) * (t.round + t.pair * static_cast<double>(pairs) + t.keys * (a.quantized ? t.quantized : 1.0) * static_cast<double>(tile ? (each + 63) / 64 : each));
       if (parts > 1) us += t.parts + t.megabyte * static_cast<double>(a.rows * a.heads * parts * a.head_dim * 4) * 1e-6;
-      if (least < 0.0 || us < least) least = us, best = TreeShape{tile != 0, parts};
+      if (least < 0.0 || us < least) least = us, best = TreeShape{tile, pairs, parts};
     }
   }
   return best;

@@ -9,7 +9,7 @@ from test_kernel_resources import HIPCC, resource_remarks
 @pytest.mark.skipif(shutil.which(HIPCC) is None, reason="hipcc not found")
 def test_no_scratch_memory():
     kernels = resource_remarks("attention_tree.hip")
-    for want in ("attention_rows_kernel", "attention_tree_kernel"):
+    for want in ("attention_pairs_kernel", "attention_tree_kernel"):
         hits = {k: v for k, v in kernels.items() if want in k}
         assert hits
         for name, res in hits.items():

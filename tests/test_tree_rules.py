@@ -16,7 +16,8 @@ def test_tree_rule(tmp_path):
     CHECK(s.tile ? call.shared : call.by_rows, "%zu rows", static_cast<size_t>(rows));
     CHECK(s.parts >= 1 && s.parts <= most, "%zu parts", static_cast<size_t>(s.parts));
     CHECK(s.parts == 1 || (keys / s.parts >= 48 && attention_parts_size(rows, kv * group, d, s.parts) <= bytes), "%zu parts", static_cast<size_t>(s.parts));
-    CHECK(tree_units(call, s.tile) >= 1, "units");
+    CHECK(s.tile ? s.pairs == 64 : s.pairs >= 1 && s.pairs <= (call.fp32 ? 16 : 8), "%zu pairs", static_cast<size_t>(s.pairs));
+    CHECK(tree_units(call, s.pairs) >= 1 && tree_units(call, s.pairs) * s.pairs >= rows * kv * group, "units");
   }
   CHECK(tiles > calls / 4 && tiles < calls * 3 / 4 && parted > calls / 8, "%d of %d, %d", tiles, calls, parted);
 """)
