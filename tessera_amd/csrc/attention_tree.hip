@@ -49,6 +49,13 @@ __device__ __forceinline__ void load_run(__amdgpu_buffer_rsrc_t from, uint32_t o
   }
 }
 
+// A value the compiler takes for a new one: what is needed only now and then or after the walk over the keys is formed from
+// the thread's number or the head size again, not held, where the registers are just enough.
+__device__ __forceinline__ uint32_t again(uint32_t v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // (row, head) pair `pair` over the keys of start .. last that its row sees, in fp32 by THREADS threads (256 at least): where
 // infinities or NaN keep the matrix instructions from it.  Keys 64 at a time, a wavefront's lanes along head_dim for a score, a
 // thread or two an element of the sum.
@@ -67,7 +74,7 @@ __device__ __forceinline__ void attend_pair(const AttentionArgs& a, TreePair whi
     key_range<true>(a, which.row, row_start, row_last);
     start = row_start > start ? row_start : start;
   }
-  const float scale = 1.0f / sqrtf(static_cast<float>(D));
+  const float scale = 1.0f / sqrtf(static_cast<float>(again(D)));
   float run_max = -INFINITY, run_sum = 0.0f, acc = 0.0f;
   for (uint64_t j0 = start; j0 <= last; j0 += 64u) {
     const uint32_t count = last - j0 < 63u ? static_cast<uint32_t>(last - j0) + 1u : 64u;
@@ -127,19 +134,14 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   const uint32_t columns = static_cast<uint32_t>(a.rows * group);
   const uint32_t c0 = unit / split * 64u;
   const uint32_t c_end = c0 + 64u < columns ? c0 + 64u : columns;
-  // A value the compiler takes for a new one: what is needed only now and then or after the walk over the keys is formed
-  // from the thread's number again, not held, where the registers are just enough.
-  auto again = [](uint32_t v) {
-    asm volatile("" : "+v"(v));
-    return v;
-  };
   // A lane's column of the workgroup's, past the last one the last.
   struct Column {
     uint32_t row, head;
   };
   auto column = [&](uint32_t thread) {
     const uint32_t at = c0 + col_group * 16u + (thread & 15u), col = at < c_end ? at : c_end - 1u;
-    return Column{col / group, kv * group + col % group};
+    const uint32_t per = again(group);
+    return Column{col / per, kv * group + col % per};
   };
 
   // The keys that the columns' rows see begin in no order: the earliest start and the latest.  Past the prefix a tile goes by
@@ -470,7 +472,10 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   // workgroup's columns are done again one by one.
   if (__builtin_amdgcn_readfirstlane(sh.special) != 0u) {          // workgroup-uniform
     __syncthreads();
-    for (uint32_t c = c0; c < c_end; ++c) attend_pair<KV, 512>(a, tree_pair(a, kv, c), kv, wg_start, wg_last, s_part, *reinterpret_cast<PairShared*>(sh.stage[0]));
+    for (uint32_t c = c0; c < c_end; ++c) {
+      const TreePair pair{c / group, c / group * a.heads + kv * group + c % group};
+      attend_pair<KV, 512>(a, pair, kv, wg_start, wg_last, s_part, *reinterpret_cast<PairShared*>(sh.stage[0]));
+    }
     return;
   }
   if (c0 + own_at >= c_end) return;
