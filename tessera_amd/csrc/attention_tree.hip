@@ -17,7 +17,7 @@ namespace {
 // Bound by the matrix instructions and what does not go on beside them, as all wavefronts are at the same place.  So nothing
 // is done to the running sums but by the matrix instructions: weights are taken relative to a reference that follows the
 // largest score only where it would leave 2^kSlack of it, and just then the sums are scaled; and the next tile goes to LDS a
-// piece at a time between them.  64 rows of 24 heads of 256 over 4 on 32832 fp16 keys in ten parts: 115 us (702 with a
+// piece at a time between them.  64 rows of 24 heads of 256 over 4 on 32832 fp16 keys in ten parts: 111 us (702 with a
 // workgroup a row and key head); a tile of 64 keys 1.47 us, 1.79 with the next one's way to LDS in one go, 2.57 with every
 // tile's sums added to the running ones by the vector unit.
 constexpr float kSlack = 4.0f;                    // in powers of two

@@ -14,7 +14,8 @@ namespace {
 // Bound by latency.  An ancestor chain has up to `nodes` links, so it is not walked link by link: all nodes first walk
 // the links inside their own 32 (one word of the bits, at most 31 links) and keep those bits and the ancestor outside
 // (`leave`); then a node needs one step a word.  A workgroup does the first for every node before its last one and the
-// second for 64 of its own, whose rows it gathers in LDS to write them whole.  16 nodes TIME16, 1000 nodes TIME1000.
+// second for 64 of its own, whose rows it gathers in LDS to write them whole.  16 nodes 3.5 us among others
+// (an empty launch), 1000 nodes 5.8.
 constexpr uint32_t kRoot = 0xFFFFFFFFu, kPadding = 0xFFFFFFFEu;
 constexpr uint32_t kTreeNodes = 64, kTreeThreads = 256;
 

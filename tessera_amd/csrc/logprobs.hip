@@ -363,7 +363,7 @@ struct Plan {
 };
 // Threads of a workgroup: as many as eight entries each make a short row, 1024 where there is much to read, otherwise 512, whose
 // barriers are shorter (us, 256 / 512 / 1024 threads: 512 rows of 1000 6.7 / 7.3 / 10.2, 512 of 4000 13.1 / 10.1 / 14.7, one of
-// 131072 10.5 / 9.7 / 10.7, 128 of 131072 28.4 / 27.0 / 24.9, 512 of them 75 / 70 / 58).
+// 131072 10.5 / 9.7 / 10.7, 128 of 131072 28.4 / 27.0 / 24.9, 512 of them 75 / 70 / 58.5, 4.6 TB/s).
 // Tiles of a row a workgroup takes: the shortest time in tiles, the chip's threads full, each workgroup with one tile's time of
 // its own, the second launch with two (128 rows of 131072 as 1, 4, 16 tiles a workgroup: 34 / 25 / 36 us).
 Plan plan_of(uint64_t rows, uint64_t vocab, bool shared) {

@@ -27,6 +27,7 @@ struct QkNormArgs {
 __device__ __forceinline__ float2 cos_sin(const QkNormArgs& a, uint64_t row, uint32_t j) {
   uint64_t p = a.pos_base + row;
   if (a.pos3 != nullptr) p = a.pos3[row * 3 + (j < a.sec_t ? 0u : j < a.sec_t + a.sec_h ? 1u : 2u)];
+  if (p > (uint64_t{1} << 50)) p = uint64_t{1} << 50;              // above, n below is off by more than one
   double f = 1.0;
 #pragma unroll
   for (uint32_t b = 0; b < 7; ++b) f *= (j >> b & 1u) != 0u ? a.turn[b] : 1.0;
@@ -213,10 +214,10 @@ hipError_t launch_qk_norm_rope(const QkNormCall& call, const float* q, const flo
     constexpr int LANES = decltype(lanes)::value;
     const uint64_t groups = (all + 64 / LANES - 1) / (64 / LANES);
     // With many heads a wavefront takes several of a row, which share its angles and hide each other's way to memory (us, 1 / 2
-    // / 4 / 7 / 14 at a time: 2048 rows of 28 heads of 256 53 / 38 / 31 / 29 / 31, 512 rows 16 / 11.3 / 10.1 / 9.8 / 11.9, 128 rows
-    // 6.4 / 5.3 / 5.3 / 6.7 / 9.9, one row 4.2 / 4.2 / 4.8 / 6.2 / 9.3).
+    // / 4 / 7 / 14 at a time: 2048 rows of 28 heads of 256 with fp16 keys 44 / 30 / 24.3 / 25.4 / 26, 4.7 TB/s of them; 512 rows 12.7 / 9.2 /
+    // 8.5 / 8.2 / 10.7, 128 rows 5.3 / 4.5 / 5.0 / 6.3 / 9.7, one row 3.4 / 3.4 / 4.4 / 5.6 / 8.7).
     const uint64_t units = call.rows * groups;
-    a.each = units >= 32768 ? 7 : units >= 8192 ? 4 : units >= 2048 ? 2 : 1;
+    a.each = units >= 8192 ? 4 : units >= 2048 ? 2 : 1;
     a.chunks = static_cast<uint32_t>((groups + a.each - 1) / a.each);
     const dim3 g = grid(call.rows * a.chunks);
     if (f16) hipLaunchKernelGGL((qk_norm_rope_kernel<LANES, true>), g, dim3(256), 0, stream, a);

@@ -117,6 +117,23 @@ def test_qk_norm_rope_far_positions(backend, base):
     qk_norm(backend, (4, 2, 1, 34, 34), True, gated=False, f16=False, base=base, theta=10000.0)
 
 
+@pytest.mark.parametrize("dim", [128, 34])
+def test_qk_norm_mrope_positions_past_2_to_50(backend, dim):
+    """They count as 2^50: bounded results whatever the positions' buffer holds."""
+    rows, heads, kv = 6, 2, 1
+    rs = np.random.RandomState(dim)
+    up = backend.Upload
+    q, k, w = up(rs.randn(rows, heads * dim).astype(np.float32)), up(rs.randn(rows, kv * dim).astype(np.float32)), up(np.ones(dim, np.float32))
+    outs = []
+    for far in ([1 << 50] * 3, [(1 << 50) + 1, 1 << 63, (1 << 64) - 1]):
+        out = [backend.AllocateBuffer(rows * n * dim * 4) for n in (heads, kv)]
+        pos = up(np.array([far] * rows, np.uint64))
+        run(backend, "qk_norm_mrope", [q, k, w, w, pos, *out], [rows, heads, kv, dim, dim, f32_bits(1e6), f32_bits(1e-6), 0, 0, 0, 0, dim // 2 - 10, 5, 5])
+        backend.Synchronize()
+        outs.append([backend.CopyD2H(x, dtype=np.float32) for x in out])
+    assert all(np.array_equal(x, y) for x, y in zip(*outs))
+
+
 @pytest.mark.parametrize("gain", [0.0, 1e-12, 1e12])
 def test_qk_norm_rope_magnitudes(backend, gain):
     qk_norm(backend, (3, 4, 2, 128, 64), False, gated=False, f16=False, gain=gain, eps=1e-5)
