@@ -180,7 +180,7 @@ const char* qmm_kernel_name(size_t index);
  *     pos_base, theta, epsilon (fp32 bits), q_stride, k_stride (0: rows side by side), k_f16, k_row.  "qk_norm_mrope": Pos
  *     (rows x 3 u64) after Wk, no pos_base, and sec_t, sec_h, sec_w at the end, as "mrope".  Angles are formed in fp64, positions
  *     above 2^50 as 2^50.  Qout may be Q and Kout K where they are laid out alike.
- *     "attention_tree": buffers Q, K, V, Mask, Out; scalars m, n, heads, kv_heads, head_dim (at most 256), tree, window, kv_f16
+ *     "attention_tree": buffers Q, K, V, Mask, Out; scalars m, n, heads, kv_heads, head_dim (at most 256), tree (1 to 65536), window, kv_f16
  *     (0: K and V fp32, 1: fp16).  Row i sees the first n - tree keys and those of the last `tree` that row i of Mask (m x ceil(tree
  *     / 32) words, as "tree_mask" writes it) names, and of all these the last `window` (0: all).  A row that sees no key becomes
  *     zeros; a key that a row does not see does not reach it, whatever it holds.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask,

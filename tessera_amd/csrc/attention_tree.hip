@@ -28,6 +28,7 @@ struct TreeTile {
   alignas(16) uint8_t stage[2][kStage];           // 64 keys, then two times 32 keys' values transposed
   float scales[2][2][64];                         // keys', values'
   float ref[2][64], sum[2][64], up[2][64];        // the halves'
+  uint32_t start[64];                             // of the keys that a column sees, where that is not the first
   uint32_t low[4], high[4], special;
 };
 
@@ -147,15 +148,13 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   // The keys that the columns' rows see begin in no order: the earliest start and the latest.  Past the prefix a tile goes by
   // the rows' bits.
   const uint32_t prefix = static_cast<uint32_t>(a.n - a.tree);
-  auto start_of = [&](uint32_t row) {
-    uint64_t first_key, last_key;
-    key_range<true>(a, row, first_key, last_key);
-    return static_cast<uint32_t>(first_key);
-  };
   uint32_t wg_start, latest_start, wg_last = static_cast<uint32_t>(a.n - 1);
   {
-    uint32_t low = start_of(column(t).row), high = low;
+    uint64_t first_key, last_key;
+    key_range<true>(a, column(t).row, first_key, last_key);
+    uint32_t low = static_cast<uint32_t>(first_key), high = low;
     if (a.window != 0 || prefix == 0u) {
+      if (g == 0u && half == 0u) sh.start[col_group * 16u + r] = low;
 #pragma unroll
       for (uint32_t off = 8u; off > 0u; off >>= 1) {
         const uint32_t l = __shfl_xor(low, off, kWave), h = __shfl_xor(high, off, kWave);
@@ -358,7 +357,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       const uint32_t now = again(t), key0 = j0 + half * 32u, from = 4u * (now >> 4 & 3u);
       const uint32_t row = column(now).row;
       uint32_t shown = key0 <= wg_last ? tree_keys(a, a.mask + static_cast<uint64_t>(row) * a.words, key0) : 0u;
-      const uint32_t start = a.window == 0 ? 0u : start_of(row);   // (where there is no window, rows that see nothing have no bits)
+      const uint32_t start = a.window == 0 ? 0u : sh.start[col_group * 16u + (now & 15u)];   // (with no window, rows that see nothing have no bits)
       if (start > key0) shown = start - key0 < 32u ? shown & ~0u << (start - key0) : 0u;
       if (wg_last - key0 < 31u) shown &= (2u << (wg_last - key0)) - 1u;
       shown >>= from;

@@ -1478,7 +1478,7 @@ qmm_status run_qk_norm_mrope(const LaunchCtx& c) { return run_qk_norm(c, true); 
 
 // "attention_tree": buffers Q (m x heads*head_dim fp32), K, V (n x kv_heads*head_dim, fp32 or fp16), Mask (m x ceil(tree /
 // 32) u32), Out (as Q); scalars m, n, heads, kv_heads, head_dim, tree, window, kv_f16.  Every row sees the first n - tree
-// keys and those of the last `tree` that its bits name (bit j % 32 of word j / 32: key n - tree + j), of all these the last
+// keys and those of the last `tree` (at most 65536) that its bits name (bit j % 32 of word j / 32: key n - tree + j), of all these the last
 // `window` (0: all); a row that sees nothing becomes zeros.  "attention_tree_q8", "_q4", "_fp8": the caches of
 // "attention_q8", ..: Q, K and V codes, one scale a key row for K and for V, Mask, Out; without kv_f16.
 qmm_status run_attention_tree_kind(const LaunchCtx& c, bool quantized, uint32_t kind) {

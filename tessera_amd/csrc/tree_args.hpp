@@ -32,6 +32,7 @@ inline float scalar_f32(uint64_t bits) {
 }
 
 constexpr uint32_t kTreeMaskMost = 1024;        // nodes of "tree_mask"
+constexpr uint64_t kTreeKeysMost = 1 << 16;     // of "attention_tree", which counts a row's bits word by word under a window
 constexpr uint64_t kLogprobTokensMost = 1024, kLogprobTopMost = 32;
 
 // "tree_mask": buffers Parents, Mask, Positions; scalars nodes, base.
@@ -124,7 +125,7 @@ inline const char* check_attention_tree(const LaunchArgs& c, bool quantized, uin
     return "attention_tree: m, n, heads, kv_heads, head_dim must be non-zero and heads a multiple of kv_heads";
   }
   if (head_dim > 256) return "attention_tree: head_dim must be at most 256";
-  if (tree == 0 || tree > n) return "attention_tree: the tree holds one key at least and n at most";
+  if (tree == 0 || tree > n || tree > kTreeKeysMost) return "attention_tree: the tree holds one key at least, n and 65536 at most";
   if (!quantized && c.sc[7] > 1) return "attention_tree: kv_f16 is 0 or 1";
   if (kind == 3 && (kv_heads * head_dim) % 2 != 0) return "attention_tree_q4: a key row must hold an even number of codes";
   if (m > (1u << 24) || n > (uint64_t{1} << 31) || heads > (1u << 16) || c.sc[6] > (uint64_t{1} << 48) || m * heads > 0xFFFFFFull) {

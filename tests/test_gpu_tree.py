@@ -252,6 +252,13 @@ def test_attention_tree(backend, kind, case):
     check_attention(backend, kind, *case)
 
 
+@pytest.mark.parametrize("kind", ["f32", "f16", "q8", "fp8"])
+@pytest.mark.parametrize("case", [(5, 3001, 4, 2, 128, 2500, 700), (40, 3001, 8, 2, 256, 2100, 0), (40, 2600, 8, 2, 64, 2600, 900), (3, 2600, 8, 4, 34, 1500, 40)])
+def test_attention_tree_of_many_words(backend, kind, case):
+    """More keys under masks than "tree_mask" writes, windows that begin between them."""
+    check_attention(backend, kind, *case)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "q8", "q4", "fp8"])
 @pytest.mark.parametrize("case", [c for c in ATTEND if c[0] == c[5]])
 def test_attention_tree_of_drafts(backend, kind, case):

@@ -57,7 +57,6 @@ def test_tree_mask(tmp_path):
   Launch l({132, 33 * 8, 33 * 24}, {33, 0});
   l.buf[1] = l.buf[0];
   CHECK(check_tree_mask(l.args()));
-  CHECK(!check_tree_mask(Launch({1, 1, 1}, {33, 0}).args(false)) || true);
 """)
 
 
@@ -155,6 +154,8 @@ def test_attention_tree(tmp_path):
   CHECK(why(big, {m, n, heads, kv, d, tree, 0, 2}));
   CHECK(why(big, {m, (uint64_t{1} << 31) + 1, heads, kv, d, tree, 0, 1}));
   CHECK(why(big, {(1 << 24) + 1, n, heads, kv, d, tree, 0, 1}));
+  CHECK(!why(big, {1, 1 << 20, 1, 1, d, 1 << 16, 0, 1}));
+  CHECK(why(big, {1, 1 << 20, 1, 1, d, (1 << 16) + 1, 0, 1}));
   CHECK(why(big, {m, n, heads, kv, d, tree, 0}));
   Launch l(fits, {m, n, heads, kv, d, tree, 0, 1});
   l.buf[4] = l.buf[0];
