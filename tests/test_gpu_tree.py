@@ -260,6 +260,20 @@ def test_attention_tree_of_many_words(backend, kind, case):
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "q8", "q4", "fp8"])
+@pytest.mark.parametrize("case", [(3, 900, 4, 2, 128, 900, 0), (40, 900, 12, 2, 64, 900, 30), (33, 70, 6, 2, 256, 70, 0), (3, 900, 8, 4, 34, 900, 5), (1, 1, 8, 4, 34, 1, 0)])
+@pytest.mark.parametrize("which", ["none", "one", "last"])
+def test_attention_tree_of_rows_that_see_nothing(backend, kind, case, which):
+    """No row sees a key, one row does, the last key alone is seen: whatever else the cache holds."""
+    m, n = case[:2]
+    seen = np.zeros((m, n), bool)
+    if which == "one":
+        seen[m // 2, n // 3:n // 3 + 5] = True
+    elif which == "last":
+        seen[:, n - 1] = True
+    check_attention(backend, kind, *case, seen=seen, spoil=n > 1)
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "q8", "q4", "fp8"])
 @pytest.mark.parametrize("case", [c for c in ATTEND if c[0] == c[5]])
 def test_attention_tree_of_drafts(backend, kind, case):
     m = case[0]
