@@ -12,14 +12,18 @@ namespace {
 // v_mfma_f32_16x16x32_f16; the fp32 side (queries, weights) enters as two fp16 terms of a value x, hi = RN16(x) and lo =
 // RN16(x - hi), into the same sums: off by at most 2^-23 of x, or 2^-40 of the largest that x is scaled under.  Eight
 // wavefronts, two a SIMD: four groups of 16 columns times two halves of a tile of 64 keys.  A tile is made fp16 (exactly: fp16
-// numbers or codes) once, on its way into LDS, keys row by row, values transposed; all columns read the same operands.
+// numbers or codes) once, on its way into LDS, keys row by row, values transposed; all columns read the same operands.  An
+// fp32 key's elements, and a value's, become two such terms under a power of two of the key's own, to 2^-23 of an element down to
+// 2^-39 of the key's largest; of the four products of terms that of the second ones, 2^-22 of the whole at most, is left out.
 //
 // Bound by the matrix instructions and what does not go on beside them, as all wavefronts are at the same place.  So nothing
 // is done to the running sums but by the matrix instructions: weights are taken relative to a reference that follows the
 // largest score only where it would leave 2^kSlack of it, and just then the sums are scaled; and the next tile goes to LDS a
 // piece at a time between them.  64 rows of 24 heads of 256 over 4 on 32832 fp16 keys in ten parts: 111 us (702 with a
 // workgroup a row and key head); a tile of 64 keys 1.47 us, 1.79 with the next one's way to LDS in one go, 2.57 with every
-// tile's sums added to the running ones by the vector unit.
+// tile's sums added to the running ones by the vector unit.  Two terms of 64 fp32 keys of 256 fill the LDS: their tiles go
+// there between two barriers, 5 us each (of 128 3, of 64 2.1), the next one's loads under way meanwhile.  64 rows of 24
+// heads of 256 over 4 on 8192 fp32 keys: 85 us (220 by the kernel below).
 constexpr float kSlack = 4.0f;                    // in powers of two
 
 template <int DP>
@@ -32,7 +36,7 @@ struct TreeTile {
   uint32_t low[4], high[4], special;
 };
 
-// BYTES (1 to 16) at `offset` of a buffer whose end the hardware checks: what lies past it reads as 0.
+// BYTES (1 to 32) at `offset` of a buffer whose end the hardware checks: what lies past it reads as 0.
 template <int BYTES>
 __device__ __forceinline__ void load_run(__amdgpu_buffer_rsrc_t from, uint32_t offset, uint32_t (&r)[(BYTES + 3) / 4]) {
   if constexpr (BYTES == 1) {
@@ -45,9 +49,47 @@ __device__ __forceinline__ void load_run(__amdgpu_buffer_rsrc_t from, uint32_t o
     const auto v = __builtin_amdgcn_raw_buffer_load_b64(from, offset, 0, 0);
     r[0] = v[0], r[1] = v[1];
   } else {
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, offset, 0, 0);
-    r[0] = v[0], r[1] = v[1], r[2] = v[2], r[3] = v[3];
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(from, offset + 16u * i, 0, 0);
+      r[4 * i] = v[0], r[4 * i + 1] = v[1], r[4 * i + 2] = v[2], r[4 * i + 3] = v[3];
+    }
   }
+}
+
+// A key of an fp32 cache is taken under a power of two of its own, as its codes' scale is of a quantized one: `up` brings its largest
+// element to 2^14 .. 2^15.  The largest of a key's elements in the LANES lanes that hold them (with 32: lanes apart by 16 hold
+// two keys where `apart`).
+template <int LANES>
+__device__ __forceinline__ float key_most(float v, bool apart) {
+  auto step = [&](auto ctrl) {
+    constexpr int kCtrl = decltype(ctrl)::value;
+    v = fmaxf(v, bit_cast<float>(__builtin_amdgcn_update_dpp(0, bit_cast<int>(v), kCtrl, 0xF, 0xF, true)));
+  };
+  step(std::integral_constant<int, 0xB1>{});     // quad_perm [1,0,3,2]
+  step(std::integral_constant<int, 0x4E>{});     // quad_perm [2,3,0,1]
+  step(std::integral_constant<int, 0x141>{});    // row_half_mirror
+  if constexpr (LANES >= 16) step(std::integral_constant<int, 0x140>{});   // row_mirror
+  if constexpr (LANES == 32) {
+    const uint32_t x = bit_cast<uint32_t>(v);
+    if (apart) {
+      const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+      v = fmaxf(bit_cast<float>(b[0]), bit_cast<float>(b[1]));
+    } else {
+      const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+      v = fmaxf(bit_cast<float>(b[0]), bit_cast<float>(b[1]));
+    }
+  }
+  return v;
+}
+// The two terms of x under `up`.
+struct Terms {
+  _Float16 hi, lo;
+};
+__device__ __forceinline__ Terms terms_of(uint32_t x, float up) {
+  const float v = bit_cast<float>(x) * up;
+  const _Float16 hi = static_cast<_Float16>(v);
+  return Terms{hi, static_cast<_Float16>(v - static_cast<float>(hi))};
 }
 
 // A value the compiler takes for a new one: what is needed only now and then or after the walk over the keys is formed from
@@ -117,12 +159,14 @@ __device__ __forceinline__ void attend_pair(const AttentionArgs& a, TreePair whi
 
 template <KvKind KV, int DP>
 __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a) {
-  constexpr bool QUANT = kv_quantized(KV);
+  constexpr bool F32 = KV == KvKind::F32, QUANT = kv_quantized(KV), SCALED = QUANT || F32;
+  constexpr bool LATE = F32 && DP == 256;                          // the next values' way begins behind the products: no registers before
   constexpr int BITS = kv_bits(KV);
   constexpr int STEPS = DP / 32;                                   // matrix instructions of a score, in two sums
   constexpr int VE = DP / 16, RE = DP / 32;                        // elements of a row of the result, of a value run
   constexpr int CHUNKS = DP / 8;                                   // runs of eight elements of a key
   constexpr int KLOADS = 64 * CHUNKS / 512;
+  constexpr int EARLY = LATE ? KLOADS / 2 : KLOADS;
   constexpr int KDW = 8 * BITS / 32, VDW = (RE * BITS + 31) / 32;
   using Shared = TreeTile<DP>;
   __shared__ Shared sh;
@@ -233,6 +277,58 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     }
   };
 
+  // An fp32 tile's terms: the first in stage 0, the second in stage 1.
+  auto stash_f32 = [&] {
+    if constexpr (F32) {
+      const uint32_t now = again(t), to_key = now / CHUNKS, to_chunk = now % CHUNKS;
+#pragma unroll
+      for (int i = 0; i < KLOADS; ++i) {
+        const uint32_t key = to_key + i * (512u / CHUNKS);
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(bit_cast<float>(kr[i][e])));
+        most = key_most<CHUNKS>(most, false);
+        const float up = most == 0.0f ? 1.0f : power_of_two_to(most, 14);
+        if (!(most < INFINITY)) sh.special = 1u;
+        if (to_chunk == 0u) sh.scales[0][0][key] = 1.0f / up;
+        half8_t hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const Terms x = terms_of(kr[i][e], up);
+          hi[e] = x.hi, lo[e] = x.lo;
+        }
+        const uint32_t to = key * (DP * 2u) + ((to_chunk ^ key_swizzle(key)) * 16u);
+        *reinterpret_cast<half8_t*>(sh.stage[0] + to) = hi;
+        *reinterpret_cast<half8_t*>(sh.stage[1] + to) = lo;
+      }
+      const uint32_t to_run = (now & 15u) * 2u + (now >> 5 & 1u), to_four = half * 8u + (now >> 4 & 1u) * 4u + col_group;
+      const uint32_t to_row = to_run * RE & 15u, to_block = to_run * RE / 16u;
+      const uint32_t v_base = Shared::kKeyBytes + half * (DP * 64u) + to_block * 1024u + (((to_row * 4u + (to_four & 3u)) ^ (to_row & 12u) ^ to_block) * 16u) + (to_four >> 2 & 1u) * 8u;
+      float ups[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float most = 0.0f;
+#pragma unroll
+        for (int e = 0; e < RE; ++e) most = fmaxf(most, fabsf(bit_cast<float>(vr[k][e])));
+        most = key_most<32>(most, true);
+        ups[k] = most == 0.0f ? 1.0f : power_of_two_to(most, 14);
+        if (to_run == 0u) sh.scales[0][1][to_four * 4u + k] = 1.0f / ups[k];
+      }
+#pragma unroll
+      for (int j = 0; j < RE; ++j) {
+        __attribute__((ext_vector_type(4))) _Float16 hi, lo;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const Terms x = terms_of(vr[k][j], ups[k]);
+          hi[k] = x.hi, lo[k] = x.lo;
+        }
+        const uint32_t to = v_base ^ static_cast<uint32_t>(((4 * j) ^ (j & 12)) * 16);
+        *reinterpret_cast<uint2*>(sh.stage[0] + to) = bit_cast<uint2>(hi);
+        *reinterpret_cast<uint2*>(sh.stage[1] + to) = bit_cast<uint2>(lo);
+      }
+    }
+  };
+
   if (t == 0) sh.special = 0u;
   fetch_scales(wg_start);
 #pragma unroll
@@ -275,13 +371,15 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       }
       swap[(half * OWN + i) * 128u] = hi, swap[(half * OWN + i) * 128u + 64u] = lo;
     }
-    stash_scales(0);
-    fetch_scales(wg_start + 64u);
+    if constexpr (!F32) {
+      stash_scales(0);
+      fetch_scales(wg_start + 64u);
 #pragma unroll
-    for (int i = 0; i < KLOADS; ++i) stash_keys(0, i), fetch_keys(wg_start + 64u, i);
+      for (int i = 0; i < KLOADS; ++i) stash_keys(0, i), fetch_keys(wg_start + 64u, i);
 #pragma unroll
-    for (int j = 0; j < RE; ++j) stash_values(0, j);
-    fetch_values(wg_start + 64u);
+      for (int j = 0; j < RE; ++j) stash_values(0, j);
+      fetch_values(wg_start + 64u);
+    }
     lds_barrier();
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) q_hi[i] = swap[i * 128], q_lo[i] = swap[i * 128 + 64];
@@ -291,13 +389,20 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 #pragma unroll
   for (int j = 0; j < VE; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   float ref = -INFINITY, shift = 0.0f, run_sum = 0.0f;             // shift: ref in units of log2, 0 while there is none
-  float lane_most = 0.0f, value_up = QUANT ? power_of_two_to(0.0f, 14) : 0x1p10f;
+  float lane_most = 0.0f, value_up = SCALED ? power_of_two_to(0.0f, 14) : 0x1p10f;
   const uint32_t key_row = (half * 32u + r) * (DP * 2u), key_swz = key_swizzle(r);
   const uint32_t value_row = Shared::kKeyBytes + half * (DP * 64u) + (((r * 4u + g) ^ (r & 12u)) * 16u);
   // While a tile is multiplied the next one goes to LDS, a piece at a time between the matrix instructions, and the registers
   // of every piece take the tile after that one's.
   for (uint32_t j0 = wg_start, b = 0; j0 <= wg_last; j0 += 64u, b ^= 1u) {
-    const uint8_t* stage = sh.stage[b];
+    const uint8_t* stage = sh.stage[F32 ? 0 : b];
+    if constexpr (F32) {
+      stash_f32();
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i) fetch_keys(j0 + 64u, i);
+      if constexpr (!LATE) fetch_values(j0 + 64u);
+      lds_barrier();
+    }
 
     // Element 4 h + e of a lane: key 16 h + 4 g + e of the wavefront's 32.  Operands are read DEEP steps ahead of
     // their matrix instructions; the barriers keep the compiler from moving each read to its use.
@@ -305,21 +410,31 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int DEEP = 2;
-    half8_t kf[DEEP + 1][2];
+    half8_t kf[DEEP + 1][2], kl[F32 ? DEEP + 1 : 1][2];
     auto read_keys = [&](int step) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        kf[step % (DEEP + 1)][h] = *reinterpret_cast<const half8_t*>(stage + key_row + h * (16u * DP * 2u) + (((4u * step + g) ^ key_swz) * 16u));
+        const uint8_t* from = stage + key_row + h * (16u * DP * 2u) + (((4u * step + g) ^ key_swz) * 16u);
+        kf[step % (DEEP + 1)][h] = *reinterpret_cast<const half8_t*>(from);
+        if constexpr (F32) kl[step % (DEEP + 1)][h] = *reinterpret_cast<const half8_t*>(from + Shared::kStage);
       }
     };
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) read_keys(i);
-    stash_scales(b ^ 1u);
-    fetch_scales(j0 + 128u);
+    if constexpr (!F32) {
+      stash_scales(b ^ 1u);
+      fetch_scales(j0 + 128u);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int step = 0; step < STEPS; ++step) {
       if (step + DEEP < STEPS) read_keys(step + DEEP);
+      if constexpr (F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          acc[h][step % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[step % (DEEP + 1)][h], q_hi[step], acc[h][step % 2], 0, 0, 0);
+        }
+      }
 #pragma unroll
       for (int term = 0; term < 2; ++term) {
 #pragma unroll
@@ -328,13 +443,19 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
           x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % (DEEP + 1)][h], term == 0 ? q_hi[step] : q_lo[step], x, 0, 0, 0);
         }
       }
-      if (step % 2 == 1) stash_keys(b ^ 1u, step / 2), fetch_keys(j0 + 128u, step / 2);
+      if constexpr (!F32) {
+        if (step % 2 == 1) stash_keys(b ^ 1u, step / 2), fetch_keys(j0 + 128u, step / 2);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     // The values' operands, read AHEAD blocks ahead of their matrix instructions, two blocks at a time.
     constexpr int AHEAD = 2;
-    half8_t vf[AHEAD + 2];
-    auto read_values = [&](int j) { vf[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(stage + (value_row ^ static_cast<uint32_t>(j * 16)) + j * 1024u); };
+    half8_t vf[AHEAD + 2], vl[F32 ? AHEAD + 2 : 1];
+    auto read_values = [&](int j) {
+      const uint8_t* from = stage + (value_row ^ static_cast<uint32_t>(j * 16)) + j * 1024u;
+      vf[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(from);
+      if constexpr (F32) vl[j % (AHEAD + 2)] = *reinterpret_cast<const half8_t*>(from + Shared::kStage);
+    };
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) read_values(j);
 
@@ -343,10 +464,10 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float4_t x = acc[h][0] + acc[h][1];
-      if constexpr (QUANT) {
-        const uint32_t at = half * 32u + h * 16u + g * 4u;
-        const float4 ks = *reinterpret_cast<const float4*>(&sh.scales[b][0][at]);
-        vsv[h] = *reinterpret_cast<const float4*>(&sh.scales[b][1][at]);
+      if constexpr (SCALED) {
+        const uint32_t at = half * 32u + h * 16u + g * 4u, of = F32 ? 0u : b;
+        const float4 ks = *reinterpret_cast<const float4*>(&sh.scales[of][0][at]);
+        vsv[h] = *reinterpret_cast<const float4*>(&sh.scales[of][1][at]);
         s[4 * h] = x[0] * ks.x, s[4 * h + 1] = x[1] * ks.y, s[4 * h + 2] = x[2] * ks.z, s[4 * h + 3] = x[3] * ks.w;
       } else {
 #pragma unroll
@@ -382,7 +503,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       sum += s[e];
     }
     run_sum = fmaf(corr, run_sum, sum);
-    if constexpr (QUANT) {
+    if constexpr (SCALED) {
       // The values' scales enter the weights, under a power of two that keeps the largest contribution so far
       // between 2^9 and 2^15.
       lane_most *= corr;
@@ -424,6 +545,10 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       for (int i = 0; i < 2; ++i) {
         if (j + AHEAD + i < VE) read_values(j + AHEAD + i);
       }
+      if constexpr (F32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) o[j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(j + i) % (AHEAD + 2)], p_hi, o[j + i], 0, 0, 0);
+      }
 #pragma unroll
       for (int term = 0; term < 2; ++term) {
 #pragma unroll
@@ -431,10 +556,15 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
           o[j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[(j + i) % (AHEAD + 2)], term == 0 ? p_lo : p_hi, o[j + i], 0, 0, 0);
         }
       }
-      stash_values(b ^ 1u, j / 2);
+      if constexpr (!F32) stash_values(b ^ 1u, j / 2);
       __builtin_amdgcn_sched_barrier(0);
     }
-    fetch_values(j0 + 128u);
+    if constexpr (!F32) fetch_values(j0 + 128u);
+    if constexpr (LATE) {
+#pragma unroll
+      for (int i = EARLY; i < KLOADS; ++i) fetch_keys(j0 + 64u, i);
+      fetch_values(j0 + 64u);
+    }
     lds_barrier();                                                 // (the loads stay under way)
   }
   __syncthreads();
@@ -499,11 +629,10 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 
 // ---- few pairs a workgroup: eight at most, sixteen over an fp32 cache -------------------------------------------------------
 //
-// attend_row with `each` (row, head) pairs in place of a row's heads, so that a key is read once for all of them.  Over fp32 keys,
-// which the kernel above does not take, 64 rows of 24 heads over 4 of 256 on 8192 keys are 220 us by sixteen pairs and 428 by a
-// row's heads, 59 Tflop/s where fp32 matrix instructions do 157 at most; few keys are the other way round, 46 rows
-// of 8 heads over 1 of 128 on 52 9.4 by pairs and 7.6 by rows, as the sums of sixteen are merged.
-// The shortest calls are a launch and its latencies: 10 rows of 12 heads over 2 of 64 on 62 fp16 keys 7.0 us (an empty launch
+// attend_row with `each` (row, head) pairs in place of a row's heads, so that a key is read once for all of them: sixteen fp32
+// pairs or a row's heads, as tree_rule says.  10 rows of 8 heads over 8 of 128 on 4565 fp32 keys 49 us by rows, 15.7 by sixteen
+// pairs; few keys are the other way round, 46 rows of 8 heads over 1 of 128 on 52 7.6 and 9.4, as the sums of sixteen are merged.
+// The shortest calls are a launch and its latencies: 10 rows of 12 heads over 2 of 64 on 62 fp16 keys 5.5 us (an empty launch
 // among others 3.5).
 template <KvKind KV, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 1) void attention_pairs_kernel(AttentionArgs a, uint32_t each) {
@@ -572,7 +701,7 @@ TreeShape attention_tree_shape(uint32_t kind, uint64_t m, uint64_t n, uint64_t h
   const uint32_t dim = static_cast<uint32_t>(head_dim);
   const bool by_rows = with_kind(kind, [&](auto tag) { return runs_fit<decltype(tag)::value>(dim); });
   // (a tile's rows lie within 2^31 bytes, its loads are runs of eight elements)
-  const bool shared = kind != 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0 && kv_heads * head_dim * 2 < (1u << 25) && n < (1u << 31) && dim % 8 == 0;
+  const bool shared = reinterpret_cast<uintptr_t>(out) % 16 == 0 && kv_heads * head_dim * (kind == 0 ? 4 : 2) < (1u << 25) && n < (1u << 31) && dim % 8 == 0;
   const TreeCall call{m, window != 0 && window < n ? window : n, heads, kv_heads, head_dim, padded_head(dim), kind == 0, kind > 1, by_rows, shared};
   if (by_rows || shared) return tree_rule(call, static_cast<uint64_t>(num_cus()), most_parts, kAttentionPartsMost);
   uint64_t parts = 2 * static_cast<uint64_t>(num_cus()) / (m * heads);      // a workgroup a row and head
@@ -595,9 +724,7 @@ hipError_t launch_attention_tree(uint32_t kind, const float* q, const void* k, c
   }
   const hipError_t e = with_kind(kind, [&](auto tag) {
     constexpr KvKind KV = decltype(tag)::value;
-    if constexpr (KV != KvKind::F32) {
-      if (shape.tile) return launch_tree_tiles<KV>(a, stream);
-    }
+    if (shape.tile) return launch_tree_tiles<KV>(a, stream);
     if (runs_fit<KV>(a.head_dim)) return launch_pairs<KV>(a, shape.pairs, stream);
     hipLaunchKernelGGL((attention_any_kernel<KV, true>), dim3(static_cast<uint32_t>(m * heads * (parts < 2 ? 1 : parts))), dim3(256), 0, stream, a);
     return hipGetLastError();

@@ -318,6 +318,24 @@ def test_attention_tree_spoiled_for_others(backend, kind, head_dim):
     assert np.max(np.abs(got[::2] - want)) <= ref.attention_bound(q[::2], ke, ve, see, heads, kv_heads, head_dim)
 
 
+@pytest.mark.parametrize("case", [(1, 700, 4, 4, 64), (40, 2000, 8, 2, 64), (40, 2000, 8, 2, 128), (40, 2000, 6, 1, 256), (40, 1500, 4, 2, 72)])
+def test_attention_tree_f32_of_many_magnitudes(backend, case):
+    """Keys and values from 2^-115 to 2^100, elements of one key apart by 2^30, some below the least normal number, some keys 0."""
+    m, n, heads, kv_heads, head_dim = case
+    rs = np.random.RandomState(n + head_dim)
+    width = kv_heads * head_dim
+    scale = lambda low, high: np.exp2(rs.randint(low, high, (n, kv_heads, 1)).astype(np.float64))
+    q = (rs.randn(m, heads * head_dim) * 2.0 ** 50).astype(np.float32)
+    k = (rs.randn(n, kv_heads, head_dim) * scale(-115, -49) * np.exp2(-rs.randint(0, 31, (1, 1, head_dim)))).reshape(n, width).astype(np.float32)
+    v = (rs.randn(n, kv_heads, head_dim) * scale(-115, 100) * np.exp2(-rs.randint(0, 31, (n, 1, head_dim)))).reshape(n, width).astype(np.float32)
+    k[::50], v[25::50], k[7] = 0.0, 0.0, np.float32(3e-42)
+    seen = rs.rand(m, m) < 0.5
+    see = ref.visible(seen, n - m, 0)
+    got = attend_tree(backend, "f32", q, k, v, None, None, ref.words_of(seen), m, m, n, heads, kv_heads, head_dim, 0)
+    want = ref.attention(q, k, v, see, heads, kv_heads, head_dim)
+    assert np.max(np.abs(got - want)) <= ref.attention_bound(q, k, v, see, heads, kv_heads, head_dim)
+
+
 @pytest.mark.parametrize("kind", ["f16", "q8"])
 @pytest.mark.parametrize("m", [1, 8, 40])
 def test_attention_tree_of_a_chain_is_causal_attention(backend, kind, m):
