@@ -318,6 +318,42 @@ def test_attention_tree_spoiled_for_others(backend, kind, head_dim):
     assert np.max(np.abs(got[::2] - want)) <= ref.attention_bound(q[::2], ke, ve, see, heads, kv_heads, head_dim)
 
 
+@pytest.mark.parametrize("kind,what", [("f32", np.inf), ("f32", -np.inf), ("f32", np.nan), ("f16", np.inf), ("f16", -np.inf), ("f16", np.nan), ("q8", np.nan), ("q4", np.nan), ("fp8", np.nan)])
+@pytest.mark.parametrize("case", [(18, 150, 8, 4, 64), (18, 1500, 8, 4, 128), (40, 1500, 24, 4, 256), (5, 150, 8, 4, 34), (2, 90, 4, 2, 256)])
+def test_attention_tree_of_a_key_not_finite(backend, kind, what, case):
+    """One element of a key (a quantized one's scale): the rows that see it become what the formula makes of them, no other."""
+    m, n, heads, kv_heads, head_dim = case
+    rs, g = np.random.RandomState(2), np.random.default_rng(head_dim)
+    width, at = kv_heads * head_dim, n - m + 1
+    q = rs.randn(m, heads * head_dim).astype(np.float32)
+    k, ks = cache(g, kind, n, width)
+    v, vs = cache(g, kind, n, width)
+    seen = np.ones((m, m), bool)
+    seen[::2, 1] = False
+    if ks is None:
+        k = k.copy().reshape(n, width)
+        k[at, 3::head_dim] = what
+    else:
+        ks = ks.copy()
+        ks[at] = what
+    got = attend_tree(backend, kind, q, k, v, ks, vs, ref.words_of(seen), m, m, n, heads, kv_heads, head_dim, 0)
+    see = ref.visible(seen, n - m, 0)
+    ke, ve = elements(kind, k, ks, width).astype(np.float64), elements(kind, v, vs, width)
+    want = np.zeros((m, heads, head_dim))
+    with np.errstate(invalid="ignore"):
+        for i in range(m):
+            for h in range(heads):
+                on = slice(h // (heads // kv_heads) * head_dim, (h // (heads // kv_heads) + 1) * head_dim)
+                x = ke[see[i], on] @ q[i, h * head_dim:(h + 1) * head_dim].astype(np.float64) / np.sqrt(head_dim)
+                w = np.exp(x - x.max())
+                want[i, h] = w @ ve[see[i], on] / w.sum()
+    want = want.reshape(m, -1)
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.isnan(want).any() and not np.isnan(want).all()
+    finite = np.where(np.isfinite(ke), ke, 0.0)
+    bound = ref.attention_bound(q, finite, ve, see, heads, kv_heads, head_dim)
+    assert np.nanmax(np.abs(got - want)) <= bound
+
+
 @pytest.mark.parametrize("case", [(1, 700, 4, 4, 64), (40, 2000, 8, 2, 64), (40, 2000, 8, 2, 128), (40, 2000, 6, 1, 256), (40, 1500, 4, 2, 72)])
 def test_attention_tree_f32_of_many_magnitudes(backend, case):
     """Keys and values from 2^-115 to 2^100, elements of one key apart by 2^30, some below the least normal number, some keys 0."""
