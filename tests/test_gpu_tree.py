@@ -372,6 +372,29 @@ def test_attention_tree_f32_of_many_magnitudes(backend, case):
     assert np.max(np.abs(got - want)) <= ref.attention_bound(q, k, v, see, heads, kv_heads, head_dim)
 
 
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+def test_attention_tree_past_4_gib(backend, kind):
+    """A window at the end of a cache of more than 2^32 bytes, which is keys and values in one."""
+    heads, kv_heads, head_dim, window = 16, 8, 256, 500
+    width, elem = kv_heads * head_dim, np.float16 if kind == "f16" else np.float32
+    n = (1 << 32) // (width * elem().itemsize) + 5000
+    rs = np.random.RandomState(3)
+    rows = rs.randn(997, width).astype(elem)                 # row j of the cache: row j % 997 of these
+    kv = backend.Upload(np.take(rows, np.arange(n) % 997, axis=0))
+    tail = rows[np.arange(n - 1000, n) % 997]
+    for m in (1, 40):
+        q = rs.randn(m, heads * head_dim).astype(np.float32)
+        seen = np.tril(np.ones((m, m), bool))
+        out = backend.AllocateBuffer(q.nbytes)
+        run(backend, "attention_tree", [backend.Upload(q), kv, kv, backend.Upload(ref.words_of(seen)), out],
+            [m, n, heads, kv_heads, head_dim, m, window, int(kind == "f16")])
+        backend.Synchronize()
+        see = ref.visible(seen, 1000 - m, window)
+        want = ref.attention(q, tail, tail, see, heads, kv_heads, head_dim)
+        got = backend.CopyD2H(out, dtype=np.float32).reshape(want.shape)
+        assert np.max(np.abs(got - want)) <= ref.attention_bound(q, tail, tail, see, heads, kv_heads, head_dim)
+
+
 @pytest.mark.parametrize("kind", ["f16", "q8"])
 @pytest.mark.parametrize("m", [1, 8, 40])
 def test_attention_tree_of_a_chain_is_causal_attention(backend, kind, m):
@@ -439,6 +462,17 @@ def test_token_logprobs(backend, vocab, rows, top_k):
     tokens[:, 1] = x[2:].argmax(1)
     tokens[0, 2] = vocab                       # no token
     check_logprobs(backend, x, tokens, min(top_k, vocab), row_base=2)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_token_logprobs_past_4_gib(backend, rows):
+    """Rows behind 2^32 bytes of others."""
+    vocab = 131072
+    base = (1 << 32) // (vocab * 4) + 3
+    rs = np.random.RandomState(rows)
+    x = np.zeros((base + rows, vocab), np.float32)
+    x[base:] = rs.randn(rows, vocab)
+    check_logprobs(backend, x, rs.randint(0, vocab, (rows, 3)), 5, row_base=base)
 
 
 @pytest.mark.parametrize("vocab", [700, 9000, 40003])
