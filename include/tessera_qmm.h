@@ -182,9 +182,9 @@ const char* qmm_kernel_name(size_t index);
  *     above 2^50 as 2^50.  Qout may be Q and Kout K where they are laid out alike.
  *     "attention_tree": buffers Q, K, V, Mask, Out; scalars m, n, heads, kv_heads, head_dim (at most 256), tree (1 to 65536), window, kv_f16
  *     (0: K and V fp32, 1: fp16).  Row i sees the first n - tree keys and those of the last `tree` that row i of Mask (m x ceil(tree
- *     / 32) words, as "tree_mask" writes it) names, and of all these the last `window` (0: all).  A row that sees no key becomes
- *     zeros; a key that a row does not see does not reach it, whatever it holds.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask,
- *     Out over the caches of "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but where fp32 keys are shared
+ *     / 32) words, as "tree_mask" writes it) names, and of all these the last `window` (0: all).  A row that sees no key, or none
+ *     with a score above -infinity, becomes zeros; a key that a row does not see does not reach it, whatever it holds.  Scores may be as
+ *     large as fp32 holds their sums of products.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask, Out over the caches of "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but where fp32 keys are shared
  *     among many rows their elements and the values' are carried to 2^-23 of themselves down to 2^-39 of the key's largest.
  *     "token_logprobs": buffers Logits (row_base + rows rows of vocab floats), Tokens (rows x tokens u32), Logprobs (rows x
  *     tokens: log softmax of the row at each token, -infinity for one of vocab or more), Entropy (rows) and, with top_k, TopTokens (rows x top_k u32),

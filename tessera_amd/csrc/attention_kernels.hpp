@@ -32,7 +32,7 @@ constexpr bool kv_quantized(KvKind k) { return k == KvKind::Q8 || k == KvKind::Q
 // SPLIT (the flash-decoding ids, src/backends/rocm/rocm_kernels_basic.cpp:275-440): the part s of
 // (row, head) is chunk s of ceil(span / split) keys of the row's key range; it leaves the unnormalized
 // sum, the chunk's largest score and its sum of weights in pacc / pmax / psum at index
-// (row * heads + head) * split + s (an empty chunk: 0, -1e30, 0); attention_combine_kernel merges them.
+// (row * heads + head) * split + s (an empty chunk: 0, kNoScore, 0); attention_combine_kernel merges them.
 struct SplitOut {
   float *pacc, *pmax, *psum;
   uint64_t split;   // 0: no parts, `out` receives the rows
@@ -257,15 +257,30 @@ struct RowsShared {
   alignas(16) float o[NW][rows_heads<KV>()][16][DP / 16 + 4];
 };
 
+// The largest score of a part that has none.  The attention ids' parts are the reference's, for which that is -1e30, and no
+// score counts for less; the tree's are its own.
+template <bool TREE>
+constexpr float kNoScore = TREE ? -INFINITY : -1e30f;
+// A part's largest score in natural units, `largest` of the matrix instructions' times `natural`, is rounded; its sums move by
+// what that took from it.  TREE: by 2^20 at most, so that they stay in range.  Rounding takes more from scores of 2^28 on only, whose
+// neighbours in fp32 are 32 apart.
+template <bool TREE>
+__device__ __forceinline__ float part_move(float largest, float natural) {
+  if (largest == -INFINITY) return 1.0f;
+  float moved = fmaf(largest, natural, -(largest * natural)) * kLog2E;
+  if constexpr (TREE) moved = fminf(fmaxf(moved, -20.0f), 20.0f);
+  return __builtin_amdgcn_exp2f(moved);
+}
+
 // A part without keys, of heads head0 .. head0 + here - 1 of a row.
-template <int THREADS>
+template <int THREADS, bool TREE = false>
 __device__ __forceinline__ void empty_part(const AttentionArgs& a, uint64_t row, uint32_t head0, uint32_t here, uint64_t s_part) {
   const uint32_t t = threadIdx.x, D = a.head_dim;
   const uint64_t split = a.part.split;
   for (uint32_t i = t; i < here * D; i += THREADS) a.part.pacc[((row * a.heads + head0 + i / D) * split + s_part) * D + i % D] = 0.0f;
   if (t < here) {
     const uint64_t at = (row * a.heads + head0 + t) * split + s_part;
-    a.part.pmax[at] = -1e30f, a.part.psum[at] = 0.0f;
+    a.part.pmax[at] = kNoScore<TREE>, a.part.psum[at] = 0.0f;
   }
 }
 
@@ -615,11 +630,9 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
     if (TREE && !(fabsf(acc) < INFINITY && fabsf(sum) < INFINITY)) pairs->special = 1u;
     if (a.part.split != 0) {
       const uint64_t at = (TREE ? static_cast<uint64_t>(pairs->at[h]) : row * a.heads + head0 + h) * split + s_part;
-      // The part's largest score in natural units is rounded; the sums move by what that took from it.
-      const float natural = scale * kLn2, largest = m * natural;
-      const float moved = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(m, natural, -largest) * kLog2E);
+      const float natural = scale * kLn2, moved = part_move<TREE>(m, natural);
       a.part.pacc[at * D + d] = acc * moved;
-      if (d == 0) a.part.pmax[at] = largest, a.part.psum[at] = sum * moved;
+      if (d == 0) a.part.pmax[at] = m * natural, a.part.psum[at] = sum * moved;
     } else {
       a.out[(TREE ? static_cast<uint64_t>(pairs->at[h]) : (a.row_base + row) * a.heads + head0 + h) * D + d] = TREE && sum == 0.0f ? 0.0f : acc / sum;
     }
@@ -1120,10 +1133,9 @@ __global__ __launch_bounds__(512, 2) void attention_tile_kernel(AttentionArgs a)
   if (split > 1u) {
     const uint64_t part = (own.row * a.heads + own.head) * split + s_part;
     out = a.part.pacc + part * D;
-    // The part's largest score in natural units is rounded; the sums move by what that took from it.
-    const float most = sh.most[at], natural = score_scale * kLn2, largest = most * natural;
-    factor = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(most, natural, -largest) * kLog2E);
-    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(largest, -1e30f), a.part.psum[part] = total * factor;
+    const float most = sh.most[at], natural = score_scale * kLn2;
+    factor = part_move<false>(most, natural);
+    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(most * natural, kNoScore<false>), a.part.psum[part] = total * factor;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -1175,7 +1187,7 @@ __global__ __launch_bounds__(256) void attention_any_kernel(AttentionArgs a) {
   key_range<TREE>(a, i, start, last);
   if (a.part.split != 0 && !key_chunk(a, at % split, start, last)) {   // workgroup-uniform
     if (t < D) a.part.pacc[at * D + t] = 0.0f;
-    if (t == 0) a.part.pmax[at] = -1e30f, a.part.psum[at] = 0.0f;
+    if (t == 0) a.part.pmax[at] = kNoScore<TREE>, a.part.psum[at] = 0.0f;
     return;
   }
   const float scale = 1.0f / sqrtf(static_cast<float>(D));
@@ -1265,16 +1277,17 @@ __global__ __launch_bounds__(WAVES * 64) void attention_combine_kernel(const flo
     }
   };
   fetch(0);
-  float first_max = lane < split ? pmax[base + lane] : -1e30f;
+  float first_max = lane < split ? pmax[base + lane] : kNoScore<TREE>;
   float first_sum = lane < split ? psum[base + lane] : 0.0f;
-  float top = fmaxf(first_max, -1e30f);
+  float top = fmaxf(first_max, kNoScore<TREE>);
   for (uint32_t s = lane + 64u; s < split; s += 64u) top = fmaxf(top, pmax[base + s]);
   top = wave_max(top);
+  if constexpr (TREE) top = reference_score(top);
   float n[V] = {}, d = 0.0f;
   for (uint32_t s0 = 0; s0 < split; s0 += kRound) {
     if (s0 != 0u) {
       fetch(s0);
-      first_max = s0 + lane < split ? pmax[base + s0 + lane] : -1e30f;
+      first_max = s0 + lane < split ? pmax[base + s0 + lane] : kNoScore<TREE>;
       first_sum = s0 + lane < split ? psum[base + s0 + lane] : 0.0f;
     }
     const bool here = lane < kRound && s0 + lane < split;

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   if (split > 1u) {                                                // whole tiles of the workgroup's keys a part
     const uint32_t chunk = ((wg_last - wg_start + split) / split + 63u) / 64u * 64u;
     if (static_cast<uint64_t>(s_part) * chunk > wg_last - wg_start) {
-      for (uint32_t c = c0; c < c_end; ++c) empty_part<512>(a, c / group, kv * group + c % group, 1, s_part);
+      for (uint32_t c = c0; c < c_end; ++c) empty_part<512, true>(a, c / group, kv * group + c % group, 1, s_part);
       return;
     }
     wg_start += s_part * chunk;
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   float4_t o[VE];
 #pragma unroll
   for (int j = 0; j < VE; ++j) o[j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  float ref = -INFINITY, shift = 0.0f, run_sum = 0.0f;             // shift: ref in units of log2, 0 while there is none
+  float ref = -INFINITY, origin = 0.0f, run_sum = 0.0f;            // origin: ref, 0 while there is none
   float lane_most = 0.0f, value_up = SCALED ? power_of_two_to(0.0f, 14) : 0x1p10f;
   const uint32_t key_row = (half * 32u + r) * (DP * 2u), key_swz = key_swizzle(r);
   const uint32_t value_row = Shared::kKeyBytes + half * (DP * 64u) + (((r * 4u + g) ^ (r & 12u)) * 16u);
@@ -408,7 +408,10 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     // their matrix instructions; the barriers keep the compiler from moving each read to its use.
     float4_t acc[2][2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i / 2][i % 2] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int h = 0; h < 2; ++h) {
+      acc[h][0] = SCALED ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : float4_t{-origin, -origin, -origin, -origin};
+      acc[h][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     constexpr int DEEP = 2;
     half8_t kf[DEEP + 1][2], kl[F32 ? DEEP + 1 : 1][2];
     auto read_keys = [&](int step) {
@@ -468,7 +471,8 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
         const uint32_t at = half * 32u + h * 16u + g * 4u, of = F32 ? 0u : b;
         const float4 ks = *reinterpret_cast<const float4*>(&sh.scales[of][0][at]);
         vsv[h] = *reinterpret_cast<const float4*>(&sh.scales[of][1][at]);
-        s[4 * h] = x[0] * ks.x, s[4 * h + 1] = x[1] * ks.y, s[4 * h + 2] = x[2] * ks.z, s[4 * h + 3] = x[3] * ks.w;
+        s[4 * h] = fmaf(x[0], ks.x, -origin), s[4 * h + 1] = fmaf(x[1], ks.y, -origin);
+        s[4 * h + 2] = fmaf(x[2], ks.z, -origin), s[4 * h + 3] = fmaf(x[3], ks.w, -origin);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * h + e] = x[e];
@@ -489,17 +493,21 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 #pragma unroll
     for (int e = 1; e < 8; ++e) most = fmaxf(most, s[e]);
     float corr = 1.0f;
-    if (__any(most > ref && (ref == -INFINITY || fmaf(most, score_scale, -shift) > kSlack))) {
-      const bool none = ref == -INFINITY;                          // the same in all lanes of the column, as ref is
-      ref = fmaxf(ref, groups_max(most));
-      const float to = ref == -INFINITY ? 0.0f : ref * score_scale;
-      corr = none ? 1.0f : __builtin_amdgcn_exp2f(shift - to);
-      shift = to;
+    // Scores are formed as differences from the reference, and only those are brought to units of log2: what rounding takes from a
+    // large score would else be a power of two to scale by.
+    if (__any(most * score_scale > kSlack || (ref == -INFINITY && most > ref))) {
+      const float before = ref;                                    // the same in all lanes of the column
+      ref = fmaxf(ref, groups_max(most + origin));
+      corr = before == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((before - ref) * score_scale);
+      const float to = reference_score(ref);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = (s[e] + origin) - to;
+      origin = to;
     }
     float sum = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], score_scale, -shift));
+      s[e] = __builtin_amdgcn_exp2f(s[e] * score_scale);
       sum += s[e];
     }
     run_sum = fmaf(corr, run_sum, sum);
@@ -578,10 +586,8 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 #pragma unroll
   for (int j = 0; j < VH; ++j) pieces[(half * VH + j) * 64u] = half == 0u ? o[VH + j] : o[j];
   __syncthreads();
-  const float ref0 = sh.ref[0][own_at], ref1 = sh.ref[1][own_at], top = fmaxf(ref0, ref1);
-  const float to = top == -INFINITY ? 0.0f : top * score_scale;
-  const float w0 = ref0 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref0 * score_scale - to);
-  const float w1 = ref1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ref1 * score_scale - to);
+  const float ref0 = sh.ref[0][own_at], ref1 = sh.ref[1][own_at], top = fmaxf(ref0, ref1), to = reference_score(top);
+  const float w0 = __builtin_amdgcn_exp2f((ref0 - to) * score_scale), w1 = __builtin_amdgcn_exp2f((ref1 - to) * score_scale);
   const float total = fmaf(w1, sh.sum[1][own_at], w0 * sh.sum[0][own_at]);
   const float f0 = w0 / sh.up[0][own_at], f1 = w1 / sh.up[1][own_at];
   float4_t merged[VH];                                             // elements 16 (half * VH + j) + 4 g ..
@@ -615,10 +621,9 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
   if (split > 1u) {
     const uint64_t part = pair * split + s_part;
     out = a.part.pacc + part * D;
-    // The part's largest score in natural units is rounded; the sums move by what that took from it.
-    const float natural = score_scale * kLn2, largest = top * natural;
-    factor = top == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(fmaf(top, natural, -largest) * kLog2E);
-    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(largest, -1e30f), a.part.psum[part] = total * factor;
+    const float natural = score_scale * kLn2;
+    factor = part_move<true>(top, natural);
+    if (late_g == 0u && half == 0u) a.part.pmax[part] = top * natural, a.part.psum[part] = total * factor;
   }
 #pragma unroll
   for (int j = 0; j < VH; ++j) {
@@ -665,7 +670,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attention_pairs_kernel(AttentionAr
   if (a.part.split != 0 && !key_chunk(a, s_part, start, last)) {   // workgroup-uniform
     for (uint32_t i = 0; i < here; ++i) {
       const TreePair pair = tree_pair(a, kv, first + i);
-      empty_part<NW * 64>(a, pair.row, pair.at - pair.row * a.heads, 1, s_part);
+      empty_part<NW * 64, true>(a, pair.row, pair.at - pair.row * a.heads, 1, s_part);
     }
     return;
   }
