@@ -184,8 +184,11 @@ const char* qmm_kernel_name(size_t index);
  *     (0: K and V fp32, 1: fp16).  Row i sees the first n - tree keys and those of the last `tree` that row i of Mask (m x ceil(tree
  *     / 32) words, as "tree_mask" writes it) names, and of all these the last `window` (0: all).  A row that sees no key, or none
  *     with a score above -infinity, becomes zeros; a key that a row does not see does not reach it, whatever it holds.  Scores may be as
- *     large as fp32 holds their sums of products.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask, Out over the caches of "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but where fp32 keys are shared
- *     among many rows their elements and the values' are carried to 2^-23 of themselves down to 2^-39 of the key's largest.
+ *     large as fp32 holds their sums of products.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask, Out over the caches of "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but for calls
+ *     whose rows share their keys (many rows on many keys, by the time that they are estimated to take): there a softmax weight (over
+ *     fp32 and quantized caches times its value's largest element or scale) is carried to 2^-23 of itself down to 2^-11 of the row's
+ *     largest, and below to 2^-34 of that, and fp32 keys and values to 2^-23 of an element down to 2^-28 of its key's largest,
+ *     below to 2^-50 of that, a product to 2^-22.
  *     "token_logprobs": buffers Logits (row_base + rows rows of vocab floats), Tokens (rows x tokens u32), Logprobs (rows x
  *     tokens: log softmax of the row at each token, -infinity for one of vocab or more), Entropy (rows) and, with top_k, TopTokens (rows x top_k u32),
  *     TopLogprobs; scalars rows, vocab, tokens (1 to 1024), top_k (0 to 32), row_base.  The largest entries in descending order,

@@ -9,12 +9,17 @@ namespace {
 // ---- a workgroup shares its keys among 64 (row, head) pairs ---------------------------------------
 //
 // The pairs of a key head, `group` to a row, are the columns of the contractions S^T = K Q^T and O^T = V^T P^T on
-// v_mfma_f32_16x16x32_f16; the fp32 side (queries, weights) enters as two fp16 terms of a value x, hi = RN16(x) and lo =
-// RN16(x - hi), into the same sums: off by at most 2^-23 of x, or 2^-40 of the largest that x is scaled under.  Eight
-// wavefronts, two a SIMD: four groups of 16 columns times two halves of a tile of 64 keys.  A tile is made fp16 (exactly: fp16
-// numbers or codes) once, on its way into LDS, keys row by row, values transposed; all columns read the same operands.  An
-// fp32 key's elements, and a value's, become two such terms under a power of two of the key's own, to 2^-23 of an element down to
-// 2^-39 of the key's largest; of the four products of terms that of the second ones, 2^-22 of the whole at most, is left out.
+// v_mfma_f32_16x16x32_f16.  Eight wavefronts, two a SIMD: four groups of 16 columns times two halves of a tile of 64 keys.  A tile is
+// made fp16 (exactly: fp16 numbers or codes) once, on its way into LDS, keys row by row, values transposed; all columns read the
+// same operands.
+//
+// What is fp32 enters as two fp16 terms under a power of two that brings the largest of its head, key or row near 2^14: hi =
+// RN16(x) and lo = RN16(2^11 (x - hi)), 2^-23 of x down to 2^-28 of the largest and 2^-50 of that below.  Of a query, and of an fp32
+// key under a power of two of its own, the products with a second term have sums of their own, scaled once a tile.  Values and
+// weights have one sum of all, as registers for two are not to be had and the vector unit takes 0.8 us a tile to add them up: an
+// fp32 value's second term is multiplied by 2^-11 of the weight, and a weight's is RN16(x - hi), which leaves 2^-23 of a weight (times its
+// value's power of two or scale) down to 2^-11 of its row's largest and 2^-34 of that below.  Of fp32 keys and values the product of
+// two second terms, 2^-22 of the whole at most, is left out.
 //
 // Bound by the matrix instructions and what does not go on beside them, as all wavefronts are at the same place.  So nothing
 // is done to the running sums but by the matrix instructions: weights are taken relative to a reference that follows the
@@ -82,14 +87,14 @@ __device__ __forceinline__ float key_most(float v, bool apart) {
   }
   return v;
 }
-// The two terms of x under `up`.
+// The two terms of x under `up`, the second one times 2^11.
 struct Terms {
   _Float16 hi, lo;
 };
 __device__ __forceinline__ Terms terms_of(uint32_t x, float up) {
   const float v = bit_cast<float>(x) * up;
   const _Float16 hi = static_cast<_Float16>(v);
-  return Terms{hi, static_cast<_Float16>(v - static_cast<float>(hi))};
+  return Terms{hi, static_cast<_Float16>((v - static_cast<float>(hi)) * 0x1p11f)};
 }
 
 // A value the compiler takes for a new one: what is needed only now and then or after the walk over the keys is formed from
@@ -367,7 +372,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       for (int e = 0; e < 8; ++e) {
         const float v = raw[i][kq_dim<KV>(e)] * up;
         hi[e] = static_cast<_Float16>(v);
-        lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+        lo[e] = static_cast<_Float16>((v - static_cast<float>(hi[e])) * 0x1p11f);
       }
       swap[(half * OWN + i) * 128u] = hi, swap[(half * OWN + i) * 128u + 64u] = lo;
     }
@@ -406,7 +411,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
 
     // Element 4 h + e of a lane: key 16 h + 4 g + e of the wavefront's 32.  Operands are read DEEP steps ahead of
     // their matrix instructions; the barriers keep the compiler from moving each read to its use.
-    float4_t acc[2][2];
+    float4_t acc[2][2];                                            // of the first terms, and of those that stand for 2^-11
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       acc[h][0] = SCALED ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : float4_t{-origin, -origin, -origin, -origin};
@@ -434,15 +439,13 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       if (step + DEEP < STEPS) read_keys(step + DEEP);
       if constexpr (F32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          acc[h][step % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[step % (DEEP + 1)][h], q_hi[step], acc[h][step % 2], 0, 0, 0);
-        }
+        for (int h = 0; h < 2; ++h) acc[h][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl[step % (DEEP + 1)][h], q_hi[step], acc[h][1], 0, 0, 0);
       }
 #pragma unroll
       for (int term = 0; term < 2; ++term) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float4_t& x = acc[h][step % 2];
+          float4_t& x = acc[h][term];
           x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[step % (DEEP + 1)][h], term == 0 ? q_hi[step] : q_lo[step], x, 0, 0, 0);
         }
       }
@@ -466,7 +469,9 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
     float4 vsv[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float4_t x = acc[h][0] + acc[h][1];
+      float x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = fmaf(acc[h][1][e], 0x1p-11f, acc[h][0][e]);
       if constexpr (SCALED) {
         const uint32_t at = half * 32u + h * 16u + g * 4u, of = F32 ? 0u : b;
         const float4 ks = *reinterpret_cast<const float4*>(&sh.scales[of][0][at]);
@@ -546,6 +551,11 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       p_hi[e] = hi;
       p_lo[e] = static_cast<_Float16>(x - static_cast<float>(hi));
     }
+    half8_t p_down;                                                // for the values' second terms
+    if constexpr (F32) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p_down[e] = p_hi[e] * static_cast<_Float16>(0x1p-11f);
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < VE; j += 2) {
@@ -555,7 +565,7 @@ __global__ __launch_bounds__(512, 2) void attention_tree_kernel(AttentionArgs a)
       }
       if constexpr (F32) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) o[j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(j + i) % (AHEAD + 2)], p_hi, o[j + i], 0, 0, 0);
+        for (int i = 0; i < 2; ++i) o[j + i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl[(j + i) % (AHEAD + 2)], p_down, o[j + i], 0, 0, 0);
       }
 #pragma unroll
       for (int term = 0; term < 2; ++term) {
