@@ -282,6 +282,42 @@ constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_par
   return best;
 }
 
+// ---- "token_logprobs" ------------------------------------------------------------------------------------------------
+// Threads of a workgroup: as many as eight entries each make a short row, 1024 where there is much to read, otherwise 512, whose
+// barriers are shorter (us, 256 / 512 / 1024 threads: 512 rows of 1000 6.7 / 7.3 / 10.2, 512 of 4000 13.1 / 10.1 / 14.7, one of
+// 131072 10.5 / 9.7 / 10.7, 128 of 131072 28.4 / 27.0 / 24.9, 512 of them 75 / 70 / 58.5, 4.6 TB/s).
+// Tiles of a row a workgroup takes: the shortest time in tiles, the chip's threads full, each workgroup with one tile's time of
+// its own, the second launch with two (128 rows of 131072 as 1, 4, 16 tiles a workgroup: 34 / 25 / 36 us).  Rows are shared where the
+// shares of all of them fit `most` bytes and one launch; more rows fill the chip as they are.
+constexpr uint32_t kLogprobEach = 8, kLogprobShares = 64;   // entries of a tile a thread; workgroups a row, at most
+constexpr uint64_t kLogprobRows = uint64_t{1} << 14;        // rows of a launch: so many workgroups of 1024 threads, 64 a row, stay a grid
+struct LogprobPlan {
+  uint32_t threads, width, tiles, shares;                   // columns of a tile, a multiple of four; tiles a workgroup; workgroups a row
+};
+// What the shares of `rows` rows take: three sums and top_k keys each.
+constexpr size_t logprob_bytes(const LogprobPlan& plan, uint64_t rows, uint64_t top_k) {
+  return plan.shares < 2 ? 0 : static_cast<size_t>(rows * plan.shares * (12u + 8u * top_k));
+}
+constexpr LogprobPlan logprob_plan(uint64_t rows, uint64_t vocab, uint64_t top_k, uint64_t cus, size_t most) {
+  const uint32_t threads = vocab <= 2048u ? 256u : vocab <= 4096u || rows * vocab <= (1u << 20) ? 512u : 1024u;
+  const uint64_t padded = vocab + (vocab % 4u == 0 ? 0u : 3u);      // rows that begin anywhere are read from the 16 bytes before
+  const uint64_t widest = uint64_t{threads} * kLogprobEach, all = (padded + widest - 1u) / widest;
+  const uint64_t slots = cus * (2048u / threads);
+  LogprobPlan best{threads, 0, static_cast<uint32_t>(all), 1};
+  if (rows <= kLogprobRows) {
+    uint64_t least = (rows + slots - 1) / slots * (all + 1);
+    for (uint64_t tiles = (all + kLogprobShares - 1) / kLogprobShares, last = tiles + 64u; tiles < all && tiles < last; ++tiles) {
+      const uint64_t shares = (all + tiles - 1) / tiles, cost = (rows * shares + slots - 1) / slots * (tiles + 1) + 2;
+      const LogprobPlan plan{threads, 0, static_cast<uint32_t>(tiles), static_cast<uint32_t>(shares)};
+      if (cost < least && logprob_bytes(plan, rows, top_k) <= most) least = cost, best = plan;
+    }
+  }
+  // all tiles of a row about as wide
+  const uint64_t tiles = uint64_t{best.tiles} * best.shares, width = ((padded + tiles - 1u) / tiles + 3u) / 4u * 4u;
+  best.width = static_cast<uint32_t>(width < widest ? width : widest);
+  return best;
+}
+
 // ---- "attention_combine" ---------------------------------------------------------------------------------------------
 // Wavefronts of a (row, head): sixteen where there are few and many parts, four where the rows fill the chip by themselves or
 // sixteen parts are all that there are, one where its four are and that does not make a lane's run long with few rows (us, 1 /

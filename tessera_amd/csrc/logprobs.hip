@@ -8,6 +8,7 @@
 // -0 and +0 tie, NaN ranks below everything.  A token id of vocab or more has log probability -infinity.
 
 #include "qmm_device.hpp"
+#include "launch_rules.hpp"
 #include "qmm_kernels.hpp"
 #include "tree_args.hpp"
 
@@ -15,7 +16,7 @@ namespace qmm {
 namespace {
 
 constexpr float kLog2E = 1.44269504088896340736f;
-constexpr uint32_t kEach = 8;                                 // entries of a tile a thread
+constexpr uint32_t kEach = kLogprobEach;
 constexpr uint32_t kMost = kLogprobTopMost, kListMost = 1024;
 
 struct LogprobArgs {
@@ -313,7 +314,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) void logprob_tile
 
 // The shares of a row (at most kSharesMost): their sums under the largest reference; of their sorted keys those that reach
 // a bound that top_k of them do, each counting those above it.
-constexpr uint32_t kSharesMost = 64, kMergeThreads = 256;
+constexpr uint32_t kSharesMost = kLogprobShares, kMergeThreads = 256;
 __global__ __launch_bounds__(kMergeThreads) void logprob_merge_kernel(LogprobArgs a) {
   constexpr uint32_t kKeys = kSharesMost * kMost / kMergeThreads;   // a thread's
   __shared__ uint64_t list[kSharesMost * kMost], best[kMost], level[kSharesMost], bound_s;
@@ -358,54 +359,22 @@ __global__ __launch_bounds__(kMergeThreads) void logprob_merge_kernel(LogprobArg
   finish(a, row, all, best, own, t, kMergeThreads);
 }
 
-struct Plan {
-  uint32_t threads, width, tiles, shares;
-};
-// Threads of a workgroup: as many as eight entries each make a short row, 1024 where there is much to read, otherwise 512, whose
-// barriers are shorter (us, 256 / 512 / 1024 threads: 512 rows of 1000 6.7 / 7.3 / 10.2, 512 of 4000 13.1 / 10.1 / 14.7, one of
-// 131072 10.5 / 9.7 / 10.7, 128 of 131072 28.4 / 27.0 / 24.9, 512 of them 75 / 70 / 58.5, 4.6 TB/s).
-// Tiles of a row a workgroup takes: the shortest time in tiles, the chip's threads full, each workgroup with one tile's time of
-// its own, the second launch with two (128 rows of 131072 as 1, 4, 16 tiles a workgroup: 34 / 25 / 36 us).
-Plan plan_of(uint64_t rows, uint64_t vocab, bool shared) {
-  const uint32_t threads = vocab <= 2048u ? 256u : vocab <= 4096u || rows * vocab <= (1u << 20) ? 512u : 1024u;
-  const uint64_t padded = vocab + (vocab % 4u == 0 ? 0u : 3u);      // rows that begin anywhere are read from the 16 bytes before
-  const uint64_t most = uint64_t{threads} * kEach, all = (padded + most - 1u) / most;
-  const uint64_t slots = static_cast<uint64_t>(num_cus()) * (2048u / threads);
-  Plan best{threads, 0, static_cast<uint32_t>(all), 1};
-  if (shared) {
-    uint64_t least = (rows + slots - 1) / slots * (all + 1);
-    for (uint64_t tiles = (all + kSharesMost - 1) / kSharesMost, last = tiles + 64u; tiles < all && tiles < last; ++tiles) {
-      const uint64_t shares = (all + tiles - 1) / tiles, cost = (rows * shares + slots - 1) / slots * (tiles + 1) + 2;
-      if (cost < least) least = cost, best.tiles = static_cast<uint32_t>(tiles), best.shares = static_cast<uint32_t>(shares);
-    }
-  }
-  // all tiles of a row about as wide
-  const uint64_t tiles = uint64_t{best.tiles} * best.shares, width = ((padded + tiles - 1u) / tiles + 3u) / 4u * 4u;
-  best.width = static_cast<uint32_t>(width < most ? width : most);
-  return best;
+LogprobPlan plan_of(uint64_t rows, uint64_t vocab, uint32_t top_k, size_t most) {
+  return logprob_plan(rows, vocab, top_k, static_cast<uint64_t>(num_cus()), most);
 }
-constexpr uint64_t kRowsMost = uint64_t{1} << 20;                 // rows of a launch: 64 workgroups of 1024 threads each stay a grid
-size_t bytes_a_row(const Plan& plan, uint32_t top_k) { return plan.shares < 2 ? 0 : size_t{plan.shares} * (12u + 8u * top_k); }
 
 }  // namespace
 
-// What the shares of all rows take, or of as many rows as fit `most` bytes.
 size_t token_logprobs_scratch_bytes(uint64_t rows, uint64_t vocab, uint32_t top_k, size_t most) {
-  const size_t each = bytes_a_row(plan_of(rows, vocab, true), top_k);
-  if (each == 0) return 0;
-  const uint64_t at_once = most / each < rows ? most / each : rows;
-  return static_cast<size_t>(at_once) * each + 16;
+  return logprob_bytes(plan_of(rows, vocab, top_k, most), rows, top_k);
 }
 
 hipError_t launch_token_logprobs(const float* logits, const uint32_t* tokens, float* logprobs, float* entropy, uint32_t* top_tokens,
                                  float* top_logprobs, uint64_t rows, uint64_t vocab, uint32_t count, uint32_t top_k, uint64_t row_base,
-                                 void* scratch, size_t scratch_bytes, hipStream_t stream) {
-  const Plan plan = plan_of(rows, vocab, scratch != nullptr);
-  const size_t each = bytes_a_row(plan, top_k);
-  uint64_t at_once = each == 0 ? rows : (scratch_bytes - 16) / each;
-  if (at_once > kRowsMost / 64) at_once = kRowsMost / 64;
-  for (uint64_t r = 0; r < rows; r += at_once) {
-    const uint32_t here = static_cast<uint32_t>(rows - r < at_once ? rows - r : at_once);
+                                 void* scratch, size_t most, hipStream_t stream) {
+  const LogprobPlan plan = plan_of(rows, vocab, top_k, scratch != nullptr ? most : 0);
+  for (uint64_t r = 0; r < rows; r += kLogprobRows) {
+    const uint32_t here = static_cast<uint32_t>(rows - r < kLogprobRows ? rows - r : kLogprobRows);
     LogprobArgs a{logits + (row_base + r) * vocab, tokens + r * count, logprobs + r * count, entropy + r,
                   top_k == 0 ? nullptr : top_tokens + r * top_k, top_k == 0 ? nullptr : top_logprobs + r * top_k, vocab, count, top_k,
                   plan.width, plan.tiles, plan.shares, nullptr, nullptr};

@@ -1512,11 +1512,11 @@ qmm_status run_token_logprobs(const LaunchCtx& c) {
   if (const char* why = qmm::check_token_logprobs(args_of(c))) return bad(why);
   const uint64_t rows = c.sc[0], vocab = c.sc[1], row_base = c.sc[4];
   const uint32_t count = static_cast<uint32_t>(c.sc[2]), top_k = static_cast<uint32_t>(c.sc[3]);
-  const size_t need = qmm::token_logprobs_scratch_bytes(rows, vocab, top_k, kPartsLimits.small - 16);
+  const size_t need = qmm::token_logprobs_scratch_bytes(rows, vocab, top_k, kPartsLimits.small);
   const StreamBlock block(c, need, g_parts_scratch);
   return map_hip(qmm::launch_token_logprobs(c.ptr<const float>(0), c.ptr<const uint32_t>(1), c.ptr<float>(2), c.ptr<float>(3),
                                             top_k == 0 ? nullptr : c.ptr<uint32_t>(4), top_k == 0 ? nullptr : c.ptr<float>(5), rows, vocab, count,
-                                            top_k, row_base, need == 0 ? nullptr : block.get(), need, c.stream));
+                                            top_k, row_base, need == 0 ? nullptr : block.get(), kPartsLimits.small, c.stream));
 }
 
 struct Entry {

@@ -274,11 +274,12 @@ hipError_t launch_tree_mask(const uint32_t* parents, uint32_t* mask, uint64_t* p
 // pos3 null: positions pos_base + row; gate null: none.
 hipError_t launch_qk_norm_rope(const QkNormCall& call, const float* q, const float* k, const float* wq, const float* wk, const uint64_t* pos3,
                                float* q_out, void* k_out, float* gate, hipStream_t stream);
-// token_logprobs_scratch_bytes: what the shares of rows take of `scratch`, at most `most`; null: rows are not shared.
+// token_logprobs_scratch_bytes: what the shares of rows take of `scratch`, 0 where they are not shared or would take more than
+// `most`; without scratch rows are not shared.
 size_t token_logprobs_scratch_bytes(uint64_t rows, uint64_t vocab, uint32_t top_k, size_t most);
 hipError_t launch_token_logprobs(const float* logits, const uint32_t* tokens, float* logprobs, float* entropy, uint32_t* top_tokens,
                                  float* top_logprobs, uint64_t rows, uint64_t vocab, uint32_t count, uint32_t top_k, uint64_t row_base,
-                                 void* scratch, size_t scratch_bytes, hipStream_t stream);
+                                 void* scratch, size_t most, hipStream_t stream);
 hipError_t launch_quantize_kv(const float* in, uint8_t* out, float* scale, uint64_t rows, uint64_t cols, uint32_t bits,
                               hipStream_t stream);
 hipError_t launch_cast_f32_f16(const float* in, void* out, uint64_t n, hipStream_t stream);
