@@ -261,15 +261,12 @@ struct RowsShared {
 // score counts for less; the tree's are its own.
 template <bool TREE>
 constexpr float kNoScore = TREE ? -INFINITY : -1e30f;
-// A part's largest score in natural units, `largest` of the matrix instructions' times `natural`, is rounded; its sums move by
-// what that took from it.  TREE: by 2^20 at most, so that they stay in range.  Rounding takes more from scores of 2^28 on only, whose
-// neighbours in fp32 are 32 apart.
+// A part's largest score in natural units is rounded; the sums move by what that took from it, in powers of two.  TREE: by 2^20 at
+// most, so that they stay in range.  Rounding takes more from scores of 2^28 on only, whose neighbours in fp32 are 32 apart.
 template <bool TREE>
-__device__ __forceinline__ float part_move(float largest, float natural) {
-  if (largest == -INFINITY) return 1.0f;
-  float moved = fmaf(largest, natural, -(largest * natural)) * kLog2E;
-  if constexpr (TREE) moved = fminf(fmaxf(moved, -20.0f), 20.0f);
-  return __builtin_amdgcn_exp2f(moved);
+__device__ __forceinline__ float part_move(float taken) {
+  const float by = taken * kLog2E;
+  return TREE ? fminf(fmaxf(by, -20.0f), 20.0f) : by;
 }
 
 // A part without keys, of heads head0 .. head0 + here - 1 of a row.
@@ -630,9 +627,10 @@ __device__ __forceinline__ void attend_row(const AttentionArgs& a, uint64_t row,
     if (TREE && !(fabsf(acc) < INFINITY && fabsf(sum) < INFINITY)) pairs->special = 1u;
     if (a.part.split != 0) {
       const uint64_t at = (TREE ? static_cast<uint64_t>(pairs->at[h]) : row * a.heads + head0 + h) * split + s_part;
-      const float natural = scale * kLn2, moved = part_move<TREE>(m, natural);
+      const float natural = scale * kLn2, largest = m * natural;
+      const float moved = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(part_move<TREE>(fmaf(m, natural, -largest)));
       a.part.pacc[at * D + d] = acc * moved;
-      if (d == 0) a.part.pmax[at] = m * natural, a.part.psum[at] = sum * moved;
+      if (d == 0) a.part.pmax[at] = largest, a.part.psum[at] = sum * moved;
     } else {
       a.out[(TREE ? static_cast<uint64_t>(pairs->at[h]) : (a.row_base + row) * a.heads + head0 + h) * D + d] = TREE && sum == 0.0f ? 0.0f : acc / sum;
     }
@@ -1133,9 +1131,9 @@ __global__ __launch_bounds__(512, 2) void attention_tile_kernel(AttentionArgs a)
   if (split > 1u) {
     const uint64_t part = (own.row * a.heads + own.head) * split + s_part;
     out = a.part.pacc + part * D;
-    const float most = sh.most[at], natural = score_scale * kLn2;
-    factor = part_move<false>(most, natural);
-    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(most * natural, kNoScore<false>), a.part.psum[part] = total * factor;
+    const float most = sh.most[at], natural = score_scale * kLn2, largest = most * natural;
+    factor = most == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(part_move<false>(fmaf(most, natural, -largest)));
+    if (late_g == 0u && half == 0u) a.part.pmax[part] = fmaxf(largest, kNoScore<false>), a.part.psum[part] = total * factor;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
