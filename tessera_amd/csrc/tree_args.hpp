@@ -74,7 +74,7 @@ inline const char* check_qk_norm(const LaunchArgs& c, bool axes, QkNormCall* out
   }
   if (a.rows > (1u << 24) || a.heads > (1u << 16) || a.kv_heads > (1u << 16) || a.pos_base > (uint64_t{1} << 48) ||
       a.q_stride > (uint64_t{1} << 32) || a.k_stride > (uint64_t{1} << 32) || a.k_row > (uint64_t{1} << 40) || a.k_f16 > 1 ||
-      a.rows * (a.heads + a.kv_heads) > 0x3FFFFFFull) {
+      a.rows * (a.heads + a.kv_heads) > 0x3FFFFFCull) {               // (a wavefront each: fewer than 2^32 threads)
     return "qk_norm_rope/mrope: a scalar is out of range";
   }
   if (!(a.theta > 0.0f) || a.theta > 3.4e38f || !(a.eps >= 0.0f) || a.eps > 3.4e38f) return "qk_norm_rope/mrope: theta must be positive, eps not negative, both finite";
