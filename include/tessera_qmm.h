@@ -31,8 +31,9 @@
  *     their own, 16 MB for the eager launches of each stream and what they need for each capture and
  *     stream that records them: "gemm_fp8" from 17 rows (128 MB more where a call does not fit) and
  *     "gemm_q5k*" / "gemm_q6k*" with 2..16 rows out of the 256 MB that qmm_init reserves, then out of slabs of
- *     128 MB, 2 GB in all; "attention", "attention_q8", "_q4" and "_fp8" from 17 rows, "attention_tree" and its forms over
- *     long caches, "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
+ *     128 MB, 2 GB in all; "attention", "attention_q8", "_q4" and "_fp8" from 17 rows, "attention_tree" and its forms
+ *     over long caches, "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in
+ *     all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
  *     workspace has no room for what they hand on (a caller's of just the operands, a capture before the library's
  *     has grown) likewise, 16 to 40 MB out of slabs of 128 MB, 1 GB in all; qmm_set_workspace reserves the first.
  *     While a caller's workspace is set no slab is allocated.  The blocks are not given back (a graph may
@@ -167,32 +168,38 @@ const char* qmm_kernel_name(size_t index);
  *     softmax weights likewise (over a quantized cache a weight times its value's scale, down to 2^-18 of
  *     the row's largest); keys and values enter as the cache holds them, scores and sums are fp32.  Over
  *     an fp32 cache everything is fp32.
- *   - the verification of a tree of drafted tokens, for which the reference has no ids.  Node i of the tree follows node
- *     parents[i] < i or, for 0xFFFFFFFF, the cache's last token; the tree's keys are the cache's last.  Launches of these
- *     ids may be made on any streams at once.
- *     "tree_mask": buffers Parents (u32 a node), Mask (nodes x ceil(nodes / 32) u32: bit j % 32 of word j / 32, the row sees
- *     node j: its ancestors and itself), Positions (nodes x 3 u64, base plus depth, as "mrope" takes them); scalars nodes
- *     (1 to 1024), base.  A parent that is no earlier node marks padding: it and what follows it see nothing, at `base`.
- *     "qk_norm_rope": "rmsnorm" of every head of Q and K and "rope" of the result, in one launch.  Buffers Q (rows of q_stride floats:
- *     heads x head_dim, with Gate bound heads x (query, gate) as "qgate_split" takes them), K (rows of k_stride floats), Wq, Wk
- *     (head_dim each), Qout (rows x heads*head_dim), Kout (from row k_row on: rows of kv_heads*head_dim, fp32 or, with k_f16 =
- *     1, fp16 to nearest), optionally Gate (as Qout); scalars rows, heads, kv_heads, head_dim (even, at most 256), rope_dim,
- *     pos_base, theta, epsilon (fp32 bits), q_stride, k_stride (0: rows side by side), k_f16, k_row.  "qk_norm_mrope": Pos
- *     (rows x 3 u64) after Wk, no pos_base, and sec_t, sec_h, sec_w at the end, as "mrope".  Angles are formed in fp64, positions
- *     above 2^50 as 2^50.  Qout may be Q and Kout K where they are laid out alike.
- *     "attention_tree": buffers Q, K, V, Mask, Out; scalars m, n, heads, kv_heads, head_dim (at most 256), tree (1 to 65536), window, kv_f16
- *     (0: K and V fp32, 1: fp16).  Row i sees the first n - tree keys and those of the last `tree` that row i of Mask (m x ceil(tree
- *     / 32) words, as "tree_mask" writes it) names, and of all these the last `window` (0: all).  A row that sees no key, or none
- *     with a score above -infinity, becomes zeros; a key that a row does not see does not reach it, whatever it holds.  Scores may be as
- *     large as fp32 holds their sums of products.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask, Out over the caches of "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but for calls
- *     whose rows share their keys (many rows on many keys, by the time that they are estimated to take): there a softmax weight (over
- *     fp32 and quantized caches times its value's largest element or scale) is carried to 2^-23 of itself down to 2^-11 of the row's
- *     largest, and below to 2^-34 of that, and fp32 keys and values to 2^-23 of an element down to 2^-28 of its key's largest,
- *     below to 2^-50 of that, a product to 2^-22.
- *     "token_logprobs": buffers Logits (row_base + rows rows of vocab floats), Tokens (rows x tokens u32), Logprobs (rows x
- *     tokens: log softmax of the row at each token, -infinity for one of vocab or more), Entropy (rows) and, with top_k, TopTokens (rows x top_k u32),
- *     TopLogprobs; scalars rows, vocab, tokens (1 to 1024), top_k (0 to 32), row_base.  The largest entries in descending order,
- *     equal ones by their column; -infinity is a banned entry, of probability 0.
+ *   - the verification of a tree of drafted tokens, for which the reference has no ids.  Node i of the tree follows
+ *     node parents[i] < i or, for 0xFFFFFFFF, the cache's last token; the tree's keys are the cache's last.
+ *     Launches of these ids may be made on any streams at once.
+ *     "tree_mask": buffers Parents (u32 a node), Mask (nodes x ceil(nodes / 32) u32: bit j % 32 of word j / 32, the
+ *     row sees node j: its ancestors and itself), Positions (nodes x 3 u64, base plus depth, as "mrope" takes
+ *     them); scalars nodes (1 to 1024), base.  A parent that is no earlier node marks padding: it and what follows
+ *     it see nothing, at `base`.
+ *     "qk_norm_rope": "rmsnorm" of every head of Q and K and "rope" of the result, in one launch.  Buffers Q (rows
+ *     of q_stride floats: heads x head_dim, with Gate bound heads x (query, gate) as "qgate_split" takes them), K
+ *     (rows of k_stride floats), Wq, Wk (head_dim each), Qout (rows x heads*head_dim), Kout (from row k_row on:
+ *     rows of kv_heads*head_dim, fp32 or, with k_f16 = 1, fp16 to nearest), optionally Gate (as Qout); scalars
+ *     rows, heads, kv_heads, head_dim (even, at most 256), rope_dim, pos_base, theta, epsilon (fp32 bits),
+ *     q_stride, k_stride (0: rows side by side), k_f16, k_row.  "qk_norm_mrope": Pos (rows x 3 u64) after Wk, no
+ *     pos_base, and sec_t, sec_h, sec_w at the end, as "mrope".  Angles are formed in fp64, positions above 2^50 as
+ *     2^50.  Qout may be Q and Kout K where they are laid out alike.
+ *     "attention_tree": buffers Q, K, V, Mask, Out; scalars m, n, heads, kv_heads, head_dim (at most 256), tree (1
+ *     to 65536), window, kv_f16 (0: K and V fp32, 1: fp16).  Row i sees the first n - tree keys and those of the
+ *     last `tree` that row i of Mask (m x ceil(tree / 32) words, as "tree_mask" writes it) names, and of all these
+ *     the last `window` (0: all).  A row that sees no key, or none with a score above -infinity, becomes zeros; a
+ *     key that a row does not see does not reach it, whatever it holds (but values that no row sees should be
+ *     finite: NaN among them cost some hundred times the time).  Scores may be as large as fp32 holds their sums of
+ *     products.  "attention_tree_q8", "_q4", "_fp8": Q, K, V, Ks, Vs, Mask, Out over the caches of
+ *     "attention_q8", "_q4", "_fp8"; without kv_f16.  Numerics as the attention ids above, but for calls whose rows
+ *     share their keys (many rows on many keys, by the time that they are estimated to take): there a softmax
+ *     weight (over fp32 and quantized caches times its value's largest element or scale) is carried to 2^-23 of
+ *     itself down to 2^-11 of the row's largest, and below to 2^-34 of that, and fp32 keys and values to 2^-23 of
+ *     an element down to 2^-28 of its key's largest, below to 2^-50 of that, a product to 2^-22.
+ *     "token_logprobs": buffers Logits (row_base + rows rows of vocab floats), Tokens (rows x tokens u32), Logprobs
+ *     (rows x tokens: log softmax of the row at each token, -infinity for one of vocab or more), Entropy (rows)
+ *     and, with top_k, TopTokens (rows x top_k u32), TopLogprobs; scalars rows, vocab, tokens (1 to 1024), top_k (0
+ *     to 32), row_base.  The largest entries in descending order, equal ones by their column; -infinity is a banned
+ *     entry, of probability 0.  NaN or +infinity in a row, or -infinity alone, make its results but the tokens NaN.
  *   - "mfma_probe": buffer Out (workgroups * 256 floats); scalars kind (0 fp16 32x32x16, 1 scaled
  *     fp8 x fp4 32x32x64, 2 int8 16x16x64), random (0 constant operands, 1 hashed), iterations,
  *     workgroups.  "read_probe": a plain read of a buffer.  Measurement ids: the matrix-core and the

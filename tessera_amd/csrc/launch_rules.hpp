@@ -227,13 +227,13 @@ constexpr uint64_t attention_rule(const AttentionCall& a, uint64_t cus, uint64_t
 // How a call runs: a workgroup a row and key head, at most eight heads (sixteen over fp32 keys); or sixteen (row, head) pairs of a
 // key head, fp32 keys only; or 64 that share their keys, 64 at a time (`tile`); and the parts of the keys.  The shortest of the
 // estimated times, in us: a fixed part, the rounds of workgroups that the chip holds, each with a part of its own and what its
-// keys take, and for parts the second launch and the sums' way through memory.  Fitted to 9010 calls of 620 shapes (1 to 64
-// rows, 1 to 30000 keys, 1 to 64 heads over 1 to 8 key heads of 64 to 256, all kinds of cache), which they meet within 10 % on
-// average: the way taken is 1.5 % over the best of those measured on average, 28 % at most.  A workgroup a row and key head /
+// keys take, and for parts the second launch and the sums' way through memory.  Fitted to 600 calls run in 9348 ways (1 to 64
+// rows, 1 to 30000 keys, 1 to 64 heads over 1 to 8 key heads of 64 to 256, all kinds of cache; profiles/tree_rule_times.csv): the
+// way taken is 1.6 % over the fastest of them on average, 5 % in nine calls of ten, 35 % at most.  A workgroup a row and key head /
 // shared keys, each in its best number of parts: 1 row of 48 heads over 8 of 128 on 18168 4-bit keys 15 / 22, 10 rows of 12 heads
 // over 2 of 64 on 62 5.8 / 7.1, 13 rows of 6 over 2 of 256 on 13892 fp16 keys 46 / 22, 59 rows of 24 over 4 of 128 on 11138
 // 113 / 32; a row's heads / sixteen pairs / shared keys, fp32: 7 rows of 6 heads over 2 of 64 on 8199 12 / 11 / 15, 24 of 8 over 2 of 256
-// on 71 15 / 20 / 16, 64 of 24 over 4 of 256 on 8192 428 / 220 / 85.
+// on 71 15 / 20 / 16, 64 of 24 over 4 of 256 on 8192 428 / 220 / 87.
 struct TreeCall {
   uint64_t rows, keys, heads, kv_heads, head_dim, padded;   // keys: that a row sees at most; padded: the head size, 64, 128 or 256
   bool fp32, quantized;
@@ -253,10 +253,18 @@ constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_par
     bool whole;
     double pair = 0.0;
   };
-  constexpr Times kRows[3] = {{4.7, 0.48, 0.0056, 1.23, 0.81, 2.6, 3.0, false}, {3.5, 2.76, 0.0089, 1.04, 0.76, 2.6, 1.1, false}, {2.35, 6.2, 0.0196, 1.02, 1.0, 3.2, 1.96, true}};
-  constexpr Times kRowsF32[3] = {{4.57, 0.55, 0.0128, 1.0, 0.84, 3.0, 1.44, false, 0.017}, {4.76, 1.48, 0.0245, 1.0, 0.76, 3.13, 2.3, false, 0.039}, {3.59, 4.86, 0.0519, 1.0, 0.8, 3.74, 2.35, false, 0.19}};
-  constexpr Times kTiles[3] = {{4.85, 0.27, 0.706, 1.36, 2.0, 3.0, 1.77, true}, {3.42, 2.55, 0.93, 1.35, 1.0, 3.05, 1.08, true}, {2.3, 5.6, 1.41, 1.29, 1.0, 4.3, 0.89, true}};
-  constexpr Times kTilesF32[3] = {{4.0, 0.71, 2.13, 1.0, 2.0, 3.16, 1.71, true}, {5.4, 0.4, 3.02, 1.0, 1.0, 3.16, 1.17, true}, {7.9, 0.0, 4.98, 1.0, 1.0, 4.1, 1.05, true}};
+  constexpr Times kRows[3] = {{4.7, 0.48, 0.0056, 1.23, 0.81, 2.6, 3.0, false},
+                              {3.5, 2.76, 0.0089, 1.04, 0.76, 2.6, 1.1, false},
+                              {2.35, 6.2, 0.0196, 1.02, 1.0, 3.2, 1.96, true}};
+  constexpr Times kRowsF32[3] = {{4.57, 0.55, 0.0128, 1.0, 0.84, 3.0, 1.44, false, 0.017},
+                                 {4.76, 1.48, 0.0245, 1.0, 0.76, 3.13, 2.3, false, 0.039},
+                                 {3.59, 4.86, 0.0519, 1.0, 0.8, 3.74, 2.35, false, 0.19}};
+  constexpr Times kTiles[3] = {{4.85, 0.27, 0.706, 1.36, 2.0, 3.0, 1.77, true},
+                               {3.42, 2.55, 0.93, 1.35, 1.0, 3.05, 1.08, true},
+                               {2.3, 5.6, 1.41, 1.29, 1.0, 4.3, 0.89, true}};
+  constexpr Times kTilesF32[3] = {{4.0, 0.71, 2.13, 1.0, 2.0, 3.16, 1.71, true},
+                                  {5.4, 0.4, 3.02, 1.0, 1.0, 3.16, 1.17, true},
+                                  {7.9, 0.0, 4.98, 1.0, 1.0, 4.1, 1.05, true}};
   const int size = a.padded == 64 ? 0 : a.padded == 128 ? 1 : 2;
   const uint64_t group = a.heads / a.kv_heads, fit = a.fp32 ? 16 : 8, own = group < fit ? group : fit;
   TreeShape best{false, own, 1};
@@ -268,13 +276,15 @@ constexpr TreeShape tree_rule(const TreeCall& a, uint64_t cus, uint64_t most_par
     const uint64_t units = tree_units(a, pairs);
     const double slots = static_cast<double>(cus) * t.at_once;
     const uint64_t fill = static_cast<uint64_t>(slots) / units;        // parts that fill the chip
-    for (uint64_t parts : {uint64_t{1}, uint64_t{2}, uint64_t{3}, uint64_t{4}, uint64_t{6}, uint64_t{8}, uint64_t{12}, uint64_t{16}, uint64_t{24}, uint64_t{32}, uint64_t{48},
-                           uint64_t{64}, fill}) {
-      if (parts == 0 || (parts > 1 && (parts > most_parts || a.keys / parts < 48 || attention_parts_size(a.rows, a.heads, a.head_dim, parts) > most_bytes))) continue;
+    for (uint64_t parts : {uint64_t{1}, uint64_t{2}, uint64_t{3}, uint64_t{4}, uint64_t{6}, uint64_t{8}, uint64_t{12}, uint64_t{16},
+                           uint64_t{24}, uint64_t{32}, uint64_t{48}, uint64_t{64}, fill}) {
+      if (parts == 0 || (parts > 1 && (parts > most_parts || a.keys / parts < 48))) continue;
+      if (parts > 1 && attention_parts_size(a.rows, a.heads, a.head_dim, parts) > most_bytes) continue;
       const uint64_t each = (a.keys + parts - 1) / parts, groups = units * parts;
       double rounds = static_cast<double>(groups) / slots;
       if (t.whole) rounds = static_cast<double>((groups + static_cast<uint64_t>(slots) - 1) / static_cast<uint64_t>(slots));
-      double us = t.fixed + (rounds < 1.0 ? 1.0 : rounds) * (t.round + t.pair * static_cast<double>(pairs) + t.keys * (a.quantized ? t.quantized : 1.0) * static_cast<double>(tile ? (each + 63) / 64 : each));
+      const double walk = t.keys * (a.quantized ? t.quantized : 1.0) * static_cast<double>(tile ? (each + 63) / 64 : each);
+      double us = t.fixed + (rounds < 1.0 ? 1.0 : rounds) * (t.round + t.pair * static_cast<double>(pairs) + walk);
       if (parts > 1) us += t.parts + t.megabyte * static_cast<double>(a.rows * a.heads * parts * a.head_dim * 4) * 1e-6;
       if (least < 0.0 || us < least) least = us, best = TreeShape{tile, pairs, parts};
     }

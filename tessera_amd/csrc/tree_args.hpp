@@ -77,7 +77,9 @@ inline const char* check_qk_norm(const LaunchArgs& c, bool axes, QkNormCall* out
       a.rows * (a.heads + a.kv_heads) > 0x3FFFFFCull) {               // (a wavefront each: fewer than 2^32 threads)
     return "qk_norm_rope/mrope: a scalar is out of range";
   }
-  if (!(a.theta > 0.0f) || a.theta > 3.4e38f || !(a.eps >= 0.0f) || a.eps > 3.4e38f) return "qk_norm_rope/mrope: theta must be positive, eps not negative, both finite";
+  if (!(a.theta > 0.0f) || a.theta > 3.4e38f || !(a.eps >= 0.0f) || a.eps > 3.4e38f) {
+    return "qk_norm_rope/mrope: theta must be positive, eps not negative, both finite";
+  }
   if (axes) {
     const uint64_t sec_w = s[8];
     if (a.sec_t > a.rope_dim || a.sec_h > a.rope_dim || sec_w > a.rope_dim || a.sec_t + a.sec_h + sec_w > a.rope_dim / 2) {

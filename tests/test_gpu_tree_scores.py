@@ -10,8 +10,8 @@ from test_gpu_tree import attend_tree, elements
 pytestmark = pytest.mark.gpu
 
 # few rows and many, keys in one part and in several (launch_rules.hpp: tree_rule), head sizes of the matrix kernels and not
-CASES = [(1, 40, 4, 2, 64), (3, 3000, 4, 2, 128), (2, 5000, 8, 2, 256), (40, 120, 8, 2, 64), (40, 130, 8, 2, 256), (40, 3000, 8, 2, 64), (40, 3000, 8, 2, 128),
-         (40, 2500, 12, 2, 256), (5, 100, 8, 4, 34), (3, 2000, 4, 2, 34)]
+CASES = [(1, 40, 4, 2, 64), (3, 3000, 4, 2, 128), (2, 5000, 8, 2, 256), (40, 120, 8, 2, 64), (40, 130, 8, 2, 256),
+         (40, 3000, 8, 2, 64), (40, 3000, 8, 2, 128), (40, 2500, 12, 2, 256), (5, 100, 8, 4, 34), (3, 2000, 4, 2, 34)]
 
 
 def one_key_leads(backend, kind, case, size, lead):
