@@ -32,15 +32,15 @@
  *     stream that records them: "gemm_fp8" from 17 rows (128 MB more where a call does not fit) and
  *     "gemm_q5k*" / "gemm_q6k*" with 2..16 rows out of the 256 MB that qmm_init reserves, then out of slabs of
  *     128 MB, 2 GB in all; "attention", "attention_q8", "_q4" and "_fp8" from 17 rows, "attention_tree" and its forms
- *     over long caches, "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in
+ *     and "attention_pages_*" over long caches, "draft_verify", "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in
  *     all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
  *     workspace has no room for what they hand on (a caller's of just the operands, a capture before the library's
  *     has grown) likewise, 16 to 40 MB out of slabs of 128 MB, 1 GB in all; qmm_set_workspace reserves the first.
  *     While a caller's workspace is set no slab is allocated.  The blocks are not given back (a graph may
  *     still use them), and a stream handle's block passes to the next stream with that handle: let a
  *     stream's launches finish before it is destroyed.  A launch that gets no block, or is made on
- *     hipStreamPerThread, runs kernels that need none (slower; "top_k_rows" and the products of Q4_K, Q5_K and Q6_K with
- *     the same bits, the others with sums in another order).
+ *     hipStreamPerThread, runs kernels that need none (slower; "top_k_rows", "draft_verify" and the products of Q4_K, Q5_K and Q6_K
+ *     with the same bits, the others with sums in another order).
  */
 #ifndef TESSERA_QMM_H_
 #define TESSERA_QMM_H_
@@ -200,6 +200,47 @@ const char* qmm_kernel_name(size_t index);
  *     and, with top_k, TopTokens (rows x top_k u32), TopLogprobs; scalars rows, vocab, tokens (1 to 1024), top_k (0
  *     to 32), row_base.  The largest entries in descending order, equal ones by their column; -infinity is a banned
  *     entry, of probability 0.  NaN or +infinity in a row, or -infinity alone, make its results but the tokens NaN.
+ *   - a batch of sequences in a paged cache of 8-bit keys and values, for which the reference has no ids.  A page holds
+ *     `block` (16, 32, 64 or 128) positions of one sequence: keys Kp [page][kv_head][position][element], values Vp
+ *     [page][kv_head][element][position], int8 codes ("_q8") or E4M3 ones ("_fp8"), an element code * scale under one
+ *     fp32 scale for each page and key head (Ks, Vs: pages x kv_heads).  Page j of sequence s is Table[s * width + j]
+ *     (u32).  Rows Starts[s] .. Starts[s + 1] - 1 of a call (u32, sequences + 1 of them) are the last positions of
+ *     sequence s, of which there are then Lens[s] (u32): one row in decode, a few with drafted tokens, many in prefill,
+ *     none for a sequence that rests.  Starts, Lens and Table are read on the device, so that one recorded launch serves
+ *     every step.  A sequence whose numbers do not hold (rows past the call's, more rows than positions, more positions
+ *     than width * block) is left out, as are rows of no sequence: what they would have written stays as it was.
+ *     head_dim is a multiple of 16, at most 256; at most 4096 sequences of 2^30 positions.  Launches of these ids may be
+ *     made on any streams at once; two sequences may share pages that neither writes.
+ *     "pages_write_q8", "pages_write_fp8": buffers K, V (rows of k_stride and v_stride floats, a multiple of 4; 0: side by
+ *     side), Table, Starts, Lens, Kp, Vp, Ks, Vs; scalars rows, kv_heads, head_dim, sequences, block, pages, width,
+ *     k_stride, v_stride.  The rows' keys and values go into their pages.  A page and head's scale becomes the larger of
+ *     its own, where it holds earlier positions, and the rows' largest magnitude / 127 (E4M3: 448); where it grows the
+ *     earlier positions are quantized again, from what they stood for.  Codes are the nearest to x / scale, ties to even;
+ *     behind the rows a page is 0.  An infinity or NaN makes its page and head NaN until it is begun anew.  So an element is
+ *     off by half a step (of the last scale) and half a step more for every time that its page's scale grew.  Rows of
+ *     unknown pages (a number of `pages` or more) are lost.
+ *     "pages_read_q8", "pages_read_fp8": buffers Kp, Vp, Ks, Vs, Table, Starts, Lens, K, V (rows x kv_heads*head_dim, fp32 or
+ *     with out_f16 = 1 fp16); scalars rows, kv_heads, head_dim, sequences, block, pages, width, out_f16.  The rows back:
+ *     code * scale, rounded to fp32 and then to fp16; zeros of unknown pages.
+ *     "attention_pages_q8", "attention_pages_fp8": buffers Q (rows x heads*head_dim), Kp, Vp, Ks, Vs, Table, Starts, Lens, Out (as
+ *     Q); scalars rows, heads, kv_heads, head_dim, sequences, block, pages, width, max_rows, max_len, window, sinks.  Each
+ *     row sees the positions up to its own; under a window (not 0) the last `window` of them and the first `sinks` of the
+ *     sequence.  Positions of unknown pages are not seen; a row that sees nothing becomes zeros, and what a row does not
+ *     see does not reach it.  max_rows, max_len: the most rows and positions that a sequence has (0: rows, width * block),
+ *     which the launch is shaped by; a sequence with more is left out.  Numerics as "attention_tree" where rows share their
+ *     keys: scores and sums fp32, a query's element to 2^-22 of itself down to 2^-16 of its head's largest (2^-38 of that
+ *     below), a weight times its value's scale to 2^-22 of itself down to 2^-12 of the row's largest (2^-34 of that below).
+ *     "draft_verify": buffers Logits (rows x vocab floats), Tokens (rows u32), Random (rows x 2 floats in [0, 1)), Starts,
+ *     Accepted, Next (sequences u32)[, DraftLogits (as Logits)]; scalars rows, vocab, sequences, temperature,
+ *     draft_temperature (fp32 bits).  Row i of a sequence holds the target's logits behind Tokens[i]; Tokens[i + 1] was
+ *     drafted there, but for the last row, from DraftLogits' row i (without DraftLogits: it was the only choice, q = 1).
+ *     With p = softmax(logits / temperature), q the draft's: a draft x stands where Random[i][0] q(x) < p(x).  Accepted:
+ *     how many stand before the first that does not; Next: the token behind them, the first whose running sum of
+ *     max(p - q, 0) there (without DraftLogits: of p but for x; where nothing is left, or behind the last row: of p)
+ *     exceeds Random[i][1] of the whole.  All in fp64.  temperature 0: a draft stands where it is the row's largest logit,
+ *     the lowest of equals, and Next is that.  -infinity is a token of probability 0.  A row that holds NaN or +infinity or
+ *     nothing but -infinity (the draft's likewise, where it is needed) ends the draft there, with Next 0xFFFFFFFF.  A token
+ *     of vocab or more never stands.  vocab is at most 2^24.
  *   - "mfma_probe": buffer Out (workgroups * 256 floats); scalars kind (0 fp16 32x32x16, 1 scaled
  *     fp8 x fp4 32x32x64, 2 int8 16x16x64), random (0 constant operands, 1 hashed), iterations,
  *     workgroups.  "read_probe": a plain read of a buffer.  Measurement ids: the matrix-core and the

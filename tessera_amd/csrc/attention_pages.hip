@@ -1,0 +1,502 @@
+// "attention_pages_q8", "attention_pages_fp8": the rows of a batch of sequences against their pages of 8-bit keys and values.
+//
+// Row i of a sequence, at position p, sees the positions up to p; under a window those of them that are among the last `window` or
+// the first `sinks` of the sequence.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = q . k_j / sqrt(head_dim), in one pass
+// over the keys with a running reference m.
+//
+// What is fp32 enters the fp16 matrix instructions as two terms, x = hi + lo, hi = RN16(x), lo = RN16(x - hi), under a power of two.
+// It brings a query's largest element to 2^13 .. 2^14: an element is carried to 2^-22 of itself down to 2^-16 of the largest, below to
+// 2^-38 of that.  It brings the largest of a row's weights times their values' scales so far to 2^9 .. 2^15: to 2^-22 of itself down
+// to 2^-12 of the largest, below to 2^-34 of that.  Codes enter exactly; a key's scale multiplies its fp32 score.  Scores, references,
+// sums and results are fp32.
+
+#include <type_traits>
+
+#include "launch_rules.hpp"
+#include "pages.hpp"
+#include "qmm_kernels.hpp"
+
+namespace qmm {
+namespace {
+
+constexpr float kLog2E = 1.44269504088896340736f;
+
+struct PageAttention {
+  PageBatch batch;
+  const float* q;
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  float* out;
+  float *part_sum, *part_most, *part_total;   // (unit, key head, part, column): head_dim sums; the reference in powers of two; the weights' sum
+  uint32_t heads, group, window, sinks;       // window 0: every position
+  uint32_t parts, part_tiles;                 // tiles of 64 positions a part
+};
+
+// ---- which positions a unit walks ----------------------------------------------------------------
+//
+// A unit is COLUMNS (row, head) pairs of a key head in one sequence, `group` pairs to a row.  It walks tiles of 64 positions: those with
+// sinks that lie before its windows, then those from the first row's window to the last row's position.
+struct UnitTiles {
+  uint32_t columns;               // that there are
+  uint32_t first_col;             // its first among the sequence's
+  uint32_t low, high;             // the first and the last row's positions
+  uint32_t sink_tiles, from_tile, tiles;
+};
+__device__ __forceinline__ UnitTiles unit_tiles(const PageAttention& a, const PageUnit& u, uint32_t most_columns) {
+  UnitTiles w;
+  const uint32_t all = u.seq.rows * a.group;
+  w.first_col = u.at * most_columns;
+  w.columns = all - w.first_col < most_columns ? all - w.first_col : most_columns;
+  const uint32_t past = u.seq.len - u.seq.rows;
+  w.low = past + w.first_col / a.group, w.high = past + (w.first_col + w.columns - 1u) / a.group;
+  const uint32_t begin = a.window != 0u && w.low + 1u > a.window ? w.low + 1u - a.window : 0u;
+  const uint32_t sinks = a.sinks < begin ? a.sinks : begin;
+  w.sink_tiles = (sinks + 63u) / 64u;
+  w.from_tile = begin / 64u > w.sink_tiles ? begin / 64u : w.sink_tiles;
+  w.tiles = w.sink_tiles + (w.high / 64u + 1u - w.from_tile);
+  return w;
+}
+__device__ __forceinline__ uint32_t tile_at(const UnitTiles& w, uint32_t i) { return i < w.sink_tiles ? i : w.from_tile + (i - w.sink_tiles); }
+
+// ---- operands ------------------------------------------------------------------------------------
+
+// Eight codes (two dwords) as fp16.  The half 0x6400 | u is 1024 + u.
+template <PageKind KIND>
+__device__ __forceinline__ half8_t operand(uint32_t w0, uint32_t w1) {
+  if constexpr (KIND == PageKind::Q8) {
+    auto two = [](uint32_t biased, uint32_t sel) {
+      const half2_t x = bit_cast<half2_t>(__builtin_amdgcn_perm(0x64646464u, biased, sel));
+      return bit_cast<uint32_t>(x - half2_t{static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)});
+    };
+    const uint32_t x = w0 ^ 0x80808080u, y = w1 ^ 0x80808080u;
+    return bit_cast<half8_t>(uint4{two(x, 0x04010400u), two(x, 0x04030402u), two(y, 0x04010400u), two(y, 0x04030402u)});
+  } else {
+    auto two = [](uint32_t w, auto high) { return bit_cast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, decltype(high)::value)); };
+    return bit_cast<half8_t>(uint4{two(w0, std::false_type{}), two(w0, std::true_type{}), two(w1, std::false_type{}), two(w1, std::true_type{})});
+  }
+}
+
+// Largest / sum over the four groups of sixteen lanes.
+__device__ __forceinline__ float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  v = fmaxf(bit_cast<float>(a[0]), bit_cast<float>(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return fmaxf(bit_cast<float>(b[0]), bit_cast<float>(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  v = bit_cast<float>(a[0]) + bit_cast<float>(a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(v), bit_cast<uint32_t>(v), false, false);
+  return bit_cast<float>(b[0]) + bit_cast<float>(b[1]);
+}
+// 2^(target - exponent of v) for v > 0, within what fp32 can hold.
+__device__ __forceinline__ float power_to(float v, int target) {
+  const int s = 254 + target - static_cast<int>(bit_cast<uint32_t>(v) >> 23 & 255u);
+  return bit_cast<float>(static_cast<uint32_t>(s > 254 ? 254 : s < 1 ? 1 : s) << 23);
+}
+__device__ __forceinline__ float from_reference(float ref) { return ref == -INFINITY ? 0.0f : ref; }
+
+// Weights are taken relative to a reference that follows a column's largest score only where that would leave it by 2^kSlack.
+constexpr float kSlack = 3.0f;
+
+// A column's running state in one wavefront: lanes r, 16 + r, 32 + r, 48 + r hold a quarter of each tile's positions.
+struct Column {
+  float ref = -INFINITY;          // in powers of two
+  float sum = 0.0f;               // of weights, this lane's share
+  float most = 0.0f;              // the largest weight times value scale so far, this lane's
+  float up = 0x1p127f;            // the power of two over those
+};
+
+// Scores (in powers of two) to weights times the values' scale, as two terms; returns what the sums so far are to be scaled by.
+// COUNT of a lane's positions of the tile; bit i of `shown`: the column sees the i-th.
+template <int COUNT>
+__device__ __forceinline__ float weigh(Column& c, float (&s)[COUNT], uint32_t shown, bool all, float v_scale, half8_t (&hi)[COUNT / 8], half8_t (&lo)[COUNT / 8]) {
+  if (!all) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) s[i] = (shown >> i & 1u) != 0u ? s[i] : -INFINITY;
+  }
+  float most = s[0];
+#pragma unroll
+  for (int i = 1; i < COUNT; ++i) most = fmaxf(most, s[i]);
+  float corr = 1.0f;
+  const bool moves = __any(most > c.ref + kSlack || (c.ref == -INFINITY && most > -INFINITY));
+  if (moves) {
+    const float before = c.ref;
+    c.ref = fmaxf(c.ref, groups_max(most));
+    corr = before == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - c.ref);
+    c.sum *= corr, c.most *= corr;
+  }
+  const float to = from_reference(c.ref);
+  const float here = __builtin_amdgcn_exp2f(most - to) * v_scale;
+  c.most = fmaxf(c.most, here);
+  if (moves || __any(!(here * c.up < 0x1p15f))) {
+    const float largest = groups_max(c.most), scaled = largest * c.up;
+    if (largest > 0.0f && !(scaled >= 0x1p9f && scaled < 0x1p15f)) {
+      const float up = power_to(largest, 13);
+      corr *= up / c.up;
+      c.up = up;
+    }
+  }
+  const float factor = v_scale * c.up;
+  float w[COUNT];
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    const float p = __builtin_amdgcn_exp2f(s[i] - to);
+    c.sum += p;
+    w[i] = p * factor;
+  }
+  if (!all) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) w[i] = (shown >> i & 1u) != 0u ? w[i] : 0.0f;     // (a hidden value's scale may be NaN)
+  }
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i) {
+    const _Float16 h = static_cast<_Float16>(w[i]);
+    hi[i / 8][i % 8] = h;
+    lo[i / 8][i % 8] = static_cast<_Float16>(w[i] - static_cast<float>(h));
+  }
+  return corr;
+}
+
+// ---- few columns ---------------------------------------------------------------------------------
+//
+// Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of 64 positions on its own, with no LDS
+// before the merge.  v_mfma_f32_16x16x32_f16 twice: S^T = K Q^T, O^T = V^T P^T.  Row 4 g + e of the t-th of a tile's four key operands is
+// position 16 g + 4 t + e, so that lane group g ends up with the scores of the tile's positions 16 g .. 16 g + 15 (which lie
+// in one page: one scale a lane), and those are the sixteen of the value operands that it loads: no score changes its lane.
+template <int DP, int CG, int NW>
+struct FewShared {
+  float ref[NW][16 * CG], sum[NW][16 * CG];
+  alignas(16) float o[NW][16 * CG][DP + 4];
+};
+
+template <PageKind KIND, int DP, int CG, int NW>
+__global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttention a) {
+  constexpr int KL = DP / 64, VL = DP / 16, STEPS = DP / 32, C = 16 * CG;
+  __shared__ FewShared<DP, CG, NW> sh;
+  const PageBatch& b = a.batch;
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
+  const uint32_t kv = blockIdx.x % b.kv_heads, rest = blockIdx.x / b.kv_heads, part = rest % a.parts, unit = rest / a.parts;
+  PageUnit u;
+  if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
+  const UnitTiles w = unit_tiles(a, u, C);
+  const uint32_t begin = part * a.part_tiles;
+  if (begin >= w.tiles) return;                                     // workgroup-uniform
+  const uint32_t end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
+  const uint32_t D = b.head_dim, block = 1u << b.log_block, past = u.seq.len - u.seq.rows;
+
+  // This lane's columns; past the last one, the last.
+  uint32_t pos[CG];
+  const float* qp[CG];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const uint32_t at = cg * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
+    pos[cg] = past + row;
+    qp[cg] = a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D;
+  }
+
+  // Page numbers of a tile's sixteen positions r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
+  const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
+  const uint32_t last_slot = (u.seq.len - 1u) >> b.log_block;
+  auto slot_of = [&](uint32_t position) {
+    const uint32_t s = position >> b.log_block;
+    return s < last_slot ? s : last_slot;
+  };
+  struct Numbers {
+    uint32_t k, v;
+  };
+  auto numbers = [&](uint32_t i) {
+    const uint32_t p0 = tile_at(w, i) * 64u;
+    return Numbers{table[slot_of(p0 + (r >> 2) * 16u)], table[slot_of(p0 + g * 16u)]};
+  };
+  uint4 kr[4][KL], vr[VL];
+  float ks, vs;
+  bool known;
+  const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
+  auto fetch_keys = [&](uint32_t i, const Numbers& n) {
+    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * 64u + (r >> 2) * 16u) & (block - 1u);
+    const uint8_t* from = a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D;
+#pragma unroll
+    for (int x = 0; x < KL; ++x) {
+      const uint32_t d = 64u * x + 16u * g;                         // (elements past head_dim meet zeros of the queries)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) kr[y][x] = load_u4(from + 4u * y * D + (d < D ? d : 0u));
+    }
+    ks = a.k_scale[static_cast<uint64_t>(n.v < b.pages ? n.v : 0u) * b.kv_heads + kv];
+  };
+  auto fetch_values = [&](uint32_t i, const Numbers& n) {
+    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * 64u + g * 16u) & (block - 1u);
+    const uint8_t* from = a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
+#pragma unroll
+    for (int x = 0; x < VL; ++x) {
+      const uint32_t d = 16u * x + r;
+      vr[x] = load_u4(from + (d < D ? d : r) * block);
+    }
+    vs = a.v_scale[static_cast<uint64_t>(page) * b.kv_heads + kv];
+    known = n.v < b.pages;
+  };
+
+  uint32_t i = begin + wave;
+  Numbers next{0u, 0u};
+  if (i < end) {
+    const Numbers now = numbers(i);
+    fetch_keys(i, now);
+    fetch_values(i, now);
+    if (i + NW < end) next = numbers(i + NW);
+  }
+
+  // The queries' terms.
+  half8_t q_hi[CG][STEPS], q_lo[CG][STEPS];
+  float q_scale[CG];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    float raw[STEPS][8], most = 0.0f;
+#pragma unroll
+    for (int x = 0; x < STEPS; ++x) {
+      const uint32_t d = 64u * (x / 2) + 16u * g + 8u * (x % 2);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 v = d < D ? *reinterpret_cast<const float4*>(qp[cg] + d + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+        raw[x][e] = v.x, raw[x][e + 1] = v.y, raw[x][e + 2] = v.z, raw[x][e + 3] = v.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(raw[x][e]));
+    }
+    most = groups_max(most);
+    const float up = most == 0.0f ? 1.0f : power_to(most, 13);
+    q_scale[cg] = kLog2E / sqrtf(static_cast<float>(D)) / up;
+#pragma unroll
+    for (int x = 0; x < STEPS; ++x) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = raw[x][e] * up;
+        const _Float16 h = static_cast<_Float16>(v);
+        q_hi[cg][x][e] = h, q_lo[cg][x][e] = static_cast<_Float16>(v - static_cast<float>(h));
+      }
+    }
+  }
+
+  Column col[CG];
+  float4_t o[CG][VL];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+    for (int x = 0; x < VL; ++x) o[cg][x] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (; i < end; i += NW) {
+    const bool more = i + NW < end;
+    float4_t acc[CG][4];
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int x = 0; x < STEPS; ++x) {
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const uint4 run = kr[y][x / 2];
+        const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+          acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q_lo[cg][x], acc[cg][y], 0, 0, 0);
+          acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q_hi[cg][x], acc[cg][y], 0, 0, 0);
+        }
+      }
+    }
+    const uint32_t first = tile_at(w, i) * 64u;
+    const float k_scale = ks, v_scale = vs;
+    const bool in_pool = known;
+    if (more) fetch_keys(i + NW, next);
+    // Every column sees every position of the tile, or it goes by bits.
+    const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
+    half8_t p_hi[CG][2], p_lo[CG][2];
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      float s[16];
+      const float scale = q_scale[cg] * k_scale;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = acc[cg][e / 4][e % 4] * scale;
+      uint32_t shown = 0xFFFFu;
+      if (!all) {
+        const uint32_t p0 = first + 16u * g;
+        shown = 0u;
+#pragma unroll
+        for (uint32_t e = 0; e < 16u; ++e) {
+          const uint32_t p = p0 + e;
+          const bool sees = p <= pos[cg] && (a.window == 0u || pos[cg] - p < a.window || p < a.sinks);
+          shown |= (in_pool && sees ? 1u : 0u) << e;
+        }
+      }
+      const float corr = weigh<16>(col[cg], s, shown, all, v_scale, p_hi[cg], p_lo[cg]);
+      if (__any(corr != 1.0f)) {
+#pragma unroll
+        for (int x = 0; x < VL; ++x) o[cg][x] *= corr;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < VL; ++x) {
+      const half8_t v0 = operand<KIND>(vr[x].x, vr[x].y), v1 = operand<KIND>(vr[x].z, vr[x].w);
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) {
+        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p_lo[cg][0], o[cg][x], 0, 0, 0);
+        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p_lo[cg][1], o[cg][x], 0, 0, 0);
+        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p_hi[cg][0], o[cg][x], 0, 0, 0);
+        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p_hi[cg][1], o[cg][x], 0, 0, 0);
+      }
+    }
+    if (more) fetch_values(i + NW, next);
+    if (i + 2 * NW < end) next = numbers(i + 2 * NW);
+  }
+
+  // Merge of the wavefronts under the largest reference.
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const float total = groups_sum(col[cg].sum);
+    if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = total;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][cg * 16u + r]);
+    const float factor = __builtin_amdgcn_exp2f(col[cg].ref - from_reference(top)) / col[cg].up;
+#pragma unroll
+    for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * factor;
+  }
+  __syncthreads();
+  const bool whole = w.tiles <= a.part_tiles;                       // no other part has tiles
+  const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * C;
+  for (uint32_t e = t; e < w.columns * (D / 4u); e += NW * 64u) {
+    const uint32_t c = e / (D / 4u), d = e % (D / 4u) * 4u;
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][c]);
+    float total = 0.0f;
+    float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int n = 0; n < NW; ++n) {
+      total = fmaf(__builtin_amdgcn_exp2f(sh.ref[n][c] - from_reference(top)), sh.sum[n][c], total);
+      x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]);
+    }
+    if (whole) {
+      const uint32_t pair = w.first_col + c;
+      float* to = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
+      *reinterpret_cast<float4_t*>(to) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
+    } else {
+      *reinterpret_cast<float4_t*>(a.part_sum + (slot + c) * D + d) = x;
+      if (d == 0u) a.part_most[slot + c] = top, a.part_total[slot + c] = total;
+    }
+  }
+}
+
+// ---- the parts' merge ----------------------------------------------------------------------------
+
+// A workgroup a column: its parts' sums under the largest of their references.
+template <int C>
+__global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttention a) {
+  __shared__ alignas(16) float piece[256 * 4];
+  const PageBatch& b = a.batch;
+  const uint32_t c = blockIdx.x % C, rest = blockIdx.x / C, kv = rest % b.kv_heads, unit = rest / b.kv_heads;
+  PageUnit u;
+  if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
+  const UnitTiles w = unit_tiles(a, u, C);
+  if (c >= w.columns || w.tiles <= a.part_tiles) return;            // workgroup-uniform
+  const uint32_t parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles, D = b.head_dim, runs = D / 4u, t = threadIdx.x;
+  const uint64_t at = (static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts * C + c;
+  float top = -INFINITY;
+  for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, a.part_most[at + static_cast<uint64_t>(p) * C]);
+  const float to = from_reference(top);
+  // 256 / runs threads a run of four elements
+  const uint32_t lanes = 256u / runs, own = t / runs, d = t % runs * 4u;
+  float total = 0.0f;
+  float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t p = own; p < parts && own < lanes; p += lanes) {
+    const uint64_t from = at + static_cast<uint64_t>(p) * C;
+    x += *reinterpret_cast<const float4_t*>(a.part_sum + from * D + d) * __builtin_amdgcn_exp2f(a.part_most[from] - to);
+  }
+  for (uint32_t p = 0; p < parts; ++p) {
+    const uint64_t from = at + static_cast<uint64_t>(p) * C;
+    total = fmaf(__builtin_amdgcn_exp2f(a.part_most[from] - to), a.part_total[from], total);
+  }
+  reinterpret_cast<float4_t*>(piece)[t] = x;
+  __syncthreads();
+  if (own != 0u) return;
+  for (uint32_t n = 1; n < lanes; ++n) x += reinterpret_cast<const float4_t*>(piece)[n * runs + t];
+  const uint32_t pair = w.first_col + c;
+  float* out = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
+  *reinterpret_cast<float4_t*>(out) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
+}
+
+uint64_t units_of(const PageAttentionCall& c, uint64_t columns) {
+  const uint64_t group = c.heads / c.page.kv_heads;
+  const uint64_t some = c.page.rows * group / columns + c.page.sequences, each = c.page.sequences * ((c.max_rows * group + columns - 1) / columns);
+  return some < each ? some : each;
+}
+
+}  // namespace
+
+// Tiles that a unit walks, at most.
+static uint64_t tiles_of(const PageAttentionCall& c) {
+  const uint64_t all = (c.max_len + 63) / 64;
+  if (c.window == 0) return all;
+  const uint64_t some = (c.sinks + 63) / 64 + (c.window + c.max_rows + 63) / 64 + 1;
+  return some < all ? some : all;
+}
+
+size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape& shape) {
+  if (shape.parts < 2) return 0;
+  return static_cast<size_t>(units_of(c, shape.columns) * c.page.kv_heads * shape.parts * shape.columns * (c.page.head_dim + 2) * 4);
+}
+
+PagesShape attention_pages_shape(const PageAttentionCall& c, uint64_t most_parts) {
+  PagesShape shape{16, 1, tiles_of(c)};
+  const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads, cus = static_cast<uint64_t>(num_cus());
+  uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
+  if (parts > most_parts) parts = most_parts;
+  if (parts > (shape.part_tiles + 3) / 4) parts = (shape.part_tiles + 3) / 4;
+  while (parts > 1) {
+    const uint64_t tiles = (tiles_of(c) + parts - 1) / parts;
+    shape.parts = (tiles_of(c) + tiles - 1) / tiles, shape.part_tiles = tiles;
+    if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
+    --parts;
+  }
+  return PagesShape{16, 1, tiles_of(c)};
+}
+
+hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
+                                  const float* ks, const float* vs, const uint32_t* table, const uint32_t* starts, const uint32_t* lens, float* out,
+                                  void* scratch, hipStream_t stream) {
+  PageAttention a{};
+  a.batch = page_batch(c.page, table, starts, lens);
+  a.batch.max_rows = static_cast<uint32_t>(c.max_rows), a.batch.max_len = static_cast<uint32_t>(c.max_len);
+  a.q = q, a.k = k, a.v = v, a.k_scale = ks, a.v_scale = vs, a.out = out;
+  a.heads = static_cast<uint32_t>(c.heads), a.group = static_cast<uint32_t>(c.heads / c.page.kv_heads);
+  // (a window or sinks past every position are all positions)
+  a.window = c.window >= c.max_len ? 0u : static_cast<uint32_t>(c.window);
+  a.sinks = static_cast<uint32_t>(c.sinks < c.max_len ? c.sinks : c.max_len);
+  a.parts = static_cast<uint32_t>(shape.parts), a.part_tiles = static_cast<uint32_t>(shape.part_tiles);
+  const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads;
+  if (shape.parts > 1) {
+    const uint64_t columns = groups * shape.parts * shape.columns;
+    a.part_sum = static_cast<float*>(scratch);
+    a.part_most = a.part_sum + columns * c.page.head_dim;
+    a.part_total = a.part_most + columns;
+  }
+  auto few = [&](auto kind, auto dim) {
+    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, 1, 4>), dim3(static_cast<uint32_t>(groups * shape.parts)),
+                       dim3(256), 0, stream, a);
+  };
+  auto with_dim = [&](auto kind) {
+    const uint64_t D = c.page.head_dim;
+    D <= 64 ? few(kind, std::integral_constant<int, 64>{}) : D <= 128 ? few(kind, std::integral_constant<int, 128>{}) : few(kind, std::integral_constant<int, 256>{});
+  };
+  fp8 ? with_dim(std::integral_constant<PageKind, PageKind::Fp8>{}) : with_dim(std::integral_constant<PageKind, PageKind::Q8>{});
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || shape.parts < 2) return e;
+  hipLaunchKernelGGL((attention_pages_merge_kernel<16>), dim3(static_cast<uint32_t>(groups * 16)), dim3(256), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace qmm

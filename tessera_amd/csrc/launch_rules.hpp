@@ -328,6 +328,11 @@ constexpr LogprobPlan logprob_plan(uint64_t rows, uint64_t vocab, uint64_t top_k
   return best;
 }
 
+// ---- "attention_pages" -----------------------------------------------------------------------------------------------
+struct PagesShape {
+  uint64_t columns, parts, part_tiles;                        // (row, head) pairs a workgroup; parts of the positions, tiles of 64 each
+};
+
 // ---- "attention_combine" ---------------------------------------------------------------------------------------------
 // Wavefronts of a (row, head): sixteen where there are few and many parts, four where the rows fill the chip by themselves or
 // sixteen parts are all that there are, one where its four are and that does not make a lane's run long with few rows (us, 1 /

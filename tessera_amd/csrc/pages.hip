@@ -1,0 +1,239 @@
+// "pages_write_*": rows of keys and values into the pages of a batch, quantized; "pages_read_*": rows of pages as fp32 or fp16.
+
+#include <type_traits>
+
+#include "pages.hpp"
+#include "qmm_kernels.hpp"
+
+namespace qmm {
+namespace {
+
+// ---- codes ---------------------------------------------------------------------------------------
+//
+// x / scale to the nearest code, ties to the even one; code times scale.  Both are fp32 operations rounded once, so that a row
+// written and read is a matter of definition, not of order.
+template <PageKind KIND>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float scale) {
+  constexpr float M = page_largest(KIND);
+  auto of = [&](float v) { return fminf(fmaxf(v / scale, -M), M); };
+  if constexpr (KIND == PageKind::Q8) {
+    auto code = [&](float v) { return static_cast<uint32_t>(static_cast<int>(__builtin_rintf(of(v)))) & 255u; };
+    return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+  } else {
+    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(of(a), of(b), 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(of(c), of(d), low, true));
+  }
+}
+template <PageKind KIND>
+__device__ __forceinline__ float decode(uint32_t four, int i) {
+  if constexpr (KIND == PageKind::Q8) return static_cast<float>(static_cast<int>(four << (24 - 8 * i)) >> 24);
+  switch (i) {
+    case 0: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(four), 0);
+    case 1: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(four), 1);
+    case 2: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(four), 2);
+    default: return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(four), 3);
+  }
+}
+
+// ---- a page of the batch -------------------------------------------------------------------------
+//
+// A workgroup takes the keys or the values of a page and key head.  A page is written as a whole by one workgroup, so that its scale
+// needs no second launch: new rows lie at places `from` .. `to` - 1 of it, places below `from` hold earlier positions.
+struct PageWork {
+  PageUnit unit;
+  uint32_t kv, page, from, to, first_row;   // first_row: the call's row at place `from`
+  bool values, held;                        // held: the page's number is one of the pool's
+};
+__device__ __forceinline__ bool page_work(const PageBatch& b, PageWork* w) {
+  const uint32_t which = blockIdx.x % (2u * b.kv_heads);
+  if (!find_unit(b, blockIdx.x / (2u * b.kv_heads), [&](const PageSequence& q) { return touched_pages(b, q); }, &w->unit)) return false;
+  const PageSequence& q = w->unit.seq;
+  const uint32_t block = 1u << b.log_block, past = q.len - q.rows, slot = (past >> b.log_block) + w->unit.at, base = slot << b.log_block;
+  w->values = which >= b.kv_heads, w->kv = w->values ? which - b.kv_heads : which;
+  w->from = past > base ? past - base : 0u;
+  w->to = q.len - base < block ? q.len - base : block;
+  w->first_row = q.first + (base + w->from - past);
+  w->page = b.table[static_cast<uint64_t>(w->unit.s) * b.width + slot];
+  w->held = w->page < b.pages;
+  return true;
+}
+
+// Thread t's runs of sixteen bytes of a page: keys by (place, sixteen elements), values by (sixteen places, element), an element a
+// lane, so that a wavefront's loads of rows are whole lines.
+constexpr uint32_t kPageThreads = 256;
+
+// Bound by memory: 8 bytes a row's element in, 2 out, and what a page that is continued holds.  Rows are read twice, for the
+// largest and for the codes, the second time out of the caches.
+template <PageKind KIND>
+__global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, const float* __restrict__ k, const float* __restrict__ v, uint64_t k_stride,
+                                                                   uint64_t v_stride, uint8_t* kp, uint8_t* vp, float* ks, float* vs) {
+  __shared__ uint32_t most_of[kPageThreads / 64];
+  PageWork w;
+  if (!page_work(b, &w) || !w.held) return;               // workgroup-uniform
+  const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block;
+  const uint64_t stride = w.values ? v_stride : k_stride;
+  const float* rows = (w.values ? v : k) + static_cast<uint64_t>(w.first_row) * stride + w.kv * D;   // of place `from`
+  const uint64_t head = static_cast<uint64_t>(w.page) * b.kv_heads + w.kv;
+  float* scale_at = (w.values ? vs : ks) + head;
+  uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
+  const float before = w.from == 0u ? 0.0f : *scale_at;
+
+  // The largest magnitude by its bits: infinities and NaN are above all numbers.
+  uint32_t most = 0u;
+  for (uint32_t i = t; i < (w.to - w.from) * (D / 4u); i += kPageThreads) {
+    const float4 x = *reinterpret_cast<const float4*>(rows + i / (D / 4u) * stride + i % (D / 4u) * 4u);
+    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = max(most, bit_cast<uint32_t>(xs[e]) & 0x7FFFFFFFu);
+  }
+#pragma unroll
+  for (uint32_t off = 32u; off > 0u; off >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(most, off, kWave)));
+  if ((t & 63u) == 0u) most_of[t >> 6] = most;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kPageThreads / 64u; ++i) most = max(most, most_of[i]);
+  const float own = bit_cast<float>(most) / page_largest(KIND);
+  // A page with an infinity or NaN is NaN until it is begun anew.
+  const bool finite = most < 0x7F800000u && before < INFINITY && before >= 0.0f;
+  const float scale = finite ? fmaxf(before, own) : bit_cast<float>(0x7FC00000u);
+  if (t == 0u) *scale_at = scale;
+  const bool empty = !(scale > 0.0f);                      // (NaN too): all codes 0
+  const bool again = w.from != 0u && (empty || scale != before);
+
+  if (!w.values) {
+    const uint32_t runs = D / 16u;
+    for (uint32_t i = t + (again ? 0u : w.from * runs); i < block * runs; i += kPageThreads) {
+      const uint32_t place = i / runs, d = i % runs * 16u;
+      uint4* to = reinterpret_cast<uint4*>(codes + place * D + d);
+      uint32_t r[4] = {0u, 0u, 0u, 0u};
+      if (!empty && place < w.to) {
+        if (place < w.from) {
+          const uint4 old = *to;
+          const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            r[j] = encode4<KIND>(decode<KIND>(o[j], 0) * before, decode<KIND>(o[j], 1) * before, decode<KIND>(o[j], 2) * before, decode<KIND>(o[j], 3) * before, scale);
+          }
+        } else {
+          const float* from = rows + (place - w.from) * stride + d;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 x = *reinterpret_cast<const float4*>(from + 4 * j);
+            r[j] = encode4<KIND>(x.x, x.y, x.z, x.w, scale);
+          }
+        }
+      }
+      *to = uint4{r[0], r[1], r[2], r[3]};
+    }
+    return;
+  }
+  const uint32_t from16 = again ? 0u : w.from / 16u;
+  for (uint32_t i = t + from16 * D; i < block / 16u * D; i += kPageThreads) {
+    const uint32_t run = i / D, d = i % D, place = run * 16u;
+    uint4* to = reinterpret_cast<uint4*>(codes + d * block + place);
+    uint32_t r[4] = {0u, 0u, 0u, 0u};
+    if (!empty && place < w.to) {
+      uint32_t o[4] = {0u, 0u, 0u, 0u};
+      if (place < w.from) {
+        const uint4 old = *to;
+        o[0] = old.x, o[1] = old.y, o[2] = old.z, o[3] = old.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t at = place + 4u * j + e;
+          x[e] = at < w.from ? decode<KIND>(o[j], e) * before : at < w.to ? rows[(at - w.from) * stride + d] : 0.0f;
+        }
+        r[j] = encode4<KIND>(x[0], x[1], x[2], x[3], scale);
+        if (!again && place + 4u * j < w.from) {           // codes that stay
+          const uint32_t stay = w.from - place - 4u * j, mask = stay < 4u ? (1u << 8u * stay) - 1u : ~0u;
+          r[j] = (r[j] & ~mask) | (o[j] & mask);
+        }
+      }
+    }
+    *to = uint4{r[0], r[1], r[2], r[3]};
+  }
+}
+
+// Bound by memory: 2 bytes a row's element in, 8 or 4 out.
+template <PageKind KIND, class Out>
+__global__ __launch_bounds__(kPageThreads) void pages_read_kernel(PageBatch b, const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp,
+                                                                  const float* __restrict__ ks, const float* __restrict__ vs, Out* k, Out* v) {
+  PageWork w;
+  if (!page_work(b, &w)) return;
+  const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block;
+  const uint64_t wide = static_cast<uint64_t>(b.kv_heads) * D;
+  Out* rows = (w.values ? v : k) + static_cast<uint64_t>(w.first_row) * wide + w.kv * D;   // of place `from`
+  const uint64_t head = static_cast<uint64_t>(w.held ? w.page : 0u) * b.kv_heads + w.kv;
+  const float scale = w.held ? (w.values ? vs : ks)[head] : 0.0f;
+  const uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
+  auto value = [&](uint32_t four, int i) {
+    float x = w.held ? decode<KIND>(four, i) * scale : 0.0f;
+    asm("" : "+v"(x));                                     // (an fp32 number before it is an fp16 one: no one operation for both)
+    return static_cast<Out>(x);
+  };
+  if (!w.values) {
+    const uint32_t runs = D / 4u;
+    for (uint32_t i = t; i < (w.to - w.from) * runs; i += kPageThreads) {
+      const uint32_t at = i / runs, d = i % runs * 4u;
+      const uint32_t four = *reinterpret_cast<const uint32_t*>(codes + (w.from + at) * D + d);
+      Out* to = rows + at * wide + d;
+      typedef Out out4 __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<out4*>(to) = out4{value(four, 0), value(four, 1), value(four, 2), value(four, 3)};
+    }
+    return;
+  }
+  for (uint32_t i = t + w.from / 16u * D; i < (w.to + 15u) / 16u * D; i += kPageThreads) {
+    const uint32_t place = i / D * 16u, d = i % D;
+    const uint4 run = load_u4(codes + d * block + place);
+    const uint32_t r[4] = {run.x, run.y, run.z, run.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t at = place + 4u * j + e;
+        if (at >= w.from && at < w.to) rows[(at - w.from) * wide + d] = value(r[j], e);
+      }
+    }
+  }
+}
+
+uint32_t workgroups(const PageCall& c) { return static_cast<uint32_t>(c.touched() * c.kv_heads * 2); }
+
+}  // namespace
+
+PageBatch page_batch(const PageCall& c, const uint32_t* table, const uint32_t* starts, const uint32_t* lens) {
+  uint32_t log_block = 4;
+  while ((uint64_t{1} << log_block) < c.block) ++log_block;
+  return PageBatch{table, starts, lens, static_cast<uint32_t>(c.rows), static_cast<uint32_t>(c.sequences), static_cast<uint32_t>(c.pages),
+                   static_cast<uint32_t>(c.width), static_cast<uint32_t>(c.rows), static_cast<uint32_t>(c.width * c.block),
+                   static_cast<uint32_t>(c.kv_heads), static_cast<uint32_t>(c.head_dim), log_block};
+}
+
+hipError_t launch_pages_write(bool fp8, const PageWriteCall& c, const float* k, const float* v, const uint32_t* table, const uint32_t* starts,
+                              const uint32_t* lens, uint8_t* kp, uint8_t* vp, float* ks, float* vs, hipStream_t stream) {
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(workgroups(c.page)), dim3(kPageThreads), 0, stream, page_batch(c.page, table, starts, lens), k, v, c.k_stride, c.v_stride,
+                       kp, vp, ks, vs);
+  };
+  fp8 ? go(pages_write_kernel<PageKind::Fp8>) : go(pages_write_kernel<PageKind::Q8>);
+  return hipGetLastError();
+}
+
+hipError_t launch_pages_read(bool fp8, const PageReadCall& c, const uint8_t* kp, const uint8_t* vp, const float* ks, const float* vs, const uint32_t* table,
+                             const uint32_t* starts, const uint32_t* lens, void* k, void* v, hipStream_t stream) {
+  auto go = [&](auto kernel, auto* as) {
+    using Out = std::remove_pointer_t<decltype(as)>;
+    hipLaunchKernelGGL(kernel, dim3(workgroups(c.page)), dim3(kPageThreads), 0, stream, page_batch(c.page, table, starts, lens), kp, vp, ks, vs,
+                       static_cast<Out*>(k), static_cast<Out*>(v));
+  };
+  float* f32 = nullptr;
+  _Float16* f16 = nullptr;
+  if (c.f16) fp8 ? go(pages_read_kernel<PageKind::Fp8, _Float16>, f16) : go(pages_read_kernel<PageKind::Q8, _Float16>, f16);
+  else fp8 ? go(pages_read_kernel<PageKind::Fp8, float>, f32) : go(pages_read_kernel<PageKind::Q8, float>, f32);
+  return hipGetLastError();
+}
+
+}  // namespace qmm

@@ -17,6 +17,7 @@
 #include "qmm_kernels.hpp"
 #include "launch_rules.hpp"
 #include "stream_scratch.hpp"
+#include "page_args.hpp"
 #include "tree_args.hpp"
 
 namespace {
@@ -1519,6 +1520,62 @@ qmm_status run_token_logprobs(const LaunchCtx& c) {
                                             top_k, row_base, need == 0 ? nullptr : block.get(), kPartsLimits.small, c.stream));
 }
 
+// "pages_write_q8", "pages_write_fp8": buffers K, V (rows of k_stride and v_stride fp32, kv_heads * head_dim of each), Table
+// (sequences x width u32), Starts (sequences + 1 u32), Lens (sequences u32), Kp, Vp (pages x kv_heads x block x head_dim codes), Ks, Vs
+// (pages x kv_heads fp32); scalars rows, kv_heads, head_dim, sequences, block, pages, width, k_stride, v_stride.
+qmm_status run_pages_write(const LaunchCtx& c, bool fp8) {
+  qmm::PageWriteCall call;
+  if (const char* why = qmm::check_pages_write(args_of(c), &call)) return bad(why);
+  return map_hip(qmm::launch_pages_write(fp8, call, c.ptr<const float>(0), c.ptr<const float>(1), c.ptr<const uint32_t>(2), c.ptr<const uint32_t>(3),
+                                         c.ptr<const uint32_t>(4), c.ptr<uint8_t>(5), c.ptr<uint8_t>(6), c.ptr<float>(7), c.ptr<float>(8), c.stream));
+}
+qmm_status run_pages_write_q8(const LaunchCtx& c) { return run_pages_write(c, false); }
+qmm_status run_pages_write_fp8(const LaunchCtx& c) { return run_pages_write(c, true); }
+
+// "pages_read_q8", "pages_read_fp8": buffers Kp, Vp, Ks, Vs, Table, Starts, Lens, K, V (rows x kv_heads*head_dim fp32 or fp16);
+// scalars rows, kv_heads, head_dim, sequences, block, pages, width, out_f16.
+qmm_status run_pages_read(const LaunchCtx& c, bool fp8) {
+  qmm::PageReadCall call;
+  if (const char* why = qmm::check_pages_read(args_of(c), &call)) return bad(why);
+  return map_hip(qmm::launch_pages_read(fp8, call, c.ptr<const uint8_t>(0), c.ptr<const uint8_t>(1), c.ptr<const float>(2), c.ptr<const float>(3),
+                                        c.ptr<const uint32_t>(4), c.ptr<const uint32_t>(5), c.ptr<const uint32_t>(6), c.ptr<void>(7), c.ptr<void>(8),
+                                        c.stream));
+}
+qmm_status run_pages_read_q8(const LaunchCtx& c) { return run_pages_read(c, false); }
+qmm_status run_pages_read_fp8(const LaunchCtx& c) { return run_pages_read(c, true); }
+
+// "attention_pages_q8", "attention_pages_fp8": buffers Q (rows x heads*head_dim), Kp, Vp, Ks, Vs, Table, Starts, Lens, Out (as Q);
+// scalars rows, heads, kv_heads, head_dim, sequences, block, pages, width, max_rows, max_len, window, sinks.
+qmm_status run_attention_pages(const LaunchCtx& c, bool fp8) {
+  qmm::PageAttentionCall call;
+  if (const char* why = qmm::check_attention_pages(args_of(c), &call)) return bad(why);
+  auto go = [&](const qmm::PagesShape& shape, void* scratch) {
+    return map_hip(qmm::launch_attention_pages(fp8, call, shape, c.ptr<const float>(0), c.ptr<const uint8_t>(1), c.ptr<const uint8_t>(2),
+                                               c.ptr<const float>(3), c.ptr<const float>(4), c.ptr<const uint32_t>(5), c.ptr<const uint32_t>(6),
+                                               c.ptr<const uint32_t>(7), c.ptr<float>(8), scratch, c.stream));
+  };
+  const qmm::PagesShape in_parts = qmm::attention_pages_shape(call, 256);
+  if (in_parts.parts > 1) {
+    const StreamBlock block(c, qmm::attention_pages_parts_bytes(call, in_parts), g_parts_scratch);
+    if (block.get() != nullptr) return go(in_parts, block.get());
+  }
+  return go(qmm::attention_pages_shape(call, 1), nullptr);
+}
+qmm_status run_attention_pages_q8(const LaunchCtx& c) { return run_attention_pages(c, false); }
+qmm_status run_attention_pages_fp8(const LaunchCtx& c) { return run_attention_pages(c, true); }
+
+// "draft_verify": buffers Logits (rows x vocab fp32), Tokens (rows u32), Random (rows x 2 fp32), Starts (sequences + 1 u32), Accepted,
+// Next (sequences u32)[, DraftLogits (as Logits)]; scalars rows, vocab, sequences, temperature, draft_temperature (fp32 bits).
+qmm_status run_draft_verify(const LaunchCtx& c) {
+  qmm::DraftCall call;
+  if (const char* why = qmm::check_draft_verify(args_of(c), &call)) return bad(why);
+  const size_t need = qmm::draft_verify_scratch_bytes(call);
+  const StreamBlock block(c, need <= kPartsLimits.small ? need : 0, g_parts_scratch);
+  return map_hip(qmm::launch_draft_verify(call, c.ptr<const float>(0), c.ptr<const uint32_t>(1), c.ptr<const float>(2), c.ptr<const uint32_t>(3),
+                                          c.ptr<uint32_t>(4), c.ptr<uint32_t>(5), call.draft ? c.ptr<const float>(6) : nullptr,
+                                          need <= kPartsLimits.small ? block.get() : nullptr, c.stream));
+}
+
 struct Entry {
   const char* id;
   qmm_fn fn;
@@ -1614,6 +1671,13 @@ const Entry kTable[] = {
     {"attention_tree_q4", run_attention_tree_q4},
     {"attention_tree_fp8", run_attention_tree_fp8},
     {"token_logprobs", run_token_logprobs},
+    {"pages_write_q8", run_pages_write_q8},
+    {"pages_write_fp8", run_pages_write_fp8},
+    {"pages_read_q8", run_pages_read_q8},
+    {"pages_read_fp8", run_pages_read_fp8},
+    {"attention_pages_q8", run_attention_pages_q8},
+    {"attention_pages_fp8", run_attention_pages_fp8},
+    {"draft_verify", run_draft_verify},
 };
 constexpr size_t kTableSize = sizeof(kTable) / sizeof(kTable[0]);
 

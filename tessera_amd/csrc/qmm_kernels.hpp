@@ -280,6 +280,26 @@ size_t token_logprobs_scratch_bytes(uint64_t rows, uint64_t vocab, uint32_t top_
 hipError_t launch_token_logprobs(const float* logits, const uint32_t* tokens, float* logprobs, float* entropy, uint32_t* top_tokens,
                                  float* top_logprobs, uint64_t rows, uint64_t vocab, uint32_t count, uint32_t top_k, uint64_t row_base,
                                  void* scratch, size_t most, hipStream_t stream);
+// The paged cache of a batch and the verification of its drafts (page_args.hpp: their calls).  attention_pages_shape: how a call
+// runs, its positions in at most `most_parts` parts, whose sums attention_pages_parts_bytes of `scratch` hold.
+struct PageWriteCall;
+struct PageReadCall;
+struct PageAttentionCall;
+struct DraftCall;
+struct PagesShape;
+hipError_t launch_pages_write(bool fp8, const PageWriteCall& call, const float* k, const float* v, const uint32_t* table, const uint32_t* starts,
+                              const uint32_t* lens, uint8_t* kp, uint8_t* vp, float* ks, float* vs, hipStream_t stream);
+hipError_t launch_pages_read(bool fp8, const PageReadCall& call, const uint8_t* kp, const uint8_t* vp, const float* ks, const float* vs,
+                             const uint32_t* table, const uint32_t* starts, const uint32_t* lens, void* k, void* v, hipStream_t stream);
+PagesShape attention_pages_shape(const PageAttentionCall& call, uint64_t most_parts);
+size_t attention_pages_parts_bytes(const PageAttentionCall& call, const PagesShape& shape);
+hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& call, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
+                                  const float* ks, const float* vs, const uint32_t* table, const uint32_t* starts, const uint32_t* lens, float* out,
+                                  void* scratch, hipStream_t stream);
+// draft_verify_scratch_bytes: what the split form takes of `scratch`; without it a workgroup takes a sequence, with the same results.
+size_t draft_verify_scratch_bytes(const DraftCall& call);
+hipError_t launch_draft_verify(const DraftCall& call, const float* logits, const uint32_t* tokens, const float* random, const uint32_t* starts,
+                               uint32_t* accepted, uint32_t* next, const float* draft, void* scratch, hipStream_t stream);
 hipError_t launch_quantize_kv(const float* in, uint8_t* out, float* scale, uint64_t rows, uint64_t cols, uint32_t bits,
                               hipStream_t stream);
 hipError_t launch_cast_f32_f16(const float* in, void* out, uint64_t n, hipStream_t stream);
