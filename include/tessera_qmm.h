@@ -237,10 +237,10 @@ const char* qmm_kernel_name(size_t index);
  *     With p = softmax(logits / temperature), q the draft's: a draft x stands where Random[i][0] q(x) < p(x).  Accepted:
  *     how many stand before the first that does not; Next: the token behind them, the first whose running sum of
  *     max(p - q, 0) there (without DraftLogits: of p but for x; where nothing is left, or behind the last row: of p)
- *     exceeds Random[i][1] of the whole.  All in fp64.  temperature 0: a draft stands where it is the row's largest logit,
+ *     exceeds Random[i][1] (outside [0, 1): the nearest in it) of the whole.  All in fp64.  temperature 0: a draft stands where it is the row's largest logit,
  *     the lowest of equals, and Next is that.  -infinity is a token of probability 0.  A row that holds NaN or +infinity or
  *     nothing but -infinity (the draft's likewise, where it is needed) ends the draft there, with Next 0xFFFFFFFF.  A token
- *     of vocab or more never stands.  vocab is at most 2^24.
+ *     of vocab or more never stands.  vocab is at most 2^21.
  *   - "mfma_probe": buffer Out (workgroups * 256 floats); scalars kind (0 fp16 32x32x16, 1 scaled
  *     fp8 x fp4 32x32x64, 2 int8 16x16x64), random (0 constant operands, 1 hashed), iterations,
  *     workgroups.  "read_probe": a plain read of a buffer.  Measurement ids: the matrix-core and the

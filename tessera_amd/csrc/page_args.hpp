@@ -10,7 +10,7 @@ namespace qmm {
 
 constexpr uint64_t kPageSequencesMost = 4096;            // a wavefront walks their starts 64 at a time
 constexpr uint64_t kPagePositionsMost = uint64_t{1} << 30;   // of a sequence: 32-bit arithmetic on positions stays in range
-constexpr uint64_t kDraftVocabMost = uint64_t{1} << 24;
+constexpr uint64_t kDraftVocabMost = uint64_t{1} << 21;
 
 // The batch and the pool, as all three families take them.
 struct PageCall {
@@ -164,7 +164,7 @@ inline const char* check_draft_verify(const LaunchArgs& c, DraftCall* out) {
   const DraftCall a{c.sc[0], c.sc[1], c.sc[2], scalar_f32(c.sc[3]), scalar_f32(c.sc[4]), c.nbuf == 7};
   if (a.rows == 0 || a.vocab == 0 || a.sequences == 0) return about(id, "rows, vocab and sequences must be non-zero");
   if (a.rows > (1u << 20) || a.vocab > kDraftVocabMost || a.sequences > kPageSequencesMost) {
-    return about(id, "at most 2^20 rows, a vocabulary of 2^24 and 4096 sequences");
+    return about(id, "at most 2^20 rows, a vocabulary of 2^21 and 4096 sequences");
   }
   if (!(a.temperature >= 0.0f) || a.temperature > 3.4e38f) return about(id, "temperature is 0 (the likeliest token) or positive and finite");
   if (a.draft && a.temperature > 0.0f && (!(a.draft_temperature > 0.0f) || a.draft_temperature > 3.4e38f)) {

@@ -53,7 +53,7 @@ def inputs(rs, rows, vocab, spread=2.5, agree=0.8):
 ROWS = [1, 5, 3, 1, 8, 2, 4, 17, 5, 5, 6]
 
 
-@pytest.mark.parametrize("vocab", [1, 2, 63, 500, 4095, 4096, 4097, 12289, 50001, 131072])
+@pytest.mark.parametrize("vocab", [1, 2, 63, 500, 511, 513, 1025, 12289, 50001, 131072])
 @pytest.mark.parametrize("temperature", [0.0, 0.3, 1.0, 4.0])
 @pytest.mark.parametrize("sampled", [False, True])
 def test_against_the_statement(backend, vocab, temperature, sampled):
@@ -186,7 +186,7 @@ def test_large_logits(backend):
 
 def test_the_largest_vocabulary(backend):
     rs = np.random.RandomState(23)
-    vocab = 1 << 24
+    vocab = 1 << 21
     logits = rs.rand(3, vocab).astype(np.float32)
     tokens = np.array([0, int(logits[0].argmax()), 5], np.uint32)
     random = np.array([[0.0, 0.3], [0.999, 0.7], [0.5, 0.999]], np.float32)

@@ -170,8 +170,8 @@ def test_draft_verify(tmp_path):
     s[i] = 0;
     CHECK(why(big, s));
   }
-  CHECK(why(big, {(1 << 20) + 1, 100, 2, one, one}) && why(big, {4, (1 << 24) + 1, 2, one, one}) && why(big, {4, 100, 4097, one, one}));
-  CHECK(!why(big, {1 << 20, 1 << 24, 4096, one, one}));
+  CHECK(why(big, {(1 << 20) + 1, 100, 2, one, one}) && why(big, {4, (1 << 21) + 1, 2, one, one}) && why(big, {4, 100, 4097, one, one}));
+  CHECK(!why(big, {1 << 20, 1 << 21, 4096, one, one}));
   for (uint64_t t : {0xBF800000ull, 0x7F800000ull, 0x7FC00000ull}) CHECK(why(big, {4, 100, 2, t, one}) && why(big, {4, 100, 2, one, t}));
   CHECK(why(big, {4, 100, 2, one, 0}) && why(big, {4, 100, 2, one}) && why({4, 4, 4, 4, 4}, {1, 1, 1, one, one}));
   for (size_t i = 4; i < 6; ++i) for (size_t j = 0; j < 7; ++j) {
