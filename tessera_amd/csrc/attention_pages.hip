@@ -4,11 +4,12 @@
 // the first `sinks` of the sequence.  out = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m), s_j = q . k_j / sqrt(head_dim), in one pass
 // over the keys with a running reference m.
 //
-// What is fp32 enters the fp16 matrix instructions as two terms, x = hi + lo, hi = RN16(x), lo = RN16(x - hi), under a power of two.
-// It brings a query's largest element to 2^13 .. 2^14: an element is carried to 2^-22 of itself down to 2^-16 of the largest, below to
-// 2^-38 of that.  It brings the largest of a row's weights times their values' scales so far to 2^9 .. 2^15: to 2^-22 of itself down
-// to 2^-12 of the largest, below to 2^-34 of that.  Codes enter exactly; a key's scale multiplies its fp32 score.  Scores, references,
-// sums and results are fp32.
+// What is fp32 enters the matrix instructions in pieces.  Over int8 pages a query is an integer of 23 bits and a sign under its row's
+// largest element, in three int8 limbs: an element is carried to 2^-23 of the largest, products and sums are exact.  Else it is two fp16
+// terms, x = hi + lo, hi = RN16(x), lo = RN16(x - hi), under a power of two that brings a query's largest element to 2^13 .. 2^14 (an
+// element is carried to 2^-22 of itself down to 2^-16 of the largest, below to 2^-38 of that), the largest of a row's weights times their
+// values' scales so far to 2^9 .. 2^15 (to 2^-22 of itself down to 2^-12 of the largest, below to 2^-34 of that).  Codes enter exactly; a
+// key's scale multiplies its fp32 score.  Scores, references, sums and results are fp32.
 
 #include <type_traits>
 
@@ -160,20 +161,97 @@ __device__ __forceinline__ float weigh(Column& c, float (&s)[COUNT], uint32_t sh
 
 // ---- few columns ---------------------------------------------------------------------------------
 //
-// Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of 64 positions on its own, with no LDS
-// before the merge.  v_mfma_f32_16x16x32_f16 twice: S^T = K Q^T, O^T = V^T P^T.  Row 4 g + e of the t-th of a tile's four key operands is
-// position 16 g + 4 t + e, so that lane group g ends up with the scores of the tile's positions 16 g .. 16 g + 15 (which lie
-// in one page: one scale a lane), and those are the sixteen of the value operands that it loads: no score changes its lane.
-template <int DP, int CG, int NW>
-struct FewShared {
-  float ref[NW][16 * CG], sum[NW][16 * CG];
-  alignas(16) float o[NW][16 * CG][DP + 4];
-};
+// Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of 64 positions on its own, with no
+// barrier between.  S^T = K Q^T and O^T = V^T P^T by matrix instructions of 16 x 16.  Row 4 g + e of the t-th of a tile's four key operands
+// is position 16 g + 4 t + e, so that lane group g ends up with the scores of the tile's positions 16 g .. 16 g + 15 (which lie
+// in one page: one scale a lane), and those are the sixteen of the value operands that it loads: no score changes its lane.  A
+// register that an operand was made from takes the next tile's at once, so that a tile's loads have a whole tile's time.  The queries'
+// operands lie in LDS, one copy for all wavefronts.
+constexpr int query_operands(PageKind kind, int dp) { return kind == PageKind::Q8 ? 3 * (dp / 64) : 2 * (dp / 32); }
 
 template <PageKind KIND, int DP, int CG, int NW>
-__global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttention a) {
-  constexpr int KL = DP / 64, VL = DP / 16, STEPS = DP / 32, C = 16 * CG;
-  __shared__ FewShared<DP, CG, NW> sh;
+struct FewShared {
+  union {
+    uint4 q[CG][query_operands(KIND, DP)][64];
+    alignas(16) float o[NW][16 * CG][DP + 4];
+  };
+  float ref[NW][16 * CG], sum[NW][16 * CG];
+};
+
+// A row's elements 64 x + 16 g + e of lane group g as operands: over int8 pages the limbs of three of them, else two terms of the sixteen in
+// two steps.  Returns what a score is to be multiplied by.  Only the operands of steps `x % step == own` are written.
+template <PageKind KIND, int DP>
+__device__ __forceinline__ float query_terms(const float* q, uint32_t D, uint4 (*to)[64], uint32_t own, uint32_t step) {
+  const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
+  float raw[DP / 64][16], most = 0.0f;
+  bool odd = false;
+#pragma unroll
+  for (int x = 0; x < DP / 64; ++x) {
+    const uint32_t d = 64u * x + 16u * g;
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const float4 v = d < D ? *reinterpret_cast<const float4*>(q + d + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+      raw[x][e] = v.x, raw[x][e + 1] = v.y, raw[x][e + 2] = v.z, raw[x][e + 3] = v.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(raw[x][e])), odd = odd || !(fabsf(raw[x][e]) < INFINITY);
+  }
+  most = groups_max(most);
+  const float natural = kLog2E / sqrtf(static_cast<float>(D));
+  if constexpr (KIND == PageKind::Q8) {
+    constexpr float kMost = 8355584.0f;                            // three limbs hold 127 more, which rounding cannot reach
+    const float up = most == 0.0f ? 1.0f : power_to(most, 0), whole = most == 0.0f ? 1.0f : most * up, scale = kMost / whole;
+    odd = groups_max(odd ? 1.0f : 0.0f) != 0.0f;
+#pragma unroll
+    for (int x = 0; x < DP / 64; ++x) {
+      if (static_cast<uint32_t>(x) % step != own) continue;
+      uint32_t limb[3][4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t n[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // two's complement with each byte's carry into the next: n + 0x8080 has bytes limb + 128 but for the highest
+          n[e] = (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(raw[x][4 * w + e] * up * scale))) + 0x8080u) ^ 0x8080u;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) {
+          const uint32_t low = __builtin_amdgcn_perm(n[1], n[0], 0x0C0C0400u + 0x0101u * i), high = __builtin_amdgcn_perm(n[3], n[2], 0x04000C0Cu + 0x01010000u * i);
+          limb[i][w] = low | high;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) to[3 * x + i][lane] = uint4{limb[i][0], limb[i][1], limb[i][2], limb[i][3]};
+    }
+    // (an infinity or NaN: all scores NaN)
+    return odd ? bit_cast<float>(0x7FC00000u) : natural * (whole / kMost) / up;
+  } else {
+    const float up = most == 0.0f ? 1.0f : power_to(most, 13);
+#pragma unroll
+    for (int x = 0; x < DP / 32; ++x) {
+      if (static_cast<uint32_t>(x) % step != own) continue;
+      half8_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = raw[x / 2][8 * (x % 2) + e] * up;
+        hi[e] = static_cast<_Float16>(v);
+        lo[e] = static_cast<_Float16>(v - static_cast<float>(hi[e]));
+      }
+      to[2 * x][lane] = bit_cast<uint4>(hi), to[2 * x + 1][lane] = bit_cast<uint4>(lo);
+    }
+    return natural / up;
+  }
+}
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+
+template <PageKind KIND, int DP, int CG, int NW>
+constexpr int few_waves() { return DP == 64 ? (CG == 1 ? 3 : 2) : DP == 128 ? (CG == 1 ? 2 : 1) : 1; }   // a SIMD, by the registers
+
+template <PageKind KIND, int DP, int CG, int NW>
+__global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void attention_pages_few_kernel(PageAttention a) {
+  constexpr int KL = DP / 64, VL = DP / 16, C = 16 * CG;
+  __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
   const uint32_t kv = blockIdx.x % b.kv_heads, rest = blockIdx.x / b.kv_heads, part = rest % a.parts, unit = rest / a.parts;
@@ -184,16 +262,6 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
   if (begin >= w.tiles) return;                                     // workgroup-uniform
   const uint32_t end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
   const uint32_t D = b.head_dim, block = 1u << b.log_block, past = u.seq.len - u.seq.rows;
-
-  // This lane's columns; past the last one, the last.
-  uint32_t pos[CG];
-  const float* qp[CG];
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const uint32_t at = cg * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
-    pos[cg] = past + row;
-    qp[cg] = a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D;
-  }
 
   // Page numbers of a tile's sixteen positions r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
   const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
@@ -213,68 +281,55 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
   float ks, vs;
   bool known;
   const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
-  auto fetch_keys = [&](uint32_t i, const Numbers& n) {
+  // Where a lane's runs of a tile begin.  (Elements past head_dim meet zeros of the queries, or are not stored.)
+  auto keys_at = [&](uint32_t i, const Numbers& n) {
     const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * 64u + (r >> 2) * 16u) & (block - 1u);
-    const uint8_t* from = a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D;
-#pragma unroll
-    for (int x = 0; x < KL; ++x) {
-      const uint32_t d = 64u * x + 16u * g;                         // (elements past head_dim meet zeros of the queries)
-#pragma unroll
-      for (int y = 0; y < 4; ++y) kr[y][x] = load_u4(from + 4u * y * D + (d < D ? d : 0u));
-    }
-    ks = a.k_scale[static_cast<uint64_t>(n.v < b.pages ? n.v : 0u) * b.kv_heads + kv];
+    return a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D;
   };
-  auto fetch_values = [&](uint32_t i, const Numbers& n) {
+  auto values_at = [&](uint32_t i, const Numbers& n) {
     const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * 64u + g * 16u) & (block - 1u);
-    const uint8_t* from = a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
-#pragma unroll
-    for (int x = 0; x < VL; ++x) {
-      const uint32_t d = 16u * x + r;
-      vr[x] = load_u4(from + (d < D ? d : r) * block);
-    }
-    vs = a.v_scale[static_cast<uint64_t>(page) * b.kv_heads + kv];
+    return a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
+  };
+  auto fetch_keys = [&](const uint8_t* from, int y, int x) {
+    const uint32_t d = 64u * x + 16u * g;
+    kr[y][x] = load_u4(from + 4u * y * D + (d < D ? d : 0u));
+  };
+  auto fetch_values = [&](const uint8_t* from, int x) {
+    const uint32_t d = 16u * x + r;
+    vr[x] = load_u4(from + (d < D ? d : r) * block);
+  };
+  auto fetch_scales = [&](const Numbers& n) {
     known = n.v < b.pages;
+    const uint64_t at = static_cast<uint64_t>(known ? n.v : 0u) * b.kv_heads + kv;
+    ks = a.k_scale[at], vs = a.v_scale[at];
   };
 
   uint32_t i = begin + wave;
   Numbers next{0u, 0u};
   if (i < end) {
     const Numbers now = numbers(i);
-    fetch_keys(i, now);
-    fetch_values(i, now);
     if (i + NW < end) next = numbers(i + NW);
+    const uint8_t *from_k = keys_at(i, now), *from_v = values_at(i, now);
+    fetch_scales(now);
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+#pragma unroll
+      for (int x = 0; x < KL; ++x) fetch_keys(from_k, y, x);
+    }
+#pragma unroll
+    for (int x = 0; x < VL; ++x) fetch_values(from_v, x);
   }
 
-  // The queries' terms.
-  half8_t q_hi[CG][STEPS], q_lo[CG][STEPS];
+  // This lane's columns; past the last one, the last.  Each wavefront makes a share of the operands.
+  uint32_t pos[CG];
   float q_scale[CG];
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
-    float raw[STEPS][8], most = 0.0f;
-#pragma unroll
-    for (int x = 0; x < STEPS; ++x) {
-      const uint32_t d = 64u * (x / 2) + 16u * g + 8u * (x % 2);
-#pragma unroll
-      for (int e = 0; e < 8; e += 4) {
-        const float4 v = d < D ? *reinterpret_cast<const float4*>(qp[cg] + d + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-        raw[x][e] = v.x, raw[x][e + 1] = v.y, raw[x][e + 2] = v.z, raw[x][e + 3] = v.w;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(raw[x][e]));
-    }
-    most = groups_max(most);
-    const float up = most == 0.0f ? 1.0f : power_to(most, 13);
-    q_scale[cg] = kLog2E / sqrtf(static_cast<float>(D)) / up;
-#pragma unroll
-    for (int x = 0; x < STEPS; ++x) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = raw[x][e] * up;
-        const _Float16 h = static_cast<_Float16>(v);
-        q_hi[cg][x][e] = h, q_lo[cg][x][e] = static_cast<_Float16>(v - static_cast<float>(h));
-      }
-    }
+    const uint32_t at = cg * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
+    pos[cg] = past + row;
+    q_scale[cg] = query_terms<KIND, DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, sh.q[cg], wave, NW);
   }
+  lds_barrier();
 
   Column col[CG];
   float4_t o[CG][VL];
@@ -283,31 +338,85 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
 #pragma unroll
     for (int x = 0; x < VL; ++x) o[cg][x] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  for (; i < end; i += NW) {
-    const bool more = i + NW < end;
-    float4_t acc[CG][4];
-#pragma unroll
-    for (int cg = 0; cg < CG; ++cg) {
-#pragma unroll
-      for (int y = 0; y < 4; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-#pragma unroll
-    for (int x = 0; x < STEPS; ++x) {
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint4 run = kr[y][x / 2];
-        const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
-#pragma unroll
-        for (int cg = 0; cg < CG; ++cg) {
-          acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q_lo[cg][x], acc[cg][y], 0, 0, 0);
-          acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, q_hi[cg][x], acc[cg][y], 0, 0, 0);
-        }
-      }
-    }
+  auto tile = [&](auto last) {
+    constexpr bool MORE = !decltype(last)::value;
     const uint32_t first = tile_at(w, i) * 64u;
     const float k_scale = ks, v_scale = vs;
     const bool in_pool = known;
-    if (more) fetch_keys(i + NW, next);
+    const uint8_t *from_k = nullptr, *from_v = nullptr;
+    if constexpr (MORE) from_k = keys_at(i + NW, next), from_v = values_at(i + NW, next);
+    float4_t acc[CG][4];
+    if constexpr (KIND == PageKind::Q8) {
+      constexpr int YB = 2;                                         // key operands that share a query operand's way from LDS
+#pragma unroll
+      for (int y0 = 0; y0 < 4; y0 += YB) {
+        int4_t sum[CG][YB][3];
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+          for (int y = 0; y < YB; ++y) sum[cg][y][0] = sum[cg][y][1] = sum[cg][y][2] = int4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int x = 0; x < KL; ++x) {
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+            for (int n = 0; n < 3; ++n) {
+              const int4_t q = bit_cast<int4_t>(sh.q[cg][3 * x + n][lane]);
+#pragma unroll
+              for (int y = 0; y < YB; ++y) {
+                sum[cg][y][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bit_cast<int4_t>(kr[y0 + y][x]), q, sum[cg][y][n], 0, 0, 0);
+              }
+            }
+          }
+          if constexpr (MORE) {
+#pragma unroll
+            for (int y = 0; y < YB; ++y) fetch_keys(from_k, y0 + y, x);
+          }
+        }
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+          for (int y = 0; y < YB; ++y) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              // (the lower two together are below 2^31)
+              const float low = static_cast<float>((sum[cg][y][1][e] << 8) + sum[cg][y][0][e]);
+              acc[cg][y0 + y][e] = fmaf(static_cast<float>(sum[cg][y][2][e]), 65536.0f, low);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      }
+#pragma unroll
+      for (int x = 0; x < 2 * KL; ++x) {
+        half8_t hi[CG], lo[CG];
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) hi[cg] = bit_cast<half8_t>(sh.q[cg][2 * x][lane]), lo[cg] = bit_cast<half8_t>(sh.q[cg][2 * x + 1][lane]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const uint4 run = kr[y][x / 2];
+          const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) {
+            acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, lo[cg], acc[cg][y], 0, 0, 0);
+            acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, hi[cg], acc[cg][y], 0, 0, 0);
+          }
+          if constexpr (MORE) {
+            if (x % 2 == 1) fetch_keys(from_k, y, x / 2);
+          }
+        }
+      }
+    }
+    if constexpr (MORE) {
+      fetch_scales(next);
+      if (i + 2 * NW < end) next = numbers(i + 2 * NW);
+    }
     // Every column sees every position of the tile, or it goes by bits.
     const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
     half8_t p_hi[CG][2], p_lo[CG][2];
@@ -344,10 +453,11 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
         o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p_hi[cg][0], o[cg][x], 0, 0, 0);
         o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p_hi[cg][1], o[cg][x], 0, 0, 0);
       }
+      if constexpr (MORE) fetch_values(from_v, x);
     }
-    if (more) fetch_values(i + NW, next);
-    if (i + 2 * NW < end) next = numbers(i + 2 * NW);
-  }
+  };
+  for (; i + NW < end; i += NW) tile(std::false_type{});
+  if (i < end) tile(std::true_type{});
 
   // Merge of the wavefronts under the largest reference.
 #pragma unroll
@@ -355,7 +465,7 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
     const float total = groups_sum(col[cg].sum);
     if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = total;
   }
-  __syncthreads();
+  __syncthreads();                                                  // (no wavefront reads the queries any more)
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
     float top = -INFINITY;
@@ -393,37 +503,50 @@ __global__ __launch_bounds__(NW * 64) void attention_pages_few_kernel(PageAttent
 
 // ---- the parts' merge ----------------------------------------------------------------------------
 
-// A workgroup a column: its parts' sums under the largest of their references.
+// A workgroup a column: its parts' sums under the largest of their references, all loads under way at once.
+constexpr uint32_t kPagePartsMost = 256;
 template <int C>
 __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttention a) {
-  __shared__ alignas(16) float piece[256 * 4];
+  __shared__ float of_wave[2][4], weight[kPagePartsMost];
+  __shared__ alignas(16) float4_t piece[256];
   const PageBatch& b = a.batch;
-  const uint32_t c = blockIdx.x % C, rest = blockIdx.x / C, kv = rest % b.kv_heads, unit = rest / b.kv_heads;
+  const uint32_t c = blockIdx.x % C, rest = blockIdx.x / C, kv = rest % b.kv_heads, unit = rest / b.kv_heads, t = threadIdx.x;
   PageUnit u;
   if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
   const UnitTiles w = unit_tiles(a, u, C);
   if (c >= w.columns || w.tiles <= a.part_tiles) return;            // workgroup-uniform
-  const uint32_t parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles, D = b.head_dim, runs = D / 4u, t = threadIdx.x;
+  const uint32_t parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles, D = b.head_dim, runs = D / 4u;
   const uint64_t at = (static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts * C + c;
-  float top = -INFINITY;
-  for (uint32_t p = 0; p < parts; ++p) top = fmaxf(top, a.part_most[at + static_cast<uint64_t>(p) * C]);
-  const float to = from_reference(top);
-  // 256 / runs threads a run of four elements
-  const uint32_t lanes = 256u / runs, own = t / runs, d = t % runs * 4u;
-  float total = 0.0f;
-  float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t p = own; p < parts && own < lanes; p += lanes) {
-    const uint64_t from = at + static_cast<uint64_t>(p) * C;
-    x += *reinterpret_cast<const float4_t*>(a.part_sum + from * D + d) * __builtin_amdgcn_exp2f(a.part_most[from] - to);
-  }
-  for (uint32_t p = 0; p < parts; ++p) {
-    const uint64_t from = at + static_cast<uint64_t>(p) * C;
-    total = fmaf(__builtin_amdgcn_exp2f(a.part_most[from] - to), a.part_total[from], total);
-  }
-  reinterpret_cast<float4_t*>(piece)[t] = x;
+  const float own = t < parts ? a.part_most[at + static_cast<uint64_t>(t) * C] : -INFINITY, sum = t < parts ? a.part_total[at + static_cast<uint64_t>(t) * C] : 0.0f;
+  // 256 / runs threads a run of four elements; the first parts' sums are asked for before their weights are there
+  constexpr uint32_t AHEAD = 4;
+  const uint32_t lanes = 256u / runs, mine = t / runs, d = t % runs * 4u;
+  float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f}, early[AHEAD];
+  auto load = [&](uint32_t p) { return p < parts && mine < lanes ? *reinterpret_cast<const float4_t*>(a.part_sum + (at + static_cast<uint64_t>(p) * C) * D + d) : x; };
+#pragma unroll
+  for (uint32_t i = 0; i < AHEAD; ++i) early[i] = load(mine + i * lanes);
+  const float most = wave_max(own);
+  if ((t & 63u) == 0u) of_wave[0][t >> 6] = most;
   __syncthreads();
-  if (own != 0u) return;
-  for (uint32_t n = 1; n < lanes; ++n) x += reinterpret_cast<const float4_t*>(piece)[n * runs + t];
+  const float top = fmaxf(fmaxf(of_wave[0][0], of_wave[0][1]), fmaxf(of_wave[0][2], of_wave[0][3]));
+  const float f = t < parts ? __builtin_amdgcn_exp2f(own - from_reference(top)) : 0.0f;
+  weight[t] = f;
+  const float total_of = wave_sum(f * sum);
+  if ((t & 63u) == 0u) of_wave[1][t >> 6] = total_of;
+  __syncthreads();
+  const float total = (of_wave[1][0] + of_wave[1][1]) + (of_wave[1][2] + of_wave[1][3]);
+#pragma unroll
+  for (uint32_t i = 0; i < AHEAD; ++i) {
+    if (mine + i * lanes < parts) x += early[i] * weight[mine + i * lanes];
+  }
+#pragma unroll 4
+  for (uint32_t p = mine + AHEAD * lanes; p < parts; p += lanes) {
+    if (mine < lanes) x += *reinterpret_cast<const float4_t*>(a.part_sum + (at + static_cast<uint64_t>(p) * C) * D + d) * weight[p];
+  }
+  piece[t] = x;
+  __syncthreads();
+  if (mine != 0u) return;
+  for (uint32_t n = 1; n < lanes; ++n) x += piece[n * runs + t];
   const uint32_t pair = w.first_col + c;
   float* out = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
   *reinterpret_cast<float4_t*>(out) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
@@ -451,7 +574,8 @@ size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape&
 }
 
 PagesShape attention_pages_shape(const PageAttentionCall& c, uint64_t most_parts) {
-  PagesShape shape{16, 1, tiles_of(c)};
+  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs > 16 && c.page.head_dim <= 128 ? 32 : 16;
+  PagesShape shape{columns, 1, tiles_of(c)};
   const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads, cus = static_cast<uint64_t>(num_cus());
   uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
   if (parts > most_parts) parts = most_parts;
@@ -462,7 +586,7 @@ PagesShape attention_pages_shape(const PageAttentionCall& c, uint64_t most_parts
     if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
     --parts;
   }
-  return PagesShape{16, 1, tiles_of(c)};
+  return PagesShape{columns, 1, tiles_of(c)};
 }
 
 hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
@@ -484,18 +608,26 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
     a.part_most = a.part_sum + columns * c.page.head_dim;
     a.part_total = a.part_most + columns;
   }
-  auto few = [&](auto kind, auto dim) {
-    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, 1, 4>), dim3(static_cast<uint32_t>(groups * shape.parts)),
-                       dim3(256), 0, stream, a);
+  auto few = [&](auto kind, auto dim, auto cg) {
+    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, decltype(cg)::value, 4>),
+                       dim3(static_cast<uint32_t>(groups * shape.parts)), dim3(256), 0, stream, a);
+  };
+  auto with_columns = [&](auto kind, auto dim) {
+    if constexpr (decltype(dim)::value <= 128) {
+      if (shape.columns == 32) return few(kind, dim, std::integral_constant<int, 2>{});
+    }
+    few(kind, dim, std::integral_constant<int, 1>{});
   };
   auto with_dim = [&](auto kind) {
     const uint64_t D = c.page.head_dim;
-    D <= 64 ? few(kind, std::integral_constant<int, 64>{}) : D <= 128 ? few(kind, std::integral_constant<int, 128>{}) : few(kind, std::integral_constant<int, 256>{});
+    D <= 64 ? with_columns(kind, std::integral_constant<int, 64>{}) : D <= 128 ? with_columns(kind, std::integral_constant<int, 128>{})
+                                                                     : with_columns(kind, std::integral_constant<int, 256>{});
   };
   fp8 ? with_dim(std::integral_constant<PageKind, PageKind::Fp8>{}) : with_dim(std::integral_constant<PageKind, PageKind::Q8>{});
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || shape.parts < 2) return e;
-  hipLaunchKernelGGL((attention_pages_merge_kernel<16>), dim3(static_cast<uint32_t>(groups * 16)), dim3(256), 0, stream, a);
+  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups * shape.columns)), dim3(256), 0, stream, a); };
+  shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : merge(attention_pages_merge_kernel<32>);
   return hipGetLastError();
 }
 

@@ -89,8 +89,9 @@ def attention(pool, table, length, q, group, window=0, sinks=0):
     """q: rows x heads x d, the last rows of a sequence.  Returns the result in 64 bits and how far fp32 sums may be from it.
 
     A score is a sum of d products: an element enters to 2^-22 of itself (two fp16 terms) or, where the second is subnormal, to half
-    of 2^-24 under a power of two that brings the row's largest to 2^13 at least; the products are exact, each addition rounds to
-    2^-24 of at most the sum of their magnitudes; then a few roundings (scales, log2 e, the reference) of the score.  A weight is
+    of 2^-24 under a power of two that brings the row's largest to 2^13 at least; over int8 pages to half a step of an integer whose
+    largest is 8355584 (2^-23 of the row's largest: 2^-24 and the rounding of what it is multiplied by); the products are exact, each
+    addition rounds to 2^-24 of at most the sum of their magnitudes; then a few roundings (scales, log2 e, the reference) of the score.  A weight is
     off by that, relatively, and by the exponential's and its own two terms' 2^-21 or, where the second is subnormal, by half of
     2^-24 under a power of two that brings the row's largest weight times value scale to 2^9 at least: 2^-34 of that, times each
     value's code.  Sums of n weights and products are off by n + 64 roundings."""
@@ -110,7 +111,7 @@ def attention(pool, table, length, q, group, window=0, sinks=0):
                 s, mass = kk @ x / np.sqrt(d), np.abs(kk) @ np.abs(x) / np.sqrt(d)
                 p = np.exp(s - s.max())
                 out[i, h] = p @ vv / p.sum()
-                low = 2.0 ** -38 * np.abs(x).max() * np.abs(kk).sum(1).max() / np.sqrt(d)
+                low = 2.0 ** (-23 if pool.fmt == "q8" else -38) * np.abs(x).max() * np.abs(kk).sum(1).max() / np.sqrt(d)
                 off = mass.max() * (2.0 ** -22 + (d + 8) * EPS) + low + np.abs(s).max() * 8 * EPS
                 bound[i, h] = (np.expm1(2 * off) + 2.0 ** -20 + (len(at) + 64) * 2 * EPS) * (p @ np.abs(vv) / p.sum())
                 vs = v_scale[at, h // group]
@@ -173,7 +174,7 @@ def verify(logits, tokens, random, starts, temperature, draft=None, draft_temper
                 p = rest if rest.sum() > 0 else p
             run = np.cumsum(p)
             u = float(random[row, 1])
-            over = np.nonzero(run > (u if u >= 0 else 0.0) * run[-1])[0]
+            over = np.nonzero(run > (min(u, 1.0 - 2.0 ** -24) if u >= 0 else 0.0) * run[-1])[0]     # (outside [0, 1): the nearest in it)
             out.append((at, int(over[0]) if len(over) else int(np.nonzero(p > 0)[0][-1])))
             break
     return out
