@@ -97,6 +97,23 @@ __device__ __forceinline__ float power_to(float v, int target) {
 }
 __device__ __forceinline__ float from_reference(float ref) { return ref == -INFINITY ? 0.0f : ref; }
 
+// Sums times corr, now and then.  In place, by hand: of a branch around products the compiler makes a second set of registers and moves
+// the sums from one to the other in every tile.  (The matrix instructions behind the sums have been
+// waited for: at most sixteen passes of four cycles.)
+template <int N>
+__device__ __forceinline__ void scale_sums(float4_t (&o)[N], float corr) {
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15\n\ts_nop 15" ::);
+#pragma unroll
+  for (int x = 0; x < N; ++x) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = o[x][e];
+      asm volatile("v_mul_f32 %0, %1, %0" : "+v"(v) : "v"(corr));
+      o[x][e] = v;
+    }
+  }
+}
+
 // Weights are taken relative to a reference that follows a column's largest score only where that would leave it by 2^kSlack.
 constexpr float kSlack = 3.0f;
 
@@ -104,14 +121,17 @@ constexpr float kSlack = 3.0f;
 struct Column {
   float ref = -INFINITY;          // in powers of two
   float sum = 0.0f;               // of weights, this lane's share
-  float most = 0.0f;              // the largest weight times value scale so far, this lane's
+  float most = 0.0f;              // a weight times its value's scale that was met, the largest where it was looked for, this lane's
   float up = 0x1p127f;            // the power of two over those
 };
 
-// Scores (in powers of two) to weights times the values' scale, as two terms; returns what the sums so far are to be scaled by.
-// COUNT of a lane's positions of the tile; bit i of `shown`: the column sees the i-th.
+// Products to weights times the values' scale, as two terms; `scale` makes a product a score in powers of two.  COUNT of a lane's positions
+// of the tile; bit i of `shown`: the column sees the i-th; `all`: every column sees all.  A weight is below 2^kSlack, so that with
+// v_scale * up below 2^12 all is as it should be; else, and where the reference moves, the sums so far are to be scaled by *corr (true).
 template <int COUNT>
-__device__ __forceinline__ float weigh(Column& c, float (&s)[COUNT], uint32_t shown, bool all, float v_scale, half8_t (&hi)[COUNT / 8], half8_t (&lo)[COUNT / 8]) {
+__device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale, uint32_t shown, bool all, float v_scale, half8_t (&hi)[COUNT / 8],
+                                      half8_t (&lo)[COUNT / 8], float* corr) {
+  scale = scale == 0.0f ? 0x1p-126f : scale;      // (keys that are all 0: a hidden product stays -infinity)
   if (!all) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) s[i] = (shown >> i & 1u) != 0u ? s[i] : -INFINITY;
@@ -119,44 +139,41 @@ __device__ __forceinline__ float weigh(Column& c, float (&s)[COUNT], uint32_t sh
   float most = s[0];
 #pragma unroll
   for (int i = 1; i < COUNT; ++i) most = fmaxf(most, s[i]);
-  float corr = 1.0f;
-  const bool moves = __any(most > c.ref + kSlack || (c.ref == -INFINITY && most > -INFINITY));
+  most *= scale;
+  const bool moves = __any(most > c.ref + kSlack || (c.ref == -INFINITY && most > -INFINITY) || !(v_scale * c.up < 0x1p12f));
   if (moves) {
     const float before = c.ref;
     c.ref = fmaxf(c.ref, groups_max(most));
-    corr = before == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - c.ref);
-    c.sum *= corr, c.most *= corr;
-  }
-  const float to = from_reference(c.ref);
-  const float here = __builtin_amdgcn_exp2f(most - to) * v_scale;
-  c.most = fmaxf(c.most, here);
-  if (moves || __any(!(here * c.up < 0x1p15f))) {
+    float by = before == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - c.ref);
+    c.sum *= by;
+    c.most = fmaxf(c.most * by, __builtin_amdgcn_exp2f(most - from_reference(c.ref)) * v_scale);
     const float largest = groups_max(c.most), scaled = largest * c.up;
-    if (largest > 0.0f && !(scaled >= 0x1p9f && scaled < 0x1p15f)) {
-      const float up = power_to(largest, 13);
-      corr *= up / c.up;
+    if (largest > 0.0f && !(scaled >= 0x1p9f && scaled < 0x1p12f)) {
+      const float up = power_to(largest, 10);
+      by *= up * (1.0f / c.up);                   // (powers of two)
       c.up = up;
     }
+    *corr = by;
   }
-  const float factor = v_scale * c.up;
-  float w[COUNT];
+  const float to = from_reference(c.ref), factor = v_scale * c.up;
+  typedef float float2_v __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int i = 0; i < COUNT; ++i) {
-    const float p = __builtin_amdgcn_exp2f(s[i] - to);
-    c.sum += p;
-    w[i] = p * factor;
-  }
-  if (!all) {
+  for (int i = 0; i < COUNT; i += 2) {
+    float2_v w;
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) w[i] = (shown >> i & 1u) != 0u ? w[i] : 0.0f;     // (a hidden value's scale may be NaN)
+    for (int e = 0; e < 2; ++e) {
+      float p = __builtin_amdgcn_exp2f(fmaf(s[i + e], scale, -to));
+      if (!all) p = (shown >> (i + e) & 1u) != 0u ? p : 0.0f;                             // (a hidden position's scales may be NaN)
+      c.sum += p;
+      w[e] = p * factor;
+      if (!all) w[e] = (shown >> (i + e) & 1u) != 0u ? w[e] : 0.0f;
+    }
+    const half2_t h = __builtin_convertvector(w, half2_t);
+    const float2_v rest = {fmaf(static_cast<float>(h[0]), -1.0f, w[0]), fmaf(static_cast<float>(h[1]), -1.0f, w[1])};
+    const half2_t l = __builtin_convertvector(rest, half2_t);
+    hi[i / 8][i % 8] = h[0], hi[i / 8][i % 8 + 1] = h[1], lo[i / 8][i % 8] = l[0], lo[i / 8][i % 8 + 1] = l[1];
   }
-#pragma unroll
-  for (int i = 0; i < COUNT; ++i) {
-    const _Float16 h = static_cast<_Float16>(w[i]);
-    hi[i / 8][i % 8] = h;
-    lo[i / 8][i % 8] = static_cast<_Float16>(w[i] - static_cast<float>(h));
-  }
-  return corr;
+  return moves;
 }
 
 // ---- few columns ---------------------------------------------------------------------------------
@@ -422,10 +439,9 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
     half8_t p_hi[CG][2], p_lo[CG][2];
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
-      float s[16];
-      const float scale = q_scale[cg] * k_scale;
+      float s[16], corr;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = acc[cg][e / 4][e % 4] * scale;
+      for (int e = 0; e < 16; ++e) s[e] = acc[cg][e / 4][e % 4];
       uint32_t shown = 0xFFFFu;
       if (!all) {
         const uint32_t p0 = first + 16u * g;
@@ -433,15 +449,11 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
 #pragma unroll
         for (uint32_t e = 0; e < 16u; ++e) {
           const uint32_t p = p0 + e;
-          const bool sees = p <= pos[cg] && (a.window == 0u || pos[cg] - p < a.window || p < a.sinks);
-          shown |= (in_pool && sees ? 1u : 0u) << e;
+          const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & in_pool;
+          shown |= (sees ? 1u : 0u) << e;
         }
       }
-      const float corr = weigh<16>(col[cg], s, shown, all, v_scale, p_hi[cg], p_lo[cg]);
-      if (__any(corr != 1.0f)) {
-#pragma unroll
-        for (int x = 0; x < VL; ++x) o[cg][x] *= corr;
-      }
+      if (weigh<16>(col[cg], s, q_scale[cg] * k_scale, shown, all, v_scale, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
     }
 #pragma unroll
     for (int x = 0; x < VL; ++x) {
@@ -501,6 +513,285 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
   }
 }
 
+// ---- many columns --------------------------------------------------------------------------------
+//
+// Bound by the matrix instructions and the vector instructions beside them.  64 columns a workgroup, 4 / CG groups of 16 CG times two halves
+// of a tile of 64 positions: of each page's sixteen positions of the tile a wavefront takes the first or the last eight.  (CG 2 reads half as
+// much of the LDS; of heads of 256 its sums are more registers than there are.)
+// The tile's operands lie in LDS, made once for all columns: keys' as few_kernel's (int8 codes as they are), values' as fp16,
+// each operand's 64 lanes side by side, so that every write and read is whole lines.  While a tile is multiplied the next one goes to the
+// other half of the LDS and the one after that is under way.
+template <PageKind KIND, int DP>
+struct TileShared {
+  static constexpr int KEYS = (KIND == PageKind::Q8 ? 4 : 8) * (DP / 64), VALUES = 2 * (DP / 16);   // operands of a tile
+  static constexpr int QUERIES = query_operands(KIND, DP);
+  union {
+    uint4 stage[2][KEYS + VALUES][64];
+    uint4 q[4][QUERIES][64];                                        // of four groups of 16 columns, before the first tile
+    float4_t o[4][DP / 16][64];                                     // of the second half, behind the last
+  };
+  float scale[64], ref[2][64], sum[2][64];
+};
+
+template <PageKind KIND, int DP, int CG>
+__global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageAttention a) {
+  constexpr int KL = DP / 64, VL = DP / 16, C = 64, WAVES = 8 / CG, GROUPS = 4 / CG;
+  constexpr int KOWN = 4 * KL / WAVES, VOWN = VL / WAVES;           // a thread's runs of a tile
+  using Shared = TileShared<KIND, DP>;
+  __shared__ Shared sh;
+  const PageBatch& b = a.batch;
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
+  const uint32_t group = wave % GROUPS, half = wave / GROUPS;
+  const uint32_t kv = blockIdx.x % b.kv_heads, rest = blockIdx.x / b.kv_heads, part = rest % a.parts, unit = rest / a.parts;
+  PageUnit u;
+  if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
+  u.at = (u.seq.rows * a.group + C - 1u) / C - 1u - u.at;           // the last rows, which see most, first
+  const UnitTiles w = unit_tiles(a, u, C);
+  const uint32_t begin = part * a.part_tiles;
+  if (begin >= w.tiles) return;                                     // workgroup-uniform
+  const uint32_t end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
+  const uint32_t D = b.head_dim, block = 1u << b.log_block, past = u.seq.len - u.seq.rows;
+
+  const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
+  const uint32_t last_slot = (u.seq.len - 1u) >> b.log_block;
+  auto slot_of = [&](uint32_t position) {
+    const uint32_t s = position >> b.log_block;
+    return s < last_slot ? s : last_slot;
+  };
+  struct Numbers {
+    uint32_t k, v;
+  };
+  auto numbers = [&](uint32_t i) {
+    const uint32_t p0 = tile_at(w, i < end ? i : end - 1u) * 64u;
+    return Numbers{table[slot_of(p0 + (r >> 2) * 16u)], table[slot_of(p0 + g * 16u)]};
+  };
+  // A thread's share of a tile: key operand wave % 4, runs wave / 4, ...; value operands wave, wave + WAVES, ...; and its lane's scales.
+  uint4 kr[KOWN], vr[VOWN];
+  struct Scales {
+    float k, v;
+    uint32_t known;
+  };
+  const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
+  auto key_run = [&](int x) { return (WAVES / 4u) * x + wave / 4u; };
+  auto fetch_keys = [&](uint32_t i, const Numbers& n) {
+    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i < end ? i : end - 1u) * 64u + (r >> 2) * 16u) & (block - 1u);
+    const uint8_t* from = a.k + page * page_bytes + (kv * block + at + (r & 3u) + 4u * (wave & 3u)) * D;
+#pragma unroll
+    for (int x = 0; x < KOWN; ++x) {
+      const uint32_t d = 64u * key_run(x) + 16u * g;
+      kr[x] = load_u4(from + (d < D ? d : 0u));
+    }
+  };
+  auto fetch_values = [&](uint32_t i, const Numbers& n) {
+    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i < end ? i : end - 1u) * 64u + g * 16u) & (block - 1u);
+    const uint8_t* from = a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
+#pragma unroll
+    for (int x = 0; x < VOWN; ++x) {
+      const uint32_t d = 16u * (WAVES * x + wave) + r;
+      vr[x] = load_u4(from + (d < D ? d : r) * block);
+    }
+  };
+  auto fetch_scales = [&](const Numbers& n) {
+    const uint32_t known = n.v < b.pages ? 1u : 0u;
+    const uint64_t at = static_cast<uint64_t>(known != 0u ? n.v : 0u) * b.kv_heads + kv;
+    return Scales{a.k_scale[at], a.v_scale[at], known};
+  };
+  auto stash_keys = [&](uint32_t to, int x) {
+    const uint32_t at = (wave & 3u) * KL + key_run(x);
+    if constexpr (KIND == PageKind::Q8) {
+      sh.stage[to][at][lane] = kr[x];
+    } else {
+      sh.stage[to][2u * at][lane] = bit_cast<uint4>(operand<KIND>(kr[x].x, kr[x].y));
+      sh.stage[to][2u * at + 1u][lane] = bit_cast<uint4>(operand<KIND>(kr[x].z, kr[x].w));
+    }
+  };
+  auto stash_values = [&](uint32_t to, int x) {
+    const uint32_t at = Shared::KEYS + 2u * (WAVES * x + wave);
+    sh.stage[to][at][lane] = bit_cast<uint4>(operand<KIND>(vr[x].x, vr[x].y));
+    sh.stage[to][at + 1u][lane] = bit_cast<uint4>(operand<KIND>(vr[x].z, vr[x].w));
+  };
+
+  const Numbers of_first = numbers(begin), of_second = numbers(begin + 1u);
+  Numbers next = numbers(begin + 2u);                               // of the tile after the next
+  fetch_keys(begin, of_first);
+  fetch_values(begin, of_first);
+  Scales scales = fetch_scales(of_first), of_next = fetch_scales(of_second);
+
+  // The queries' operands: a wavefront makes those of 16 columns (of eight wavefronts two share them), and takes those of its own.
+  auto column_row = [&](uint32_t at) {
+    const uint32_t col = w.first_col + (at < w.columns ? at : w.columns - 1u);
+    return col / a.group;
+  };
+  {
+    const uint32_t own = wave & 3u, at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
+    const float scale = query_terms<KIND, DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, sh.q[own], wave / 4u, WAVES / 4u);
+    if (g == 0u) sh.scale[own * 16u + r] = scale;
+  }
+  lds_barrier();
+  uint4 q[CG][Shared::QUERIES];
+  uint32_t pos[CG];
+  float q_scale[CG];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const uint32_t from = group * CG + cg;
+#pragma unroll
+    for (int x = 0; x < Shared::QUERIES; ++x) q[cg][x] = sh.q[from][x][lane];
+    q_scale[cg] = sh.scale[from * 16u + r];
+    pos[cg] = past + column_row(from * 16u + r);
+  }
+  lds_barrier();                                                    // the first tile goes where they were
+#pragma unroll
+  for (int x = 0; x < KOWN; ++x) stash_keys(0u, x);
+#pragma unroll
+  for (int x = 0; x < VOWN; ++x) stash_values(0u, x);
+  fetch_keys(begin + 1u, of_second);
+  fetch_values(begin + 1u, of_second);
+  lds_barrier();
+
+  Column col[CG];
+  float4_t o[CG][VL];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+    for (int x = 0; x < VL; ++x) o[cg][x] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (uint32_t i = begin, buf = 0u; i < end; ++i, buf ^= 1u) {
+    const uint32_t first = tile_at(w, i) * 64u;
+    const Scales after = fetch_scales(next);
+    const Numbers further = numbers(i + 3u);
+    // Scores of the key operands 2 half, 2 half + 1.
+    float s[CG][8];
+    if constexpr (KIND == PageKind::Q8) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        int4_t sum[CG][3];
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) sum[cg][0] = sum[cg][1] = sum[cg][2] = int4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < KL; ++x) {
+          const int4_t key = bit_cast<int4_t>(sh.stage[buf][(2u * half + y) * KL + x][lane]);
+#pragma unroll
+          for (int n = 0; n < 3; ++n) {
+#pragma unroll
+            for (int cg = 0; cg < CG; ++cg) sum[cg][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(key, bit_cast<int4_t>(q[cg][3 * x + n]), sum[cg][n], 0, 0, 0);
+          }
+          constexpr int EACH = 2 * KL / KOWN;
+          if ((KL * y + x) % EACH == EACH - 1) stash_keys(buf ^ 1u, (KL * y + x) / EACH);
+        }
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[cg][4 * y + e] = fmaf(static_cast<float>(sum[cg][2][e]), 65536.0f, static_cast<float>((sum[cg][1][e] << 8) + sum[cg][0][e]));
+          }
+        }
+      }
+    } else {
+      float4_t acc[CG][2];
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) acc[cg][0] = acc[cg][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < 2 * KL; ++x) {
+        half8_t key[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) key[y] = bit_cast<half8_t>(sh.stage[buf][(2u * half + y) * (2 * KL) + x][lane]);
+#pragma unroll
+        for (int term = 1; term >= 0; --term) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int cg = 0; cg < CG; ++cg) acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[y], bit_cast<half8_t>(q[cg][2 * x + term]), acc[cg][y], 0, 0, 0);
+          }
+        }
+        if (x % (2 * KL / KOWN) == 1) stash_keys(buf ^ 1u, x / (2 * KL / KOWN));
+      }
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[cg][e] = acc[cg][e / 4][e % 4];
+      }
+    }
+    fetch_keys(i + 2u, next);
+    const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(scales.known != 0u);
+    half8_t p_hi[CG][1], p_lo[CG][1];
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      float corr;
+      uint32_t shown = 0xFFu;
+      if (!all) {
+        const uint32_t p0 = first + 16u * g + 8u * half;
+        shown = 0u;
+#pragma unroll
+        for (uint32_t e = 0; e < 8u; ++e) {
+          const uint32_t p = p0 + e;
+          const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & (scales.known != 0u);
+          shown |= (sees ? 1u : 0u) << e;
+        }
+      }
+      if (weigh<8>(col[cg], s[cg], q_scale[cg] * scales.k, shown, all, scales.v, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
+    }
+#pragma unroll
+    for (int x = 0; x < VL; x += 4 / CG) {
+      half8_t value[4 / CG];
+#pragma unroll
+      for (int y = 0; y < 4 / CG; ++y) value[y] = bit_cast<half8_t>(sh.stage[buf][Shared::KEYS + 2 * (x + y) + half][lane]);
+#pragma unroll
+      for (int term = 1; term >= 0; --term) {                       // (the same sum's products four apart)
+#pragma unroll
+        for (int y = 0; y < 4 / CG; ++y) {
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) o[cg][x + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[y], term == 1 ? p_lo[cg][0] : p_hi[cg][0], o[cg][x + y], 0, 0, 0);
+        }
+      }
+      if ((x + 4 / CG) % WAVES == 0) stash_values(buf ^ 1u, x / WAVES);
+    }
+    fetch_values(i + 2u, next);
+    scales = of_next, of_next = after, next = further;
+    lds_barrier();                                                  // (the loads stay under way)
+  }
+
+  // Merge of the halves.
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const float total = groups_sum(col[cg].sum);
+    if (g == 0u) sh.ref[half][(group * CG + cg) * 16u + r] = col[cg].ref, sh.sum[half][(group * CG + cg) * 16u + r] = total;
+  }
+  lds_barrier();
+  float factor[CG], top[CG], total[CG];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const uint32_t at = (group * CG + cg) * 16u + r;
+    const float ref0 = sh.ref[0][at], ref1 = sh.ref[1][at];
+    top[cg] = fmaxf(ref0, ref1);
+    const float to = from_reference(top[cg]);
+    total[cg] = fmaf(__builtin_amdgcn_exp2f(ref1 - to), sh.sum[1][at], __builtin_amdgcn_exp2f(ref0 - to) * sh.sum[0][at]);
+    factor[cg] = __builtin_amdgcn_exp2f(col[cg].ref - to) / col[cg].up;
+    if (half == 1u) {
+#pragma unroll
+      for (int x = 0; x < VL; ++x) sh.o[group * CG + cg][x][lane] = o[cg][x] * factor[cg];
+    }
+  }
+  lds_barrier();
+  if (half == 1u) return;
+  const bool whole = w.tiles <= a.part_tiles;                       // no other part has tiles
+  const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * C;
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const uint32_t c = (group * CG + cg) * 16u + r;
+    if (c >= w.columns) continue;
+    const uint32_t at = w.first_col + c;
+    float* to = whole ? a.out + (static_cast<uint64_t>(u.seq.first + at / a.group) * a.heads + kv * a.group + at % a.group) * D : a.part_sum + (slot + c) * D;
+    const float scale = !whole ? 1.0f : total[cg] == 0.0f ? 0.0f : 1.0f / total[cg];
+    if (!whole && g == 0u) a.part_most[slot + c] = top[cg], a.part_total[slot + c] = total[cg];
+#pragma unroll
+    for (int x = 0; x < VL; ++x) {
+      const uint32_t d = 16u * x + 4u * g;
+      const float4_t v = (o[cg][x] * factor[cg] + sh.o[group * CG + cg][x][lane]) * scale;
+      if (d < D) *reinterpret_cast<float4_t*>(to + d) = v;
+    }
+  }
+}
+
 // ---- the parts' merge ----------------------------------------------------------------------------
 
 // A workgroup a column: its parts' sums under the largest of their references, all loads under way at once.
@@ -513,6 +804,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   const uint32_t c = blockIdx.x % C, rest = blockIdx.x / C, kv = rest % b.kv_heads, unit = rest / b.kv_heads, t = threadIdx.x;
   PageUnit u;
   if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
+  if constexpr (C == 64) u.at = (u.seq.rows * a.group + C - 1u) / C - 1u - u.at;      // as the tiles' kernel has it
   const UnitTiles w = unit_tiles(a, u, C);
   if (c >= w.columns || w.tiles <= a.part_tiles) return;            // workgroup-uniform
   const uint32_t parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles, D = b.head_dim, runs = D / 4u;
@@ -574,7 +866,7 @@ size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape&
 }
 
 PagesShape attention_pages_shape(const PageAttentionCall& c, uint64_t most_parts) {
-  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs > 16 && c.page.head_dim <= 128 ? 32 : 16;
+  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && c.page.head_dim <= 128 ? 32 : 64;
   PagesShape shape{columns, 1, tiles_of(c)};
   const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads, cus = static_cast<uint64_t>(num_cus());
   uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
@@ -608,11 +900,17 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
     a.part_most = a.part_sum + columns * c.page.head_dim;
     a.part_total = a.part_most + columns;
   }
+  auto tile = [&](auto kind, auto dim) {
+    constexpr int CG = decltype(dim)::value == 256 ? 1 : 2;
+    hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, decltype(dim)::value, CG>), dim3(static_cast<uint32_t>(groups * shape.parts)),
+                       dim3(512 / CG), 0, stream, a);
+  };
   auto few = [&](auto kind, auto dim, auto cg) {
     hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, decltype(cg)::value, 4>),
                        dim3(static_cast<uint32_t>(groups * shape.parts)), dim3(256), 0, stream, a);
   };
   auto with_columns = [&](auto kind, auto dim) {
+    if (shape.columns == 64) return tile(kind, dim);
     if constexpr (decltype(dim)::value <= 128) {
       if (shape.columns == 32) return few(kind, dim, std::integral_constant<int, 2>{});
     }
@@ -627,7 +925,7 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || shape.parts < 2) return e;
   auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups * shape.columns)), dim3(256), 0, stream, a); };
-  shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : merge(attention_pages_merge_kernel<32>);
+  shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : shape.columns == 32 ? merge(attention_pages_merge_kernel<32>) : merge(attention_pages_merge_kernel<64>);
   return hipGetLastError();
 }
 

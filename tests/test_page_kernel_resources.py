@@ -7,7 +7,7 @@ from test_kernel_resources import HIPCC, resource_remarks
 
 
 @pytest.mark.skipif(shutil.which(HIPCC) is None, reason="hipcc not found")
-@pytest.mark.parametrize("src,wanted", [("attention_pages.hip", ["attention_pages_few_kernel", "attention_pages_merge_kernel"]),
+@pytest.mark.parametrize("src,wanted", [("attention_pages.hip", ["attention_pages_few_kernel", "attention_pages_tile_kernel", "attention_pages_merge_kernel"]),
                                         ("pages.hip", ["pages_write_kernel", "pages_read_kernel"]),
                                         ("draft_verify.hip", ["draft_stats_kernel", "draft_rest_kernel"])])
 def test_no_scratch_memory(src, wanted):
