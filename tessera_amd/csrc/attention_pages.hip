@@ -28,9 +28,9 @@ struct PageAttention {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   float* out;
-  float *part_sum, *part_most, *part_total;   // (unit, key head, part, column): head_dim sums; the reference in powers of two; the weights' sum
+  float *part_sum, *part_most, *part_total;   // (unit, key head, part, one of `stored` columns): head_dim sums; the reference in powers of two; the weights' sum
   uint32_t heads, group, window, sinks;       // window 0: every position
-  uint32_t parts, part_tiles;                 // tiles of 64 positions a part
+  uint32_t parts, part_tiles, stored, even;   // tiles of 64 positions a part; columns of a unit that a part has room for; workgroups of an even split, or 0
 };
 
 // ---- which positions a unit walks ----------------------------------------------------------------
@@ -43,18 +43,27 @@ struct UnitTiles {
   uint32_t low, high;             // the first and the last row's positions
   uint32_t sink_tiles, from_tile, tiles;
 };
-__device__ __forceinline__ UnitTiles unit_tiles(const PageAttention& a, const PageUnit& u, uint32_t most_columns) {
-  UnitTiles w;
-  const uint32_t all = u.seq.rows * a.group;
-  w.first_col = u.at * most_columns;
-  w.columns = all - w.first_col < most_columns ? all - w.first_col : most_columns;
-  const uint32_t past = u.seq.len - u.seq.rows;
-  w.low = past + w.first_col / a.group, w.high = past + (w.first_col + w.columns - 1u) / a.group;
+__device__ __forceinline__ UnitTiles tiles_between(const PageAttention& a, uint32_t low, uint32_t high) {
+  UnitTiles w{};
+  w.low = low, w.high = high;
   const uint32_t begin = a.window != 0u && w.low + 1u > a.window ? w.low + 1u - a.window : 0u;
   const uint32_t sinks = a.sinks < begin ? a.sinks : begin;
   w.sink_tiles = (sinks + 63u) / 64u;
   w.from_tile = begin / 64u > w.sink_tiles ? begin / 64u : w.sink_tiles;
   w.tiles = w.sink_tiles + (w.high / 64u + 1u - w.from_tile);
+  return w;
+}
+// The one unit of a sequence whose pairs all fit.
+__device__ __forceinline__ UnitTiles sequence_tiles(const PageAttention& a, const PageSequence& seq) {
+  UnitTiles w = tiles_between(a, seq.len - seq.rows, seq.len - 1u);
+  w.columns = seq.rows * a.group;
+  return w;
+}
+__device__ __forceinline__ UnitTiles unit_tiles(const PageAttention& a, const PageUnit& u, uint32_t most_columns) {
+  const uint32_t all = u.seq.rows * a.group, first = u.at * most_columns, columns = all - first < most_columns ? all - first : most_columns;
+  const uint32_t past = u.seq.len - u.seq.rows;
+  UnitTiles w = tiles_between(a, past + first / a.group, past + (first + columns - 1u) / a.group);
+  w.first_col = first, w.columns = columns;
   return w;
 }
 __device__ __forceinline__ uint32_t tile_at(const UnitTiles& w, uint32_t i) { return i < w.sink_tiles ? i : w.from_tile + (i - w.sink_tiles); }
@@ -176,6 +185,33 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
   return moves;
 }
 
+// ---- an even split -------------------------------------------------------------------------------
+//
+// Of units that are a sequence each: all their tiles, a sequence's heads one behind the other, in runs of equal cost, one a workgroup.
+// To begin a head costs what kBegin tiles do: so many lie before its first, with nothing in them.  A run that covers a head whole gives
+// its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second those of
+// a later one.
+constexpr uint32_t kBegin = 6;
+__device__ __forceinline__ uint32_t even_of(const PageAttention& a, const PageSequence& seq) {
+  return seq.rows == 0u ? 0u : sequence_tiles(a, seq).tiles + kBegin;
+}
+struct EvenTiles {
+  uint32_t before, all;           // of a head of the sequences before the s-th; of all
+};
+__device__ __forceinline__ EvenTiles even_tiles(const PageAttention& a, uint32_t s) {
+  uint32_t before = 0u, all = 0u;
+  for (uint32_t at = threadIdx.x & 63u; at < a.batch.sequences; at += 64u) {
+    const uint32_t own = even_of(a, page_sequence(a.batch, at));
+    all += own, before += at < s ? own : 0u;
+  }
+  auto last = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(v)), 63)); };
+  return EvenTiles{last(before), last(all)};
+}
+__device__ __forceinline__ uint32_t even_share(uint32_t all, uint32_t workgroups, const PageBatch& b) {
+  const uint32_t share = (all * b.kv_heads + workgroups - 1u) / workgroups;
+  return all != 0u && share < kBegin + 4u ? kBegin + 4u : share;    // (a tile a wavefront)
+}
+
 // ---- few columns ---------------------------------------------------------------------------------
 //
 // Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of 64 positions on its own, with no
@@ -195,21 +231,30 @@ struct FewShared {
   float ref[NW][16 * CG], sum[NW][16 * CG];
 };
 
-// A row's elements 64 x + 16 g + e of lane group g as operands: over int8 pages the limbs of three of them, else two terms of the sixteen in
-// two steps.  Returns what a score is to be multiplied by.  Only the operands of steps `x % step == own` are written.
-template <PageKind KIND, int DP>
-__device__ __forceinline__ float query_terms(const float* q, uint32_t D, uint4 (*to)[64], uint32_t own, uint32_t step) {
-  const uint32_t lane = threadIdx.x & 63u, g = lane >> 4;
-  float raw[DP / 64][16], most = 0.0f;
-  bool odd = false;
+// A row's elements 64 x + 16 g + e of lane group g.
+template <int DP>
+__device__ __forceinline__ void query_load(const float* q, uint32_t D, float (&raw)[DP / 64][16]) {
+  const uint32_t g = (threadIdx.x & 63u) >> 4;
 #pragma unroll
   for (int x = 0; x < DP / 64; ++x) {
     const uint32_t d = 64u * x + 16u * g;
 #pragma unroll
     for (int e = 0; e < 16; e += 4) {
-      const float4 v = d < D ? *reinterpret_cast<const float4*>(q + d + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-      raw[x][e] = v.x, raw[x][e + 1] = v.y, raw[x][e + 2] = v.z, raw[x][e + 3] = v.w;
+      const float4 v = *reinterpret_cast<const float4*>(q + (d < D ? d : 0u) + e);
+      raw[x][e] = d < D ? v.x : 0.0f, raw[x][e + 1] = d < D ? v.y : 0.0f, raw[x][e + 2] = d < D ? v.z : 0.0f, raw[x][e + 3] = d < D ? v.w : 0.0f;
     }
+  }
+}
+
+// Those as operands: over int8 pages the limbs of three of them, else two terms of the sixteen in two steps.  Returns what a score is to
+// be multiplied by.  Only the operands of steps `x % step == own` are written.
+template <PageKind KIND, int DP>
+__device__ __forceinline__ float query_terms(const float (&raw)[DP / 64][16], uint32_t D, uint4 (*to)[64], uint32_t own, uint32_t step) {
+  const uint32_t lane = threadIdx.x & 63u;
+  float most = 0.0f;
+  bool odd = false;
+#pragma unroll
+  for (int x = 0; x < DP / 64; ++x) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) most = fmaxf(most, fabsf(raw[x][e])), odd = odd || !(fabsf(raw[x][e]) < INFINITY);
   }
@@ -263,7 +308,7 @@ __device__ __forceinline__ float query_terms(const float* q, uint32_t D, uint4 (
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
 template <PageKind KIND, int DP, int CG, int NW>
-constexpr int few_waves() { return DP == 64 ? (CG == 1 ? 3 : 2) : DP == 128 ? (CG == 1 ? 2 : 1) : 1; }   // a SIMD, by the registers
+constexpr int few_waves() { return DP * CG <= 128 ? 2 : 1; }   // a SIMD, by the registers
 
 template <PageKind KIND, int DP, int CG, int NW>
 __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void attention_pages_few_kernel(PageAttention a) {
@@ -271,14 +316,37 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
   __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
-  const uint32_t kv = blockIdx.x % b.kv_heads, rest = blockIdx.x / b.kv_heads, part = rest % a.parts, unit = rest / a.parts;
+  const uint32_t D = b.head_dim, block = 1u << b.log_block;
+  uint32_t at_tile = 0u, last_tile = 0u;
+  if (a.even != 0u) {
+    const uint32_t share = even_share(even_tiles(a, 0u).all, gridDim.x, b);
+    at_tile = blockIdx.x * share, last_tile = at_tile + share;
+  }
+  for (bool first_run = true;; first_run = false) {
   PageUnit u;
-  if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
-  const UnitTiles w = unit_tiles(a, u, C);
-  const uint32_t begin = part * a.part_tiles;
-  if (begin >= w.tiles) return;                                     // workgroup-uniform
-  const uint32_t end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
-  const uint32_t D = b.head_dim, block = 1u << b.log_block, past = u.seq.len - u.seq.rows;
+  UnitTiles w;
+  uint32_t kv, begin, end;
+  uint64_t slot;
+  if (a.even != 0u) {
+    if (at_tile >= last_tile || !find_unit(b, at_tile, [&](const PageSequence& q) { return even_of(a, q) * b.kv_heads; }, &u)) return;
+    const uint32_t in = u.at;
+    w = sequence_tiles(a, u.seq);
+    const uint32_t from = in % (w.tiles + kBegin), left = last_tile - at_tile, to = w.tiles + kBegin - from < left ? w.tiles + kBegin : from + left;
+    kv = in / (w.tiles + kBegin);
+    if (to <= kBegin) return;                                       // (the next workgroup begins it)
+    begin = from > kBegin ? from - kBegin : 0u, end = to - kBegin;
+    slot = 2u * static_cast<uint64_t>(blockIdx.x) + (first_run ? 0u : 1u);
+    at_tile += to - from;
+  } else {
+    const uint32_t rest = blockIdx.x / b.kv_heads, part = rest % a.parts;
+    if (!first_run || !find_unit(b, rest / a.parts, [](const PageSequence&) { return 1u; }, &u)) return;
+    w = sequence_tiles(a, u.seq);
+    kv = blockIdx.x % b.kv_heads, begin = part * a.part_tiles;
+    if (begin >= w.tiles) return;
+    end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
+    slot = (static_cast<uint64_t>(rest / a.parts) * b.kv_heads + kv) * a.parts + part;
+  }
+  const uint32_t past = u.seq.len - u.seq.rows;
 
   // Page numbers of a tile's sixteen positions r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
   const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
@@ -299,21 +367,21 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
   bool known;
   const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
   // Where a lane's runs of a tile begin.  (Elements past head_dim meet zeros of the queries, or are not stored.)
+  const uint32_t past_end = 16u * g < D % 64u ? 0u : 16u * g - (D % 64u == 0u ? 0u : D % 64u - 16u);       // in a run of 64 that is not whole
   auto keys_at = [&](uint32_t i, const Numbers& n) {
     const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * 64u + (r >> 2) * 16u) & (block - 1u);
-    return a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D;
+    return a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D + 16u * g;
   };
   auto values_at = [&](uint32_t i, const Numbers& n) {
     const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * 64u + g * 16u) & (block - 1u);
-    return a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
+    return a.v + page * page_bytes + (kv * D + r) * block + at;
   };
   auto fetch_keys = [&](const uint8_t* from, int y, int x) {
-    const uint32_t d = 64u * x + 16u * g;
-    kr[y][x] = load_u4(from + 4u * y * D + (d < D ? d : 0u));
+    const uint8_t* at = 64u * x + 64u <= D ? from : from - past_end;
+    kr[y][x] = load_u4(at + (4u * y * D + (64u * x < D ? 64u * x : 0u)));
   };
   auto fetch_values = [&](const uint8_t* from, int x) {
-    const uint32_t d = 16u * x + r;
-    vr[x] = load_u4(from + (d < D ? d : r) * block);
+    vr[x] = load_u4(from + (16u * x < D ? 16u * x * block : 0u));   // (uniform: no register of its own)
   };
   auto fetch_scales = [&](const Numbers& n) {
     known = n.v < b.pages;
@@ -321,12 +389,22 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
     ks = a.k_scale[at], vs = a.v_scale[at];
   };
 
+  // This lane's columns; past the last one, the last.  Their loads are before the tile's, behind whose numbers they need not wait.
+  // (No branches: where they meet again everything would be waited for.  A wavefront without a tile loads the last one.)
   uint32_t i = begin + wave;
-  Numbers next{0u, 0u};
-  if (i < end) {
-    const Numbers now = numbers(i);
-    if (i + NW < end) next = numbers(i + NW);
-    const uint8_t *from_k = keys_at(i, now), *from_v = values_at(i, now);
+  const uint32_t own = i < end ? i : end - 1u;
+  const Numbers now = numbers(own);
+  Numbers next = numbers(i + NW < end ? i + NW : own);
+  uint32_t pos[CG];
+  float q_scale[CG], raw[CG][DP / 64][16];
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const uint32_t at = cg * 16u + r, col = at < w.columns ? at : w.columns - 1u, row = col / a.group;
+    pos[cg] = past + row;
+    query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw[cg]);
+  }
+  {
+    const uint8_t *from_k = keys_at(own, now), *from_v = values_at(own, now);
     fetch_scales(now);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
@@ -336,16 +414,9 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
 #pragma unroll
     for (int x = 0; x < VL; ++x) fetch_values(from_v, x);
   }
-
-  // This lane's columns; past the last one, the last.  Each wavefront makes a share of the operands.
-  uint32_t pos[CG];
-  float q_scale[CG];
+  // Each wavefront makes a share of the operands.
 #pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const uint32_t at = cg * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
-    pos[cg] = past + row;
-    q_scale[cg] = query_terms<KIND, DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, sh.q[cg], wave, NW);
-  }
+  for (int cg = 0; cg < CG; ++cg) q_scale[cg] = query_terms<KIND, DP>(raw[cg], D, sh.q[cg], wave, NW);
   lds_barrier();
 
   Column col[CG];
@@ -488,8 +559,8 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
     for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * factor;
   }
   __syncthreads();
-  const bool whole = w.tiles <= a.part_tiles;                       // no other part has tiles
-  const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * C;
+  const bool whole = begin == 0u && end == w.tiles;                 // no other part has tiles
+  slot *= a.stored;
   for (uint32_t e = t; e < w.columns * (D / 4u); e += NW * 64u) {
     const uint32_t c = e / (D / 4u), d = e % (D / 4u) * 4u;
     float top = -INFINITY;
@@ -503,13 +574,15 @@ __global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void atte
       x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]);
     }
     if (whole) {
-      const uint32_t pair = w.first_col + c;
+      const uint32_t pair = c;
       float* to = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
       *reinterpret_cast<float4_t*>(to) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
     } else {
       *reinterpret_cast<float4_t*>(a.part_sum + (slot + c) * D + d) = x;
       if (d == 0u) a.part_most[slot + c] = top, a.part_total[slot + c] = total;
     }
+  }
+  lds_barrier();                                                    // the next run's queries go where these sums are
   }
 }
 
@@ -624,7 +697,9 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
   };
   {
     const uint32_t own = wave & 3u, at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
-    const float scale = query_terms<KIND, DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, sh.q[own], wave / 4u, WAVES / 4u);
+    float raw[DP / 64][16];
+    query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw);
+    const float scale = query_terms<KIND, DP>(raw, D, sh.q[own], wave / 4u, WAVES / 4u);
     if (g == 0u) sh.scale[own * 16u + r] = scale;
   }
   lds_barrier();
@@ -774,7 +849,7 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
   lds_barrier();
   if (half == 1u) return;
   const bool whole = w.tiles <= a.part_tiles;                       // no other part has tiles
-  const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * C;
+  const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * a.stored;
 #pragma unroll
   for (int cg = 0; cg < CG; ++cg) {
     const uint32_t c = (group * CG + cg) * 16u + r;
@@ -794,37 +869,62 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 
 // ---- the parts' merge ----------------------------------------------------------------------------
 
-// A workgroup a column: its parts' sums under the largest of their references, all loads under way at once.
-constexpr uint32_t kPagePartsMost = 256;
+// A workgroup a column: its parts' sums under the largest of their references, the first parts' loads under way at once.
+constexpr uint32_t kPagePartsMost = 1024;
 template <int C>
 __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttention a) {
   __shared__ float of_wave[2][4], weight[kPagePartsMost];
   __shared__ alignas(16) float4_t piece[256];
   const PageBatch& b = a.batch;
-  const uint32_t c = blockIdx.x % C, rest = blockIdx.x / C, kv = rest % b.kv_heads, unit = rest / b.kv_heads, t = threadIdx.x;
+  const uint32_t c = blockIdx.x % a.stored, rest = blockIdx.x / a.stored, kv = rest % b.kv_heads, unit = rest / b.kv_heads, t = threadIdx.x;
   PageUnit u;
-  if (!find_unit(b, unit, [&](const PageSequence& q) { return (q.rows * a.group + C - 1u) / C; }, &u)) return;
+  if (!find_unit(b, unit, [&](const PageSequence& q) { return C < 64 ? 1u : (q.rows * a.group + C - 1u) / C; }, &u)) return;
   if constexpr (C == 64) u.at = (u.seq.rows * a.group + C - 1u) / C - 1u - u.at;      // as the tiles' kernel has it
-  const UnitTiles w = unit_tiles(a, u, C);
-  if (c >= w.columns || w.tiles <= a.part_tiles) return;            // workgroup-uniform
-  const uint32_t parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles, D = b.head_dim, runs = D / 4u;
-  const uint64_t at = (static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts * C + c;
-  const float own = t < parts ? a.part_most[at + static_cast<uint64_t>(t) * C] : -INFINITY, sum = t < parts ? a.part_total[at + static_cast<uint64_t>(t) * C] : 0.0f;
+  const UnitTiles w = C < 64 ? sequence_tiles(a, u.seq) : unit_tiles(a, u, C);
+  if (c >= w.columns) return;                                       // workgroup-uniform, as the next ones
+  // Places of the parts: the first one's, then from `then` on, `step` apart.
+  uint64_t place, then, step;
+  uint32_t parts;
+  if (a.even != 0u) {
+    const EvenTiles tiles = even_tiles(a, u.s);
+    const uint32_t share = even_share(tiles.all, a.even, b), from = tiles.before * b.kv_heads + kv * (w.tiles + kBegin);
+    const uint32_t first = (from + kBegin) / share;
+    parts = (from + kBegin + w.tiles - 1u) / share - first + 1u;
+    place = 2u * static_cast<uint64_t>(first) + (first * share < from ? 1u : 0u), then = 2u * static_cast<uint64_t>(first + 1u), step = 2u;
+  } else {
+    parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles;
+    place = (static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts, then = place + 1u, step = 1u;
+  }
+  if (parts == 1u) return;
+  const uint32_t D = b.head_dim, runs = D / 4u;
+  auto column = [&](uint32_t p) { return (p == 0u ? place : then + (p - 1u) * step) * a.stored + c; };
   // 256 / runs threads a run of four elements; the first parts' sums are asked for before their weights are there
-  constexpr uint32_t AHEAD = 4;
+  constexpr uint32_t AHEAD = 4, OWN = kPagePartsMost / 256u;
+  float own[OWN], sum[OWN], most = -INFINITY;
+#pragma unroll
+  for (uint32_t i = 0; i < OWN; ++i) {
+    const uint32_t p = t + 256u * i;
+    own[i] = p < parts ? a.part_most[column(p)] : -INFINITY, sum[i] = p < parts ? a.part_total[column(p)] : 0.0f;
+    most = fmaxf(most, own[i]);
+  }
   const uint32_t lanes = 256u / runs, mine = t / runs, d = t % runs * 4u;
   float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f}, early[AHEAD];
-  auto load = [&](uint32_t p) { return p < parts && mine < lanes ? *reinterpret_cast<const float4_t*>(a.part_sum + (at + static_cast<uint64_t>(p) * C) * D + d) : x; };
+  auto load = [&](uint32_t p) { return p < parts && mine < lanes ? *reinterpret_cast<const float4_t*>(a.part_sum + column(p) * D + d) : x; };
 #pragma unroll
   for (uint32_t i = 0; i < AHEAD; ++i) early[i] = load(mine + i * lanes);
-  const float most = wave_max(own);
+  most = wave_max(most);
   if ((t & 63u) == 0u) of_wave[0][t >> 6] = most;
   __syncthreads();
   const float top = fmaxf(fmaxf(of_wave[0][0], of_wave[0][1]), fmaxf(of_wave[0][2], of_wave[0][3]));
-  const float f = t < parts ? __builtin_amdgcn_exp2f(own - from_reference(top)) : 0.0f;
-  weight[t] = f;
-  const float total_of = wave_sum(f * sum);
-  if ((t & 63u) == 0u) of_wave[1][t >> 6] = total_of;
+  float all = 0.0f;
+#pragma unroll
+  for (uint32_t i = 0; i < OWN; ++i) {
+    const float f = t + 256u * i < parts ? __builtin_amdgcn_exp2f(own[i] - from_reference(top)) : 0.0f;
+    weight[t + 256u * i] = f;
+    all = fmaf(f, sum[i], all);
+  }
+  all = wave_sum(all);
+  if ((t & 63u) == 0u) of_wave[1][t >> 6] = all;
   __syncthreads();
   const float total = (of_wave[1][0] + of_wave[1][1]) + (of_wave[1][2] + of_wave[1][3]);
 #pragma unroll
@@ -833,7 +933,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   }
 #pragma unroll 4
   for (uint32_t p = mine + AHEAD * lanes; p < parts; p += lanes) {
-    if (mine < lanes) x += *reinterpret_cast<const float4_t*>(a.part_sum + (at + static_cast<uint64_t>(p) * C) * D + d) * weight[p];
+    if (mine < lanes) x += *reinterpret_cast<const float4_t*>(a.part_sum + column(p) * D + d) * weight[p];
   }
   piece[t] = x;
   __syncthreads();
@@ -860,25 +960,42 @@ static uint64_t tiles_of(const PageAttentionCall& c) {
   return some < all ? some : all;
 }
 
-size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape& shape) {
-  if (shape.parts < 2) return 0;
-  return static_cast<size_t>(units_of(c, shape.columns) * c.page.kv_heads * shape.parts * shape.columns * (c.page.head_dim + 2) * 4);
+// Columns of a unit that can be there.
+static uint64_t stored_of(const PageAttentionCall& c, uint64_t columns) {
+  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads);
+  return pairs < columns ? pairs : columns;
 }
 
-PagesShape attention_pages_shape(const PageAttentionCall& c, uint64_t most_parts) {
+size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape& shape) {
+  const uint64_t places = shape.even != 0 ? 2 * shape.even : shape.parts < 2 ? 0 : units_of(c, shape.columns) * c.page.kv_heads * shape.parts;
+  return static_cast<size_t>(places * stored_of(c, shape.columns) * (c.page.head_dim + 2) * 4);
+}
+
+// Workgroups of few_kernel on a CU at once, by their registers.
+static uint64_t few_resident(uint64_t head_dim, uint64_t columns) {
+  return head_dim <= 64 || (head_dim <= 128 && columns == 16) ? 2 : 1;
+}
+
+PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
   const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && c.page.head_dim <= 128 ? 32 : 64;
-  PagesShape shape{columns, 1, tiles_of(c)};
-  const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads, cus = static_cast<uint64_t>(num_cus());
-  uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
-  if (parts > most_parts) parts = most_parts;
-  if (parts > (shape.part_tiles + 3) / 4) parts = (shape.part_tiles + 3) / 4;
-  while (parts > 1) {
-    const uint64_t tiles = (tiles_of(c) + parts - 1) / parts;
-    shape.parts = (tiles_of(c) + tiles - 1) / tiles, shape.part_tiles = tiles;
-    if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
-    --parts;
+  const uint64_t tiles = tiles_of(c), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
+  const PagesShape one{columns, 1, tiles, 0};
+  if (!in_parts) return one;
+  if (columns < 64) {
+    const uint64_t resident = few_resident(c.page.head_dim, columns) * cus, parts = (tiles + 3) / 4;
+    const PagesShape each{columns, parts, 4, 0}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost};
+    if (groups * parts <= resident && parts <= kPagePartsMost) return parts > 1 && attention_pages_parts_bytes(c, each) <= kAttentionPartsMost ? each : one;
+    return c.page.sequences * c.page.kv_heads * (tiles + kBegin) < (1u << 30) && attention_pages_parts_bytes(c, even) <= kAttentionPartsMost ? even : one;
   }
-  return PagesShape{columns, 1, tiles_of(c)};
+  uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
+  if (parts > 256) parts = 256;
+  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+  for (; parts > 1; --parts) {
+    const uint64_t each = (tiles + parts - 1) / parts;
+    const PagesShape shape{columns, (tiles + each - 1) / each, each, 0};
+    if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
+  }
+  return one;
 }
 
 hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
@@ -893,9 +1010,12 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   a.window = c.window >= c.max_len ? 0u : static_cast<uint32_t>(c.window);
   a.sinks = static_cast<uint32_t>(c.sinks < c.max_len ? c.sinks : c.max_len);
   a.parts = static_cast<uint32_t>(shape.parts), a.part_tiles = static_cast<uint32_t>(shape.part_tiles);
+  a.stored = static_cast<uint32_t>(stored_of(c, shape.columns));
   const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads;
-  if (shape.parts > 1) {
-    const uint64_t columns = groups * shape.parts * shape.columns;
+  a.even = static_cast<uint32_t>(shape.even);
+  const bool split = shape.parts > 1 || shape.even != 0;
+  if (split) {
+    const uint64_t columns = (shape.even != 0 ? 2 * shape.even : groups * shape.parts) * a.stored;
     a.part_sum = static_cast<float*>(scratch);
     a.part_most = a.part_sum + columns * c.page.head_dim;
     a.part_total = a.part_most + columns;
@@ -907,7 +1027,7 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   };
   auto few = [&](auto kind, auto dim, auto cg) {
     hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, decltype(cg)::value, 4>),
-                       dim3(static_cast<uint32_t>(groups * shape.parts)), dim3(256), 0, stream, a);
+                       dim3(static_cast<uint32_t>(shape.even != 0 ? shape.even : groups * shape.parts)), dim3(256), 0, stream, a);
   };
   auto with_columns = [&](auto kind, auto dim) {
     if (shape.columns == 64) return tile(kind, dim);
@@ -923,8 +1043,8 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   };
   fp8 ? with_dim(std::integral_constant<PageKind, PageKind::Fp8>{}) : with_dim(std::integral_constant<PageKind, PageKind::Q8>{});
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || shape.parts < 2) return e;
-  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups * shape.columns)), dim3(256), 0, stream, a); };
+  if (e != hipSuccess || !split) return e;
+  auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups * a.stored)), dim3(256), 0, stream, a); };
   shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : shape.columns == 32 ? merge(attention_pages_merge_kernel<32>) : merge(attention_pages_merge_kernel<64>);
   return hipGetLastError();
 }

@@ -8,6 +8,8 @@
 // Starts[s + 1] - 1 are the last; its page j is Table[s * width + j].
 #pragma once
 
+#include <type_traits>
+
 #include "page_args.hpp"
 #include "qmm_device.hpp"
 
@@ -37,6 +39,18 @@ __device__ __forceinline__ PageSequence page_sequence(const PageBatch& b, uint32
   return PageSequence{first, holds ? end - first : 0u, len};
 }
 
+// Sums over the lanes up to this one (of a wavefront whose lanes are all there): in rows of sixteen, then from row to row.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  auto add = [&](auto ctrl, auto rows) { v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), ctrl.value, rows.value, 0xF, false)); };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});     // a row's last to the next row
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});     // the second row's last to the upper two
+  return v;
+}
+
 // The unit `unit` of the batch, `of(sequence)` to each: its sequence and its place among that one's.  All lanes of a wavefront
 // call it alike; false: there are fewer units.
 struct PageUnit {
@@ -51,12 +65,7 @@ __device__ __forceinline__ bool find_unit(const PageBatch& b, uint32_t unit, Of 
     PageSequence seq{0u, 0u, 0u};
     if (s < b.sequences) seq = page_sequence(b, s);
     const uint32_t own = seq.rows == 0u ? 0u : of(seq);
-    uint32_t sum = own;
-#pragma unroll
-    for (uint32_t off = 1u; off < 64u; off <<= 1) {
-      const uint32_t before = __shfl_up(sum, off, kWave);
-      if (lane >= off) sum += before;
-    }
+    const uint32_t sum = wave_scan(own);
     const uint32_t all = __builtin_amdgcn_readlane(sum, 63);
     if (unit < all) {
       const int hit = __ffsll(static_cast<unsigned long long>(__ballot(sum > unit))) - 1;

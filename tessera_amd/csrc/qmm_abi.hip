@@ -1554,12 +1554,12 @@ qmm_status run_attention_pages(const LaunchCtx& c, bool fp8) {
                                                c.ptr<const float>(3), c.ptr<const float>(4), c.ptr<const uint32_t>(5), c.ptr<const uint32_t>(6),
                                                c.ptr<const uint32_t>(7), c.ptr<float>(8), scratch, c.stream));
   };
-  const qmm::PagesShape in_parts = qmm::attention_pages_shape(call, 256);
-  if (in_parts.parts > 1) {
+  const qmm::PagesShape in_parts = qmm::attention_pages_shape(call, true);
+  if (in_parts.parts > 1 || in_parts.even != 0) {
     const StreamBlock block(c, qmm::attention_pages_parts_bytes(call, in_parts), g_parts_scratch);
     if (block.get() != nullptr) return go(in_parts, block.get());
   }
-  return go(qmm::attention_pages_shape(call, 1), nullptr);
+  return go(qmm::attention_pages_shape(call, false), nullptr);
 }
 qmm_status run_attention_pages_q8(const LaunchCtx& c) { return run_attention_pages(c, false); }
 qmm_status run_attention_pages_fp8(const LaunchCtx& c) { return run_attention_pages(c, true); }

@@ -291,7 +291,7 @@ hipError_t launch_pages_write(bool fp8, const PageWriteCall& call, const float* 
                               const uint32_t* lens, uint8_t* kp, uint8_t* vp, float* ks, float* vs, hipStream_t stream);
 hipError_t launch_pages_read(bool fp8, const PageReadCall& call, const uint8_t* kp, const uint8_t* vp, const float* ks, const float* vs,
                              const uint32_t* table, const uint32_t* starts, const uint32_t* lens, void* k, void* v, hipStream_t stream);
-PagesShape attention_pages_shape(const PageAttentionCall& call, uint64_t most_parts);
+PagesShape attention_pages_shape(const PageAttentionCall& call, bool in_parts);
 size_t attention_pages_parts_bytes(const PageAttentionCall& call, const PagesShape& shape);
 hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& call, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
                                   const float* ks, const float* vs, const uint32_t* table, const uint32_t* starts, const uint32_t* lens, float* out,
