@@ -307,11 +307,11 @@ __device__ __forceinline__ float query_terms(const float (&raw)[DP / 64][16], ui
 
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
-template <PageKind KIND, int DP, int CG, int NW>
-constexpr int few_waves() { return DP * CG <= 128 ? 2 : 1; }   // a SIMD, by the registers
+template <int DP, int CG>
+constexpr int few_waves() { return DP * CG <= 128 ? 2 : 1; }        // a SIMD, by the registers
 
 template <PageKind KIND, int DP, int CG, int NW>
-__global__ __launch_bounds__(NW * 64, (few_waves<KIND, DP, CG, NW>())) void attention_pages_few_kernel(PageAttention a) {
+__global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_pages_few_kernel(PageAttention a) {
   constexpr int KL = DP / 64, VL = DP / 16, C = 16 * CG;
   __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
@@ -976,15 +976,23 @@ static uint64_t few_resident(uint64_t head_dim, uint64_t columns) {
   return head_dim <= 64 || (head_dim <= 128 && columns == 16) ? 2 : 1;
 }
 
+// Few columns: one workgroup a head of a sequence, parts of four tiles each where all of them are on the chip at once, or an even split.
+// A split costs the merge and its launch, and each run its start.  us, one workgroup / split: one sequence, 4 heads of 64, 500 positions
+// 7.6 / 11.4, 1500 11.3 / 11.5, 3000 17 / 11.5; 8 heads of 128, 500 10.4 / 12.7, 1000 13.3 / 12.4; 4 heads of 256, 500 15.2 / 16.0, 1000
+// 22 / 16; batches of all lengths up to the stated one, 40 sequences of 8 heads of 128, 1000 20 / 26, 2000 29 / 31, 3000 50 / 40, 128 of
+// them 4000 117 / 126, 48 of 4 heads of 256, 1000 24 / 32, 2000 43 / 39, 8000 124 / 91.
+// Many columns: parts only where the units are fewer than two a CU.
 PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
-  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && c.page.head_dim <= 128 ? 32 : 64;
+  const uint64_t D = c.page.head_dim, pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && D <= 128 ? 32 : 64;
   const uint64_t tiles = tiles_of(c), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
-  const PagesShape one{columns, 1, tiles, 0};
+  const uint64_t resident = few_resident(D, columns) * cus;
+  const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus && resident > cus ? 8u : 4u};
   if (!in_parts) return one;
   if (columns < 64) {
-    const uint64_t resident = few_resident(c.page.head_dim, columns) * cus, parts = (tiles + 3) / 4;
-    const PagesShape each{columns, parts, 4, 0}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost};
-    if (groups * parts <= resident && parts <= kPagePartsMost) return parts > 1 && attention_pages_parts_bytes(c, each) <= kAttentionPartsMost ? each : one;
+    const uint64_t parts = (tiles + 3) / 4;
+    const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost, 4};
+    if (tiles <= (D <= 128 ? 32 : 16) * groups / resident || (groups <= cus && tiles <= (D <= 64 ? 24 : 8))) return one;
+    if (groups * parts <= resident && parts <= kPagePartsMost) return attention_pages_parts_bytes(c, each) <= kAttentionPartsMost ? each : one;
     return c.page.sequences * c.page.kv_heads * (tiles + kBegin) < (1u << 30) && attention_pages_parts_bytes(c, even) <= kAttentionPartsMost ? even : one;
   }
   uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
@@ -992,7 +1000,7 @@ PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
   if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
   for (; parts > 1; --parts) {
     const uint64_t each = (tiles + parts - 1) / parts;
-    const PagesShape shape{columns, (tiles + each - 1) / each, each, 0};
+    const PagesShape shape{columns, (tiles + each - 1) / each, each, 0, 4};
     if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
   }
   return one;
@@ -1026,8 +1034,15 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
                        dim3(512 / CG), 0, stream, a);
   };
   auto few = [&](auto kind, auto dim, auto cg) {
-    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, decltype(dim)::value, decltype(cg)::value, 4>),
-                       dim3(static_cast<uint32_t>(shape.even != 0 ? shape.even : groups * shape.parts)), dim3(256), 0, stream, a);
+    constexpr int DP = decltype(dim)::value, CG = decltype(cg)::value;
+    const dim3 grid(static_cast<uint32_t>(shape.even != 0 ? shape.even : groups * shape.parts));
+    if constexpr (few_waves<DP, CG>() == 2) {
+      if (shape.waves == 8) {
+        hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 8>), grid, dim3(512), 0, stream, a);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 4>), grid, dim3(256), 0, stream, a);
   };
   auto with_columns = [&](auto kind, auto dim) {
     if (shape.columns == 64) return tile(kind, dim);

@@ -332,6 +332,7 @@ constexpr LogprobPlan logprob_plan(uint64_t rows, uint64_t vocab, uint64_t top_k
 struct PagesShape {
   uint64_t columns, parts, part_tiles;                        // (row, head) pairs a workgroup; parts of the positions, tiles of 64 each
   uint64_t even;                                              // workgroups that share all tiles evenly; 0: a workgroup a part
+  uint64_t waves;                                             // wavefronts a workgroup, where columns are few
 };
 
 // ---- "attention_combine" ---------------------------------------------------------------------------------------------

@@ -82,6 +82,26 @@ def test_long(backend, fmt, d, group, rows, past):
     check(b, q, [rows, rows], group, 4096, 100)
 
 
+@pytest.mark.parametrize("fmt,d,kv,group,most_rows,sequences,most", [("q8", 64, 2, 4, 1, 70, 2600), ("fp8", 128, 4, 4, 5, 66, 3000), ("q8", 256, 2, 6, 2, 40, 1800),
+                                                                     ("fp8", 80, 1, 16, 1, 90, 3500)])
+def test_many_sequences_of_all_lengths(backend, fmt, d, kv, group, most_rows, sequences, most):
+    """More tiles than the chip takes at once, of sequences of one position to many, some without rows, one that does not hold."""
+    rs = np.random.RandomState(sequences)
+    rows = rs.randint(0, most_rows + 1, sequences) if most_rows > 1 else (rs.rand(sequences) < 0.9).astype(int)
+    lens = np.maximum(rs.randint(1, most, sequences), rows)
+    lens[3], lens[4], lens[-1], rows[3], rows[-1] = rows[4] or 1, most, most, most_rows, most_rows
+    rows[7], lens[7] = most_rows, most_rows - 1             # more rows than positions
+    b = Batch(backend, 59, fmt, kv, 32, d, [int(n) for n in np.maximum(lens, 1)])
+    b.lens[7] = most_rows - 1
+    b.upload()
+    q = queries(b.rs, int(rows.sum()), kv * group * d)
+    holds = [s for s in range(sequences) if s != 7]
+    for window, sinks in ((0, 0), (700, 5)):
+        got = check(b, q, [int(n) for n in rows], group, window, sinks, only=holds, max_rows=most_rows)
+        at = int(rows[:7].sum())
+        assert np.all(got[at:at + rows[7]] == 7.0)
+
+
 def test_rows_behind_the_last_and_what_does_not_hold(backend):
     """Rows of no sequence stay as they were; so do those of sequences that do not hold, or exceed what the launch was made for."""
     kv, group, d, block = 2, 3, 64, 16
