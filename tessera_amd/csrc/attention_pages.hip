@@ -30,7 +30,7 @@ struct PageAttention {
   float* out;
   float *part_sum, *part_most, *part_total;   // (unit, key head, part, one of `stored` columns): head_dim sums; the reference in powers of two; the weights' sum
   uint32_t heads, group, window, sinks;       // window 0: every position
-  uint32_t parts, part_tiles, stored, even;   // tiles of 64 positions a part; columns of a unit that a part has room for; workgroups of an even split, or 0
+  uint32_t log_tile, parts, part_tiles, stored, even;   // positions a tile; tiles a part; columns of a unit that a part has room for; workgroups of an even split, or 0
 };
 
 // ---- which positions a unit walks ----------------------------------------------------------------
@@ -48,9 +48,9 @@ __device__ __forceinline__ UnitTiles tiles_between(const PageAttention& a, uint3
   w.low = low, w.high = high;
   const uint32_t begin = a.window != 0u && w.low + 1u > a.window ? w.low + 1u - a.window : 0u;
   const uint32_t sinks = a.sinks < begin ? a.sinks : begin;
-  w.sink_tiles = (sinks + 63u) / 64u;
-  w.from_tile = begin / 64u > w.sink_tiles ? begin / 64u : w.sink_tiles;
-  w.tiles = w.sink_tiles + (w.high / 64u + 1u - w.from_tile);
+  w.sink_tiles = (sinks + (1u << a.log_tile) - 1u) >> a.log_tile;
+  w.from_tile = begin >> a.log_tile > w.sink_tiles ? begin >> a.log_tile : w.sink_tiles;
+  w.tiles = w.sink_tiles + ((w.high >> a.log_tile) + 1u - w.from_tile);
   return w;
 }
 // The one unit of a sequence whose pairs all fit.
@@ -191,9 +191,10 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
 // To begin a head costs what kBegin tiles do: so many lie before its first, with nothing in them.  A run that covers a head whole gives
 // its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second those of
 // a later one.
-constexpr uint32_t kBegin = 6;
+constexpr uint32_t kBegin = 6;                                      // of 64 positions
+__host__ __device__ constexpr uint32_t begin_tiles(uint32_t log_tile) { return kBegin << (6u - log_tile); }
 __device__ __forceinline__ uint32_t even_of(const PageAttention& a, const PageSequence& seq) {
-  return seq.rows == 0u ? 0u : sequence_tiles(a, seq).tiles + kBegin;
+  return seq.rows == 0u ? 0u : sequence_tiles(a, seq).tiles + begin_tiles(a.log_tile);
 }
 struct EvenTiles {
   uint32_t before, all;           // of a head of the sequences before the s-th; of all
@@ -207,9 +208,9 @@ __device__ __forceinline__ EvenTiles even_tiles(const PageAttention& a, uint32_t
   auto last = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan(v)), 63)); };
   return EvenTiles{last(before), last(all)};
 }
-__device__ __forceinline__ uint32_t even_share(uint32_t all, uint32_t workgroups, const PageBatch& b) {
-  const uint32_t share = (all * b.kv_heads + workgroups - 1u) / workgroups;
-  return all != 0u && share < kBegin + 4u ? kBegin + 4u : share;    // (a tile a wavefront)
+__device__ __forceinline__ uint32_t even_share(const PageAttention& a, uint32_t all) {
+  const uint32_t share = (all * a.batch.kv_heads + a.even - 1u) / a.even, least = begin_tiles(a.log_tile) + 4u;
+  return all != 0u && share < least ? least : share;    // (a tile a wavefront)
 }
 
 // ---- few columns ---------------------------------------------------------------------------------
@@ -220,6 +221,8 @@ __device__ __forceinline__ uint32_t even_share(uint32_t all, uint32_t workgroups
 // in one page: one scale a lane), and those are the sixteen of the value operands that it loads: no score changes its lane.  A
 // register that an operand was made from takes the next tile's at once, so that a tile's loads have a whole tile's time.  The queries'
 // operands lie in LDS, one copy for all wavefronts.
+// Positions of a tile: 64, or 32 where a tile's codes and the sums together are more registers than two wavefronts a SIMD have.
+constexpr uint32_t few_tile(int elements) { return elements <= 128 ? 64 : 32; }
 constexpr int query_operands(PageKind kind, int dp) { return kind == PageKind::Q8 ? 3 * (dp / 64) : 2 * (dp / 32); }
 
 template <PageKind KIND, int DP, int CG, int NW>
@@ -307,19 +310,19 @@ __device__ __forceinline__ float query_terms(const float (&raw)[DP / 64][16], ui
 
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
-template <int DP, int CG>
-constexpr int few_waves() { return DP * CG <= 128 ? 2 : 1; }        // a SIMD, by the registers
 
 template <PageKind KIND, int DP, int CG, int NW>
-__global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_pages_few_kernel(PageAttention a) {
+__global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAttention a) {
   constexpr int KL = DP / 64, VL = DP / 16, C = 16 * CG;
+  constexpr uint32_t TILE = few_tile(DP * CG), OWN = TILE / 4;      // positions of a tile, and of a lane's
+  constexpr int NT = TILE / 16;                                     // key operands
   __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
   const uint32_t D = b.head_dim, block = 1u << b.log_block;
   uint32_t at_tile = 0u, last_tile = 0u;
   if (a.even != 0u) {
-    const uint32_t share = even_share(even_tiles(a, 0u).all, gridDim.x, b);
+    const uint32_t share = even_share(a, even_tiles(a, 0u).all);
     at_tile = blockIdx.x * share, last_tile = at_tile + share;
   }
   for (bool first_run = true;; first_run = false) {
@@ -331,10 +334,11 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
     if (at_tile >= last_tile || !find_unit(b, at_tile, [&](const PageSequence& q) { return even_of(a, q) * b.kv_heads; }, &u)) return;
     const uint32_t in = u.at;
     w = sequence_tiles(a, u.seq);
-    const uint32_t from = in % (w.tiles + kBegin), left = last_tile - at_tile, to = w.tiles + kBegin - from < left ? w.tiles + kBegin : from + left;
-    kv = in / (w.tiles + kBegin);
-    if (to <= kBegin) return;                                       // (the next workgroup begins it)
-    begin = from > kBegin ? from - kBegin : 0u, end = to - kBegin;
+    constexpr uint32_t EMPTY = kBegin * (64u / TILE);
+    const uint32_t wide = w.tiles + EMPTY, from = in % wide, left = last_tile - at_tile, to = wide - from < left ? wide : from + left;
+    kv = in / wide;
+    if (to <= EMPTY) return;                                       // (the next workgroup begins it)
+    begin = from > EMPTY ? from - EMPTY : 0u, end = to - EMPTY;
     slot = 2u * static_cast<uint64_t>(blockIdx.x) + (first_run ? 0u : 1u);
     at_tile += to - from;
   } else {
@@ -348,7 +352,7 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
   }
   const uint32_t past = u.seq.len - u.seq.rows;
 
-  // Page numbers of a tile's sixteen positions r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
+  // Page numbers of a tile's quarters r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
   const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
   const uint32_t last_slot = (u.seq.len - 1u) >> b.log_block;
   auto slot_of = [&](uint32_t position) {
@@ -359,21 +363,22 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
     uint32_t k, v;
   };
   auto numbers = [&](uint32_t i) {
-    const uint32_t p0 = tile_at(w, i) * 64u;
-    return Numbers{table[slot_of(p0 + (r >> 2) * 16u)], table[slot_of(p0 + g * 16u)]};
+    const uint32_t p0 = tile_at(w, i) * TILE;
+    return Numbers{table[slot_of(p0 + (r >> 2) * OWN)], table[slot_of(p0 + g * OWN)]};
   };
-  uint4 kr[4][KL], vr[VL];
+  uint4 kr[NT][KL];
+  std::conditional_t<OWN == 16, uint4, uint2> vr[VL];
   float ks, vs;
   bool known;
   const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
   // Where a lane's runs of a tile begin.  (Elements past head_dim meet zeros of the queries, or are not stored.)
   const uint32_t past_end = 16u * g < D % 64u ? 0u : 16u * g - (D % 64u == 0u ? 0u : D % 64u - 16u);       // in a run of 64 that is not whole
   auto keys_at = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * 64u + (r >> 2) * 16u) & (block - 1u);
+    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * TILE + (r >> 2) * OWN) & (block - 1u);
     return a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D + 16u * g;
   };
   auto values_at = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * 64u + g * 16u) & (block - 1u);
+    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * TILE + g * OWN) & (block - 1u);
     return a.v + page * page_bytes + (kv * D + r) * block + at;
   };
   auto fetch_keys = [&](const uint8_t* from, int y, int x) {
@@ -381,7 +386,9 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
     kr[y][x] = load_u4(at + (4u * y * D + (64u * x < D ? 64u * x : 0u)));
   };
   auto fetch_values = [&](const uint8_t* from, int x) {
-    vr[x] = load_u4(from + (16u * x < D ? 16u * x * block : 0u));   // (uniform: no register of its own)
+    const uint8_t* at = from + (16u * x < D ? 16u * x * block : 0u);   // (uniform: no register of its own)
+    if constexpr (OWN == 16) vr[x] = load_u4(at);
+    else vr[x] = *reinterpret_cast<const uint2*>(at);
   };
   auto fetch_scales = [&](const Numbers& n) {
     known = n.v < b.pages;
@@ -407,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
     const uint8_t *from_k = keys_at(own, now), *from_v = values_at(own, now);
     fetch_scales(now);
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < NT; ++y) {
 #pragma unroll
       for (int x = 0; x < KL; ++x) fetch_keys(from_k, y, x);
     }
@@ -428,16 +435,18 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
   }
   auto tile = [&](auto last) {
     constexpr bool MORE = !decltype(last)::value;
-    const uint32_t first = tile_at(w, i) * 64u;
+    const uint32_t first = tile_at(w, i) * TILE;
     const float k_scale = ks, v_scale = vs;
     const bool in_pool = known;
     const uint8_t *from_k = nullptr, *from_v = nullptr;
     if constexpr (MORE) from_k = keys_at(i + NW, next), from_v = values_at(i + NW, next);
-    float4_t acc[CG][4];
+    float4_t acc[CG][NT];
     if constexpr (KIND == PageKind::Q8) {
-      constexpr int YB = 2;                                         // key operands that share a query operand's way from LDS
+      constexpr int YB = DP * CG == 256 && CG == 2 ? 1 : 2;            // key operands that share a query operand's way from LDS
 #pragma unroll
-      for (int y0 = 0; y0 < 4; y0 += YB) {
+      for (int y0 = 0; y0 < NT; y0 += YB) {
+        uint32_t from = lane;
+        if constexpr (YB == 1) asm volatile("" : "+v"(from));         // (the queries are read once more, not held)
         int4_t sum[CG][YB][3];
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg) {
@@ -450,7 +459,7 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
           for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
             for (int n = 0; n < 3; ++n) {
-              const int4_t q = bit_cast<int4_t>(sh.q[cg][3 * x + n][lane]);
+              const int4_t q = bit_cast<int4_t>(sh.q[cg][3 * x + n][from]);
 #pragma unroll
               for (int y = 0; y < YB; ++y) {
                 sum[cg][y][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bit_cast<int4_t>(kr[y0 + y][x]), q, sum[cg][y][n], 0, 0, 0);
@@ -479,7 +488,7 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-        for (int y = 0; y < 4; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int y = 0; y < NT; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
       }
 #pragma unroll
       for (int x = 0; x < 2 * KL; ++x) {
@@ -487,7 +496,7 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg) hi[cg] = bit_cast<half8_t>(sh.q[cg][2 * x][lane]), lo[cg] = bit_cast<half8_t>(sh.q[cg][2 * x + 1][lane]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
+        for (int y = 0; y < NT; ++y) {
           const uint4 run = kr[y][x / 2];
           const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
 #pragma unroll
@@ -506,35 +515,37 @@ __global__ __launch_bounds__(NW * 64, (few_waves<DP, CG>())) void attention_page
       if (i + 2 * NW < end) next = numbers(i + 2 * NW);
     }
     // Every column sees every position of the tile, or it goes by bits.
-    const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
-    half8_t p_hi[CG][2], p_lo[CG][2];
+    const bool all = first + (TILE - 1u) <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
+    half8_t p_hi[CG][OWN / 8], p_lo[CG][OWN / 8];
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
-      float s[16], corr;
+      float s[OWN], corr;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = acc[cg][e / 4][e % 4];
-      uint32_t shown = 0xFFFFu;
+      for (uint32_t e = 0; e < OWN; ++e) s[e] = acc[cg][e / 4][e % 4];
+      uint32_t shown = (1u << OWN) - 1u;
       if (!all) {
-        const uint32_t p0 = first + 16u * g;
+        const uint32_t p0 = first + OWN * g;
         shown = 0u;
 #pragma unroll
-        for (uint32_t e = 0; e < 16u; ++e) {
+        for (uint32_t e = 0; e < OWN; ++e) {
           const uint32_t p = p0 + e;
           const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & in_pool;
           shown |= (sees ? 1u : 0u) << e;
         }
       }
-      if (weigh<16>(col[cg], s, q_scale[cg] * k_scale, shown, all, v_scale, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
+      if (weigh<static_cast<int>(OWN)>(col[cg], s, q_scale[cg] * k_scale, shown, all, v_scale, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
     }
 #pragma unroll
     for (int x = 0; x < VL; ++x) {
-      const half8_t v0 = operand<KIND>(vr[x].x, vr[x].y), v1 = operand<KIND>(vr[x].z, vr[x].w);
+      half8_t value[OWN / 8];
+      value[0] = operand<KIND>(vr[x].x, vr[x].y);
+      if constexpr (OWN == 16) value[1] = operand<KIND>(vr[x].z, vr[x].w);
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
-        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p_lo[cg][0], o[cg][x], 0, 0, 0);
-        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p_lo[cg][1], o[cg][x], 0, 0, 0);
-        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p_hi[cg][0], o[cg][x], 0, 0, 0);
-        o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p_hi[cg][1], o[cg][x], 0, 0, 0);
+#pragma unroll
+        for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_lo[cg][n], o[cg][x], 0, 0, 0);
+#pragma unroll
+        for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_hi[cg][n], o[cg][x], 0, 0, 0);
       }
       if constexpr (MORE) fetch_values(from_v, x);
     }
@@ -887,9 +898,9 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   uint32_t parts;
   if (a.even != 0u) {
     const EvenTiles tiles = even_tiles(a, u.s);
-    const uint32_t share = even_share(tiles.all, a.even, b), from = tiles.before * b.kv_heads + kv * (w.tiles + kBegin);
-    const uint32_t first = (from + kBegin) / share;
-    parts = (from + kBegin + w.tiles - 1u) / share - first + 1u;
+    const uint32_t share = even_share(a, tiles.all), empty = begin_tiles(a.log_tile), from = tiles.before * b.kv_heads + kv * (w.tiles + empty);
+    const uint32_t first = (from + empty) / share;
+    parts = (from + empty + w.tiles - 1u) / share - first + 1u;
     place = 2u * static_cast<uint64_t>(first) + (first * share < from ? 1u : 0u), then = 2u * static_cast<uint64_t>(first + 1u), step = 2u;
   } else {
     parts = (w.tiles + a.part_tiles - 1u) / a.part_tiles;
@@ -899,7 +910,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   const uint32_t D = b.head_dim, runs = D / 4u;
   auto column = [&](uint32_t p) { return (p == 0u ? place : then + (p - 1u) * step) * a.stored + c; };
   // 256 / runs threads a run of four elements; the first parts' sums are asked for before their weights are there
-  constexpr uint32_t AHEAD = 4, OWN = kPagePartsMost / 256u;
+  constexpr uint32_t AHEAD = 8, OWN = kPagePartsMost / 256u;
   float own[OWN], sum[OWN], most = -INFINITY;
 #pragma unroll
   for (uint32_t i = 0; i < OWN; ++i) {
@@ -952,11 +963,15 @@ uint64_t units_of(const PageAttentionCall& c, uint64_t columns) {
 
 }  // namespace
 
-// Tiles that a unit walks, at most.
-static uint64_t tiles_of(const PageAttentionCall& c) {
-  const uint64_t all = (c.max_len + 63) / 64;
+// Positions of a tile, and tiles that a unit walks at most.
+static uint32_t log_tile_of(const PageAttentionCall& c, uint64_t columns) {
+  const uint64_t D = c.page.head_dim, padded = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+  return columns < 64 && few_tile(static_cast<int>(padded * columns / 16)) == 32 ? 5u : 6u;
+}
+static uint64_t tiles_of(const PageAttentionCall& c, uint64_t columns) {
+  const uint64_t tile = uint64_t{1} << log_tile_of(c, columns), all = (c.max_len + tile - 1) / tile;
   if (c.window == 0) return all;
-  const uint64_t some = (c.sinks + 63) / 64 + (c.window + c.max_rows + 63) / 64 + 1;
+  const uint64_t some = (c.sinks + tile - 1) / tile + (c.window + c.max_rows + tile - 1) / tile + 1;
   return some < all ? some : all;
 }
 
@@ -971,29 +986,27 @@ size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape&
   return static_cast<size_t>(places * stored_of(c, shape.columns) * (c.page.head_dim + 2) * 4);
 }
 
-// Workgroups of few_kernel on a CU at once, by their registers.
-static uint64_t few_resident(uint64_t head_dim, uint64_t columns) {
-  return head_dim <= 64 || (head_dim <= 128 && columns == 16) ? 2 : 1;
-}
-
-// Few columns: one workgroup a head of a sequence, parts of four tiles each where all of them are on the chip at once, or an even split.
-// A split costs the merge and its launch, and each run its start.  us, one workgroup / split: one sequence, 4 heads of 64, 500 positions
-// 7.6 / 11.4, 1500 11.3 / 11.5, 3000 17 / 11.5; 8 heads of 128, 500 10.4 / 12.7, 1000 13.3 / 12.4; 4 heads of 256, 500 15.2 / 16.0, 1000
-// 22 / 16; batches of all lengths up to the stated one, 40 sequences of 8 heads of 128, 1000 20 / 26, 2000 29 / 31, 3000 50 / 40, 128 of
-// them 4000 117 / 126, 48 of 4 heads of 256, 1000 24 / 32, 2000 43 / 39, 8000 124 / 91.
+// Few columns: one workgroup a head of a sequence, or parts of four tiles where all of those are on the chip at once, or an even split.
+// A split costs the merge and its launch, each of its runs a start; one workgroup has the longest sequence's time.  us, one
+// workgroup / parts: a sequence of 4 heads of 64, 500 positions 7.3 / 11.3, 1500 11.0 / 11.4, 2000 13 / 12; 8 heads of 128, 400 10.4 / 13.2,
+// 1000 13.7 / 13.2; 4 heads of 256, 250 11.8 / 14.0, 500 14.9 / 14.0.  One / even split, sequences of all lengths up to the stated one: 40
+// of 8 heads of 128, 2000 29 / 32, 3000 51 / 41, 128 of them, 3000 92 / 99, 5000 142 / 141, 8000 215 / 205; 48 of 4 heads of 256, 1500
+// 27 / 31, 3000 52 / 46, 8000 124 / 88, 200 of them, 3000 147 / 151, 5000 225 / 211.
 // Many columns: parts only where the units are fewer than two a CU.
 PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
   const uint64_t D = c.page.head_dim, pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && D <= 128 ? 32 : 64;
-  const uint64_t tiles = tiles_of(c), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
-  const uint64_t resident = few_resident(D, columns) * cus;
-  const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus && resident > cus ? 8u : 4u};
+  const uint64_t tiles = tiles_of(c, columns), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
+  const uint64_t resident = 2 * cus, log_tile = log_tile_of(c, columns);
+  const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus ? 8u : 4u};
   if (!in_parts) return one;
   if (columns < 64) {
-    const uint64_t parts = (tiles + 3) / 4;
+    const uint64_t parts = (tiles + 3) / 4, of_64 = tiles >> (6 - log_tile);
     const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost, 4};
-    if (tiles <= (D <= 128 ? 32 : 16) * groups / resident || (groups <= cus && tiles <= (D <= 64 ? 24 : 8))) return one;
-    if (groups * parts <= resident && parts <= kPagePartsMost) return attention_pages_parts_bytes(c, each) <= kAttentionPartsMost ? each : one;
-    return c.page.sequences * c.page.kv_heads * (tiles + kBegin) < (1u << 30) && attention_pages_parts_bytes(c, even) <= kAttentionPartsMost ? even : one;
+    if (groups * parts <= resident) {
+      return parts < 2 || of_64 <= (D <= 64 ? 24 : D <= 128 ? 12 : 6) || attention_pages_parts_bytes(c, each) > kAttentionPartsMost ? one : each;
+    }
+    if (of_64 <= 32 || of_64 <= 38 * groups / resident) return one;
+    return c.page.sequences * c.page.kv_heads * (tiles + begin_tiles(5)) < (1u << 30) && attention_pages_parts_bytes(c, even) <= kAttentionPartsMost ? even : one;
   }
   uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
   if (parts > 256) parts = 256;
@@ -1018,7 +1031,7 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   a.window = c.window >= c.max_len ? 0u : static_cast<uint32_t>(c.window);
   a.sinks = static_cast<uint32_t>(c.sinks < c.max_len ? c.sinks : c.max_len);
   a.parts = static_cast<uint32_t>(shape.parts), a.part_tiles = static_cast<uint32_t>(shape.part_tiles);
-  a.stored = static_cast<uint32_t>(stored_of(c, shape.columns));
+  a.stored = static_cast<uint32_t>(stored_of(c, shape.columns)), a.log_tile = log_tile_of(c, shape.columns);
   const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads;
   a.even = static_cast<uint32_t>(shape.even);
   const bool split = shape.parts > 1 || shape.even != 0;
@@ -1036,13 +1049,8 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   auto few = [&](auto kind, auto dim, auto cg) {
     constexpr int DP = decltype(dim)::value, CG = decltype(cg)::value;
     const dim3 grid(static_cast<uint32_t>(shape.even != 0 ? shape.even : groups * shape.parts));
-    if constexpr (few_waves<DP, CG>() == 2) {
-      if (shape.waves == 8) {
-        hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 8>), grid, dim3(512), 0, stream, a);
-        return;
-      }
-    }
-    hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 4>), grid, dim3(256), 0, stream, a);
+    if (shape.waves == 8) hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 8>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 4>), grid, dim3(256), 0, stream, a);
   };
   auto with_columns = [&](auto kind, auto dim) {
     if (shape.columns == 64) return tile(kind, dim);
