@@ -157,44 +157,102 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
   }
 }
 
-// Bound by memory: 2 bytes a row's element in, 8 or 4 out.
+// Bound by memory: 2 bytes a row's element in, 8 or 4 out.  A workgroup takes the keys or the values of a head at 64 places that begin at
+// a multiple of 64, so that pages of 16 places do not make a workgroup of 16 bytes a thread.
+constexpr uint32_t kReadPlaces = 64;
+__device__ __forceinline__ uint32_t read_units(const PageSequence& q) { return (q.len - 1u) / kReadPlaces - (q.len - q.rows) / kReadPlaces + 1u; }
+
 template <PageKind KIND, class Out>
 __global__ __launch_bounds__(kPageThreads) void pages_read_kernel(PageBatch b, const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp,
-                                                                  const float* __restrict__ ks, const float* __restrict__ vs, Out* k, Out* v) {
-  PageWork w;
-  if (!page_work(b, &w)) return;
-  const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block;
+                                                                  const float* __restrict__ ks, const float* __restrict__ vs, Out* __restrict__ k,
+                                                                  Out* __restrict__ v) {
+  __shared__ uint32_t page_of[4];
+  __shared__ float scale_of[4];
+  const uint32_t which = blockIdx.x % (2u * b.kv_heads), t = threadIdx.x, D = b.head_dim;
+  PageUnit u;
+  if (!find_unit(b, blockIdx.x / (2u * b.kv_heads), [](const PageSequence& q) { return read_units(q); }, &u)) return;
+  const bool values = which >= b.kv_heads;
+  const uint32_t kv = values ? which - b.kv_heads : which, past = u.seq.len - u.seq.rows, base = (past / kReadPlaces + u.at) * kReadPlaces;
+  const uint32_t from = past > base ? past - base : 0u, to = u.seq.len - base < kReadPlaces ? u.seq.len - base : kReadPlaces;
+  // Quarters of sixteen places, each in one page.  (Those behind the last position are the last one's, and not used.)
+  if (t < 4u) {
+    const uint32_t at = 16u * t < to ? base + 16u * t : u.seq.len - 1u, page = b.table[static_cast<uint64_t>(u.s) * b.width + (at >> b.log_block)];
+    page_of[t] = page;
+    scale_of[t] = page < b.pages ? (values ? vs : ks)[static_cast<uint64_t>(page) * b.kv_heads + kv] : 0.0f;
+  }
+  __syncthreads();
   const uint64_t wide = static_cast<uint64_t>(b.kv_heads) * D;
-  Out* rows = (w.values ? v : k) + static_cast<uint64_t>(w.first_row) * wide + w.kv * D;   // of place `from`
-  const uint64_t head = static_cast<uint64_t>(w.held ? w.page : 0u) * b.kv_heads + w.kv;
-  const float scale = w.held ? (w.values ? vs : ks)[head] : 0.0f;
-  const uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
-  auto value = [&](uint32_t four, int i) {
-    float x = w.held ? decode<KIND>(four, i) * scale : 0.0f;
+  Out* rows = (values ? v : k) + static_cast<uint64_t>(u.seq.first + (base + from - past)) * wide + kv * D;   // of place `from`
+  const uint32_t block = 1u << b.log_block;
+  auto head_of = [&](uint32_t quarter) {
+    const uint32_t page = page_of[quarter];
+    return (values ? vp : kp) + (static_cast<uint64_t>(page < b.pages ? page : 0u) * b.kv_heads + kv) * (static_cast<uint64_t>(block) * D);
+  };
+  // (A page that is not held has the scale 0 here; its codes may be a NaN's.)
+  auto value = [&](uint32_t four, int i, float scale, bool held) {
+    float x = held ? decode<KIND>(four, i) * scale : 0.0f;
     asm("" : "+v"(x));                                     // (an fp32 number before it is an fp16 one: no one operation for both)
     return static_cast<Out>(x);
   };
-  if (!w.values) {
-    const uint32_t runs = D / 4u;
-    for (uint32_t i = t; i < (w.to - w.from) * runs; i += kPageThreads) {
-      const uint32_t at = i / runs, d = i % runs * 4u;
-      const uint32_t four = *reinterpret_cast<const uint32_t*>(codes + (w.from + at) * D + d);
-      Out* to = rows + at * wide + d;
-      typedef Out out4 __attribute__((ext_vector_type(4)));
-      *reinterpret_cast<out4*>(to) = out4{value(four, 0), value(four, 1), value(four, 2), value(four, 3)};
+  if (!values) {
+    constexpr uint32_t EACH = 16u / sizeof(Out);           // elements of a thread's sixteen bytes out
+    typedef Out outs __attribute__((ext_vector_type(EACH)));
+    const uint32_t runs = D / EACH, of_run = (1u << 20) / runs + 1u;      // (i < 64 * 64: i / runs by its product)
+    const uint32_t end = to * runs;
+    constexpr uint32_t AHEAD = 4;                          // loads on their way at once
+    for (uint32_t i0 = t + from * runs; i0 < end; i0 += AHEAD * kPageThreads) {
+      uint32_t four[AHEAD][EACH / 4];
+#pragma unroll
+      for (uint32_t n = 0; n < AHEAD; ++n) {
+        const uint32_t i = i0 + n * kPageThreads < end ? i0 + n * kPageThreads : end - 1u;
+        const uint32_t place = i * of_run >> 20, d = (i - place * runs) * EACH;
+        const uint32_t* codes = reinterpret_cast<const uint32_t*>(head_of(place / 16u) + (((base + place) & (block - 1u)) * D + d));
+#pragma unroll
+        for (uint32_t j = 0; j < EACH / 4; ++j) four[n][j] = codes[j];
+      }
+#pragma unroll
+      for (uint32_t n = 0; n < AHEAD; ++n) {
+        const uint32_t i = i0 + n * kPageThreads;
+        if (i >= end) break;
+        const uint32_t place = i * of_run >> 20, d = (i - place * runs) * EACH, quarter = place / 16u;
+        const float scale = scale_of[quarter];
+        const bool held = page_of[quarter] < b.pages;
+        outs x;
+#pragma unroll
+        for (uint32_t e = 0; e < EACH; ++e) x[e] = value(four[n][e / 4], static_cast<int>(e % 4), scale, held);
+        *reinterpret_cast<outs*>(rows + (place - from) * wide + d) = x;
+      }
     }
     return;
   }
-  for (uint32_t i = t + w.from / 16u * D; i < (w.to + 15u) / 16u * D; i += kPageThreads) {
-    const uint32_t place = i / D * 16u, d = i % D;
-    const uint4 run = load_u4(codes + d * block + place);
-    const uint32_t r[4] = {run.x, run.y, run.z, run.w};
+  // Sixteen places of two elements, which the next lane's follow in a row.
+  const uint32_t pairs = D / 2u, of_pair = (1u << 20) / pairs + 1u, end = (to + 15u) / 16u * pairs;
+  constexpr uint32_t AHEAD = 2;
+  for (uint32_t i0 = t + from / 16u * pairs; i0 < end; i0 += AHEAD * kPageThreads) {
+    uint4 run[AHEAD][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (uint32_t n = 0; n < AHEAD; ++n) {
+      const uint32_t i = i0 + n * kPageThreads < end ? i0 + n * kPageThreads : end - 1u;
+      const uint32_t quarter = i * of_pair >> 20, d = (i - quarter * pairs) * 2u;
+      const uint8_t* codes = head_of(quarter) + (d * block + ((base + quarter * 16u) & (block - 1u)));
+      run[n][0] = load_u4(codes), run[n][1] = load_u4(codes + block);
+    }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t at = place + 4u * j + e;
-        if (at >= w.from && at < w.to) rows[(at - w.from) * wide + d] = value(r[j], e);
+    for (uint32_t n = 0; n < AHEAD; ++n) {
+      const uint32_t i = i0 + n * kPageThreads;
+      if (i >= end) break;
+      const uint32_t quarter = i * of_pair >> 20, d = (i - quarter * pairs) * 2u, place = quarter * 16u;
+      const uint32_t r[2][4] = {{run[n][0].x, run[n][0].y, run[n][0].z, run[n][0].w}, {run[n][1].x, run[n][1].y, run[n][1].z, run[n][1].w}};
+      const float scale = scale_of[quarter];
+      const bool held = page_of[quarter] < b.pages;
+      typedef Out out2 __attribute__((ext_vector_type(2)));
+      Out* out = rows + static_cast<int64_t>(static_cast<int32_t>(place - from)) * static_cast<int64_t>(wide) + d;
+      const bool whole = place >= from && place + 16u <= to;
+#pragma unroll
+      for (uint32_t e = 0; e < 16u; ++e) {
+        if (whole || (place + e >= from && place + e < to)) {
+          *reinterpret_cast<out2*>(out + e * wide) = out2{value(r[0][e / 4], static_cast<int>(e % 4), scale, held), value(r[1][e / 4], static_cast<int>(e % 4), scale, held)};
+        }
       }
     }
   }
@@ -224,9 +282,11 @@ hipError_t launch_pages_write(bool fp8, const PageWriteCall& c, const float* k, 
 
 hipError_t launch_pages_read(bool fp8, const PageReadCall& c, const uint8_t* kp, const uint8_t* vp, const float* ks, const float* vs, const uint32_t* table,
                              const uint32_t* starts, const uint32_t* lens, void* k, void* v, hipStream_t stream) {
+  // (a sequence's rows lie in at most two runs of 64 places more than they fill)
+  const uint64_t some = c.page.rows / kReadPlaces + 2 * c.page.sequences, units = some < c.page.rows ? some : c.page.rows;
   auto go = [&](auto kernel, auto* as) {
     using Out = std::remove_pointer_t<decltype(as)>;
-    hipLaunchKernelGGL(kernel, dim3(workgroups(c.page)), dim3(kPageThreads), 0, stream, page_batch(c.page, table, starts, lens), kp, vp, ks, vs,
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(units * c.page.kv_heads * 2)), dim3(kPageThreads), 0, stream, page_batch(c.page, table, starts, lens), kp, vp, ks, vs,
                        static_cast<Out*>(k), static_cast<Out*>(v));
   };
   float* f32 = nullptr;
