@@ -62,15 +62,15 @@ __device__ __forceinline__ bool page_work(const PageBatch& b, PageWork* w) {
 // lane, so that a wavefront's loads of rows are whole lines.
 constexpr uint32_t kPageThreads = 256;
 
-// Bound by memory: 8 bytes a row's element in, 2 out, and what a page that is continued holds.  Rows are read twice, for the
-// largest and for the codes, the second time out of the caches.
-template <PageKind KIND>
+// Bound by memory: 8 bytes a row's element in, 2 out, and what a page that is continued holds.  A thread holds its ITEMS runs' rows from
+// the search for the largest on, so that they are read once.
+template <PageKind KIND, int ITEMS>
 __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, const float* __restrict__ k, const float* __restrict__ v, uint64_t k_stride,
                                                                    uint64_t v_stride, uint8_t* kp, uint8_t* vp, float* ks, float* vs) {
   __shared__ uint32_t most_of[kPageThreads / 64];
   PageWork w;
   if (!page_work(b, &w) || !w.held) return;               // workgroup-uniform
-  const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block;
+  const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block, runs = D / 16u;
   const uint64_t stride = w.values ? v_stride : k_stride;
   const float* rows = (w.values ? v : k) + static_cast<uint64_t>(w.first_row) * stride + w.kv * D;   // of place `from`
   const uint64_t head = static_cast<uint64_t>(w.page) * b.kv_heads + w.kv;
@@ -78,13 +78,43 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
   uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
   const float before = w.from == 0u ? 0.0f : *scale_at;
 
-  // The largest magnitude by its bits: infinities and NaN are above all numbers.
-  uint32_t most = 0u;
-  for (uint32_t i = t; i < (w.to - w.from) * (D / 4u); i += kPageThreads) {
-    const float4 x = *reinterpret_cast<const float4*>(rows + i / (D / 4u) * stride + i % (D / 4u) * 4u);
-    const float xs[4] = {x.x, x.y, x.z, x.w};
+  // A thread's n-th run: of a key's elements d .. d + 15 at `place`, or of an element d at places place .. place + 15.
+  const uint32_t count = block * runs, of_row = (1u << 20) / (w.values ? D : runs) + 1u;      // (i < 2048 is divided by its product)
+  struct Run {
+    uint32_t i, place, d;
+  };
+  auto run_of = [&](int n) {
+    const uint32_t i = t + static_cast<uint32_t>(n) * kPageThreads, row = i * of_row >> 20;
+    return w.values ? Run{i, row * 16u, i - row * D} : Run{i, row, (i - row * runs) * 16u};
+  };
+  const uint32_t rows_here = w.to - w.from;
+  float x[ITEMS][16];
+  uint32_t most = 0u;                                      // the largest magnitude by its bits: infinities and NaN are above all numbers
 #pragma unroll
-    for (int e = 0; e < 4; ++e) most = max(most, bit_cast<uint32_t>(xs[e]) & 0x7FFFFFFFu);
+  for (int n = 0; n < ITEMS; ++n) {
+    const Run r = run_of(n);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
+    if (!w.values) {
+      if (r.i < count && r.place >= w.from && r.place < w.to) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const float4 four = *reinterpret_cast<const float4*>(rows + (r.place - w.from) * stride + r.d + e);
+          x[n][e] = four.x, x[n][e + 1] = four.y, x[n][e + 2] = four.z, x[n][e + 3] = four.w;
+        }
+      }
+    } else if (r.i < count && r.place + 15u >= w.from && r.place < w.to) {
+      // (places that hold no new row: another one's, so that no load has a condition, and then nothing)
+#pragma unroll
+      for (uint32_t e = 0; e < 16u; ++e) {
+        const uint32_t at = r.place + e - w.from;          // (before the first: far above the last)
+        x[n][e] = rows[(at < rows_here ? at : 0u) * stride + r.d];
+      }
+#pragma unroll
+      for (uint32_t e = 0; e < 16u; ++e) x[n][e] = r.place + e - w.from < rows_here ? x[n][e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) most = max(most, bit_cast<uint32_t>(x[n][e]) & 0x7FFFFFFFu);
   }
 #pragma unroll
   for (uint32_t off = 32u; off > 0u; off >>= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(most, off, kWave)));
@@ -98,62 +128,36 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
   const float scale = finite ? fmaxf(before, own) : bit_cast<float>(0x7FC00000u);
   if (t == 0u) *scale_at = scale;
   const bool empty = !(scale > 0.0f);                      // (NaN too): all codes 0
-  const bool again = w.from != 0u && (empty || scale != before);
-
-  if (!w.values) {
-    const uint32_t runs = D / 16u;
-    for (uint32_t i = t + (again ? 0u : w.from * runs); i < block * runs; i += kPageThreads) {
-      const uint32_t place = i / runs, d = i % runs * 16u;
-      uint4* to = reinterpret_cast<uint4*>(codes + place * D + d);
-      uint32_t r[4] = {0u, 0u, 0u, 0u};
-      if (!empty && place < w.to) {
-        if (place < w.from) {
-          const uint4 old = *to;
-          const uint32_t o[4] = {old.x, old.y, old.z, old.w};
+  const bool again = w.from != 0u && (empty || scale != before);      // codes that were there change
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            r[j] = encode4<KIND>(decode<KIND>(o[j], 0) * before, decode<KIND>(o[j], 1) * before, decode<KIND>(o[j], 2) * before, decode<KIND>(o[j], 3) * before, scale);
-          }
-        } else {
-          const float* from = rows + (place - w.from) * stride + d;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 x = *reinterpret_cast<const float4*>(from + 4 * j);
-            r[j] = encode4<KIND>(x.x, x.y, x.z, x.w, scale);
-          }
-        }
-      }
-      *to = uint4{r[0], r[1], r[2], r[3]};
-    }
-    return;
-  }
-  const uint32_t from16 = again ? 0u : w.from / 16u;
-  for (uint32_t i = t + from16 * D; i < block / 16u * D; i += kPageThreads) {
-    const uint32_t run = i / D, d = i % D, place = run * 16u;
-    uint4* to = reinterpret_cast<uint4*>(codes + d * block + place);
-    uint32_t r[4] = {0u, 0u, 0u, 0u};
-    if (!empty && place < w.to) {
-      uint32_t o[4] = {0u, 0u, 0u, 0u};
-      if (place < w.from) {
+  for (int n = 0; n < ITEMS; ++n) {
+    const Run r = run_of(n);
+    const uint32_t old_places = r.place >= w.from ? 0u : w.values ? w.from - r.place : 1u;      // of the run's, that held codes (16 and more: all)
+    if (r.i >= count || (!again && (w.values ? old_places >= 16u : old_places != 0u))) continue;
+    uint4* to = reinterpret_cast<uint4*>(codes + (w.values ? r.d * block + r.place : r.place * D + r.d));
+    uint32_t four[4] = {0u, 0u, 0u, 0u};
+    if (!empty && r.place < w.to) {
+      if (old_places != 0u) {
         const uint4 old = *to;
-        o[0] = old.x, o[1] = old.y, o[2] = old.z, o[3] = old.w;
-      }
+        const uint32_t o[4] = {old.x, old.y, old.z, old.w}, olds = w.values ? old_places : 16u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float x[4];
+        for (uint32_t e = 0; e < 16u; ++e) {
+          if (e < olds) x[n][e] = decode<KIND>(o[e / 4], static_cast<int>(e % 4)) * before;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t at = place + 4u * j + e;
-          x[e] = at < w.from ? decode<KIND>(o[j], e) * before : at < w.to ? rows[(at - w.from) * stride + d] : 0.0f;
+        for (uint32_t j = 0; j < 4; ++j) {
+          four[j] = encode4<KIND>(x[n][4 * j], x[n][4 * j + 1], x[n][4 * j + 2], x[n][4 * j + 3], scale);
+          if (!again && 4u * j < olds) {                   // codes that stay
+            const uint32_t stay = olds - 4u * j, mask = stay < 4u ? (1u << 8u * stay) - 1u : ~0u;
+            four[j] = (four[j] & ~mask) | (o[j] & mask);
+          }
         }
-        r[j] = encode4<KIND>(x[0], x[1], x[2], x[3], scale);
-        if (!again && place + 4u * j < w.from) {           // codes that stay
-          const uint32_t stay = w.from - place - 4u * j, mask = stay < 4u ? (1u << 8u * stay) - 1u : ~0u;
-          r[j] = (r[j] & ~mask) | (o[j] & mask);
-        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) four[j] = encode4<KIND>(x[n][4 * j], x[n][4 * j + 1], x[n][4 * j + 2], x[n][4 * j + 3], scale);
       }
     }
-    *to = uint4{r[0], r[1], r[2], r[3]};
+    *to = uint4{four[0], four[1], four[2], four[3]};
   }
 }
 
@@ -276,7 +280,13 @@ hipError_t launch_pages_write(bool fp8, const PageWriteCall& c, const float* k, 
     hipLaunchKernelGGL(kernel, dim3(workgroups(c.page)), dim3(kPageThreads), 0, stream, page_batch(c.page, table, starts, lens), k, v, c.k_stride, c.v_stride,
                        kp, vp, ks, vs);
   };
-  fp8 ? go(pages_write_kernel<PageKind::Fp8>) : go(pages_write_kernel<PageKind::Q8>);
+  const uint64_t runs = c.page.block * c.page.head_dim / 16;      // of a page: at most 2048
+  auto with = [&](auto items) {
+    constexpr int N = decltype(items)::value;
+    fp8 ? go(pages_write_kernel<PageKind::Fp8, N>) : go(pages_write_kernel<PageKind::Q8, N>);
+  };
+  runs <= 256 ? with(std::integral_constant<int, 1>{}) : runs <= 512 ? with(std::integral_constant<int, 2>{})
+  : runs <= 1024 ? with(std::integral_constant<int, 4>{}) : with(std::integral_constant<int, 8>{});
   return hipGetLastError();
 }
 
