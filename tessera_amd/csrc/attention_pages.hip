@@ -135,13 +135,13 @@ struct Column {
 };
 
 // Products to weights times the values' scale, as two terms; `scale` makes a product a score in powers of two.  COUNT of a lane's positions
-// of the tile; bit i of `shown`: the column sees the i-th; `all`: every column sees all.  A weight is below 2^kSlack, so that with
+// of the tile; bit i of `shown`: the column sees the i-th; ALL: every column sees all.  A weight is below 2^kSlack, so that with
 // v_scale * up below 2^12 all is as it should be; else, and where the reference moves, the sums so far are to be scaled by *corr (true).
-template <int COUNT>
-__device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale, uint32_t shown, bool all, float v_scale, half8_t (&hi)[COUNT / 8],
+template <bool ALL, int COUNT>
+__device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale, uint32_t shown, float v_scale, half8_t (&hi)[COUNT / 8],
                                       half8_t (&lo)[COUNT / 8], float* corr) {
   scale = scale == 0.0f ? 0x1p-126f : scale;      // (keys that are all 0: a hidden product stays -infinity)
-  if (!all) {
+  if constexpr (!ALL) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) s[i] = (shown >> i & 1u) != 0u ? s[i] : -INFINITY;
   }
@@ -172,10 +172,10 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float p = __builtin_amdgcn_exp2f(fmaf(s[i + e], scale, -to));
-      if (!all) p = (shown >> (i + e) & 1u) != 0u ? p : 0.0f;                             // (a hidden position's scales may be NaN)
+      if constexpr (!ALL) p = (shown >> (i + e) & 1u) != 0u ? p : 0.0f;                             // (a hidden position's scales may be NaN)
       c.sum += p;
       w[e] = p * factor;
-      if (!all) w[e] = (shown >> (i + e) & 1u) != 0u ? w[e] : 0.0f;
+      if constexpr (!ALL) w[e] = (shown >> (i + e) & 1u) != 0u ? w[e] : 0.0f;
     }
     const half2_t h = __builtin_convertvector(w, half2_t);
     const float2_v rest = {fmaf(static_cast<float>(h[0]), -1.0f, w[0]), fmaf(static_cast<float>(h[1]), -1.0f, w[1])};
@@ -522,18 +522,21 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
       float s[OWN], corr;
 #pragma unroll
       for (uint32_t e = 0; e < OWN; ++e) s[e] = acc[cg][e / 4][e % 4];
-      uint32_t shown = (1u << OWN) - 1u;
-      if (!all) {
+      bool moves;
+      if (all) {
+        moves = weigh<true>(col[cg], s, q_scale[cg] * k_scale, 0u, v_scale, p_hi[cg], p_lo[cg], &corr);
+      } else {
         const uint32_t p0 = first + OWN * g;
-        shown = 0u;
+        uint32_t shown = 0u;
 #pragma unroll
         for (uint32_t e = 0; e < OWN; ++e) {
           const uint32_t p = p0 + e;
           const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & in_pool;
           shown |= (sees ? 1u : 0u) << e;
         }
+        moves = weigh<false>(col[cg], s, q_scale[cg] * k_scale, shown, v_scale, p_hi[cg], p_lo[cg], &corr);
       }
-      if (weigh<static_cast<int>(OWN)>(col[cg], s, q_scale[cg] * k_scale, shown, all, v_scale, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
+      if (moves) scale_sums(o[cg], corr);
     }
 #pragma unroll
     for (int x = 0; x < VL; ++x) {
@@ -803,18 +806,21 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
       float corr;
-      uint32_t shown = 0xFFu;
-      if (!all) {
+      bool moves;
+      if (all) {
+        moves = weigh<true>(col[cg], s[cg], q_scale[cg] * scales.k, 0u, scales.v, p_hi[cg], p_lo[cg], &corr);
+      } else {
         const uint32_t p0 = first + 16u * g + 8u * half;
-        shown = 0u;
+        uint32_t shown = 0u;
 #pragma unroll
         for (uint32_t e = 0; e < 8u; ++e) {
           const uint32_t p = p0 + e;
           const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & (scales.known != 0u);
           shown |= (sees ? 1u : 0u) << e;
         }
+        moves = weigh<false>(col[cg], s[cg], q_scale[cg] * scales.k, shown, scales.v, p_hi[cg], p_lo[cg], &corr);
       }
-      if (weigh<8>(col[cg], s[cg], q_scale[cg] * scales.k, shown, all, scales.v, p_hi[cg], p_lo[cg], &corr)) scale_sums(o[cg], corr);
+      if (moves) scale_sums(o[cg], corr);
     }
 #pragma unroll
     for (int x = 0; x < VL; x += 4 / CG) {
