@@ -77,6 +77,7 @@ class Pages(Call):
 # (each writes whole pages, from their first position: a pool that was cleared gives the same bits again)
 CALLS = [("pages_write_q8", [64, 7], [64, 7]), ("pages_write_fp8", [33], [65]), ("pages_read_q8", [90, 3], [200, 35]), ("pages_read_fp8", [5], [70]),
          ("attention_pages_q8", [1] * 5, [1900, 33, 700, 64, 5000]), ("attention_pages_fp8", [2], [20000]), ("attention_pages_q8", [200, 1, 30], [260, 900, 30]),
+         ("attention_pages_q8", [1] * 6, [12000, 300, 9000, 64, 12000, 5000]), ("attention_pages_fp8", [5, 3, 4], [16000, 9000, 500]),
          ("draft_verify", [5, 1, 4], [40001]), ("draft_verify", [3] * 9, [3000])]
 
 
