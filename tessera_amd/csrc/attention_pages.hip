@@ -166,6 +166,8 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
   }
   const float to = from_reference(c.ref), factor = v_scale * c.up;
   typedef float float2_v __attribute__((ext_vector_type(2)));
+  float minus_one = -1.0f;
+  asm("" : "+s"(minus_one));                                      // (a product with the fp16 number as it is, not its conversion and a difference)
 #pragma unroll
   for (int i = 0; i < COUNT; i += 2) {
     float2_v w;
@@ -178,7 +180,7 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
       if constexpr (!ALL) w[e] = (shown >> (i + e) & 1u) != 0u ? w[e] : 0.0f;
     }
     const half2_t h = __builtin_convertvector(w, half2_t);
-    const float2_v rest = {fmaf(static_cast<float>(h[0]), -1.0f, w[0]), fmaf(static_cast<float>(h[1]), -1.0f, w[1])};
+    const float2_v rest = {fmaf(static_cast<float>(h[0]), minus_one, w[0]), fmaf(static_cast<float>(h[1]), minus_one, w[1])};
     const half2_t l = __builtin_convertvector(rest, half2_t);
     hi[i / 8][i % 8] = h[0], hi[i / 8][i % 8 + 1] = h[1], lo[i / 8][i % 8] = l[0], lo[i / 8][i % 8 + 1] = l[1];
   }
@@ -801,6 +803,15 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       }
     }
     fetch_keys(i + 2u, next);
+    // The first values' operands are on their way while the weights are formed.  (Not where that costs the third wavefront a SIMD.)
+    constexpr bool EARLY = DP > 64;
+    constexpr int EACH = 4 / CG;
+    half8_t ahead[EACH];
+    auto read_values = [&](int x) {
+#pragma unroll
+      for (int y = 0; y < EACH; ++y) ahead[y] = bit_cast<half8_t>(sh.stage[buf][Shared::KEYS + 2 * (x + y) + half][lane]);
+    };
+    if constexpr (EARLY) read_values(0);
     const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(scales.known != 0u);
     half8_t p_hi[CG][1], p_lo[CG][1];
 #pragma unroll
@@ -823,19 +834,21 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       if (moves) scale_sums(o[cg], corr);
     }
 #pragma unroll
-    for (int x = 0; x < VL; x += 4 / CG) {
-      half8_t value[4 / CG];
+    for (int x = 0; x < VL; x += EACH) {
+      if constexpr (!EARLY) read_values(x);
+      half8_t value[EACH];
 #pragma unroll
-      for (int y = 0; y < 4 / CG; ++y) value[y] = bit_cast<half8_t>(sh.stage[buf][Shared::KEYS + 2 * (x + y) + half][lane]);
+      for (int y = 0; y < EACH; ++y) value[y] = ahead[y];
+      if (EARLY && x + EACH < VL) read_values(x + EACH);
 #pragma unroll
       for (int term = 1; term >= 0; --term) {                       // (the same sum's products four apart)
 #pragma unroll
-        for (int y = 0; y < 4 / CG; ++y) {
+        for (int y = 0; y < EACH; ++y) {
 #pragma unroll
           for (int cg = 0; cg < CG; ++cg) o[cg][x + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[y], term == 1 ? p_lo[cg][0] : p_hi[cg][0], o[cg][x + y], 0, 0, 0);
         }
       }
-      if ((x + 4 / CG) % WAVES == 0) stash_values(buf ^ 1u, x / WAVES);
+      if ((x + EACH) % WAVES == 0) stash_values(buf ^ 1u, x / WAVES);
     }
     fetch_values(i + 2u, next);
     scales = of_next, of_next = after, next = further;
