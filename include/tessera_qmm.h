@@ -17,7 +17,7 @@
  *     tessera::StatusCode (include/tessera/types.hpp:36-48);
  *   - no exceptions cross the boundary;
  *   - device memory: qmm_alloc allocates what the caller asks for; qmm_init allocates the 16 MB
- *     scratch of the decode-sized kernels once and reserves 256 + 64 MB for the blocks below; prefill-sized launches
+ *     scratch of the decode-sized kernels once and reserves 256 + 64 + 64 MB for the blocks below; prefill-sized launches
  *     (Q4_K/Q5_K/Q6_K and MXFP4 with fp32 rows from 17 rows, the grouped routed-expert ids) need a workspace, which is the caller's when one was
  *     set with qmm_set_workspace and otherwise a library-owned block that qmm_launch grows on
  *     demand with hipMalloc.  A block that a launch has used is never freed (growth allocates a
@@ -32,9 +32,9 @@
  *     stream that records them: "gemm_fp8" from 17 rows (128 MB more where a call does not fit) and
  *     "gemm_q5k*" / "gemm_q6k*" with 2..16 rows out of the 256 MB that qmm_init reserves, then out of slabs of
  *     128 MB, 2 GB in all; "attention", "attention_q8", "_q4" and "_fp8" from 17 rows, "attention_tree" and its forms
- *     and "attention_pages_*" over long caches, "draft_verify", "top_k_rows" and "token_logprobs" over long rows out of
- *     64 MB, then slabs of 64 MB, 512 MB in all.  Products of Q4_K, Q5_K and Q6_K with few tiles whose
- *     workspace has no room for what they hand on (a caller's of just the operands, a capture before the library's
+ *     over long caches, "top_k_rows" and "token_logprobs" over long rows out of 64 MB, then slabs of 64 MB, 512 MB in
+ *     all; "attention_pages_*" over long caches and "draft_verify" out of as much again.  Products of Q4_K,
+ *     Q5_K and Q6_K with few tiles whose workspace has no room for what they hand on (a caller's of just the operands, a capture before the library's
  *     has grown) likewise, 16 to 40 MB out of slabs of 128 MB, 1 GB in all; qmm_set_workspace reserves the first.
  *     While a caller's workspace is set no slab is allocated.  The blocks are not given back (a graph may
  *     still use them), and a stream handle's block passes to the next stream with that handle: let a

@@ -228,7 +228,7 @@ __device__ __forceinline__ uint32_t even_share(const PageAttention& a, uint32_t 
 // 33 us, of which 5 pass until the first tile is there and 4 until the last workgroup has begun; 1 row on 1187, 16 over 4 of 64: 9 us,
 // of which 2.2 go by before the sequence is found, 2 before its tiles are there, 1.5 a tile for the longest wavefront.
 // Positions of a tile: 64, or 32 where a tile's codes and the sums together are more registers than two wavefronts a SIMD have.
-constexpr uint32_t few_tile(int elements) { return elements <= 128 ? 64 : 32; }
+constexpr uint32_t few_tile(uint64_t head_dim, uint64_t columns) { return head_dim <= 128 && columns == 16 ? 64 : 32; }
 constexpr int query_operands(PageKind kind, int dp) { return kind == PageKind::Q8 ? 3 * (dp / 64) : 2 * (dp / 32); }
 
 template <PageKind KIND, int DP, int CG, int NW>
@@ -320,7 +320,7 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 template <PageKind KIND, int DP, int CG, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAttention a) {
   constexpr int KL = DP / 64, VL = DP / 16, C = 16 * CG;
-  constexpr uint32_t TILE = few_tile(DP * CG), OWN = TILE / 4;      // positions of a tile, and of a lane's
+  constexpr uint32_t TILE = few_tile(DP, C), OWN = TILE / 4;      // positions of a tile, and of a lane's
   constexpr int NT = TILE / 16;                                     // key operands
   __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
@@ -448,7 +448,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
     if constexpr (MORE) from_k = keys_at(i + NW, next), from_v = values_at(i + NW, next);
     float4_t acc[CG][NT];
     if constexpr (KIND == PageKind::Q8) {
-      constexpr int YB = DP * CG == 256 && CG == 2 ? 1 : 2;            // key operands that share a query operand's way from LDS
+      constexpr int YB = CG == 2 ? 1 : 2;                            // key operands that share a query operand's way from LDS
 #pragma unroll
       for (int y0 = 0; y0 < NT; y0 += YB) {
         uint32_t from = lane;
@@ -992,8 +992,7 @@ uint64_t units_of(const PageAttentionCall& c, uint64_t columns) {
 
 // Positions of a tile, and tiles that a unit walks at most.
 static uint32_t log_tile_of(const PageAttentionCall& c, uint64_t columns) {
-  const uint64_t D = c.page.head_dim, padded = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-  return columns < 64 && few_tile(static_cast<int>(padded * columns / 16)) == 32 ? 5u : 6u;
+  return columns < 64 && few_tile(c.page.head_dim, columns) == 32 ? 5u : 6u;
 }
 static uint64_t tiles_of(const PageAttentionCall& c, uint64_t columns) {
   const uint64_t tile = uint64_t{1} << log_tile_of(c, columns), all = (c.max_len + tile - 1) / tile;

@@ -190,6 +190,8 @@ qmm::StreamScratch g_stream_scratch;
 // calls are as correct without it and lose less, and a program that records them again and again uses theirs up.
 constexpr qmm::ScratchLimits kPartsLimits{size_t{16} << 20, size_t{16} << 20, size_t{64} << 10, size_t{64} << 20, size_t{64} << 20, size_t{512} << 20};
 qmm::StreamScratch g_parts_scratch(kPartsLimits);
+// That of "attention_pages_*" over long caches and of "draft_verify", likewise: a batch's step on many streams takes none of theirs.
+qmm::StreamScratch g_pages_scratch(kPartsLimits);
 
 class StreamBlock {
  public:
@@ -1556,7 +1558,7 @@ qmm_status run_attention_pages(const LaunchCtx& c, bool fp8) {
   };
   const qmm::PagesShape in_parts = qmm::attention_pages_shape(call, true);
   if (in_parts.parts > 1 || in_parts.even != 0) {
-    const StreamBlock block(c, qmm::attention_pages_parts_bytes(call, in_parts), g_parts_scratch);
+    const StreamBlock block(c, qmm::attention_pages_parts_bytes(call, in_parts), g_pages_scratch);
     if (block.get() != nullptr) return go(in_parts, block.get());
   }
   return go(qmm::attention_pages_shape(call, false), nullptr);
@@ -1570,7 +1572,7 @@ qmm_status run_draft_verify(const LaunchCtx& c) {
   qmm::DraftCall call;
   if (const char* why = qmm::check_draft_verify(args_of(c), &call)) return bad(why);
   const size_t need = qmm::draft_verify_scratch_bytes(call);
-  const StreamBlock block(c, need <= kPartsLimits.small ? need : 0, g_parts_scratch);
+  const StreamBlock block(c, need <= kPartsLimits.small ? need : 0, g_pages_scratch);
   return map_hip(qmm::launch_draft_verify(call, c.ptr<const float>(0), c.ptr<const uint32_t>(1), c.ptr<const float>(2), c.ptr<const uint32_t>(3),
                                           c.ptr<uint32_t>(4), c.ptr<uint32_t>(5), call.draft ? c.ptr<const float>(6) : nullptr,
                                           need <= kPartsLimits.small ? block.get() : nullptr, c.stream));
@@ -1726,6 +1728,7 @@ qmm_status qmm_init(int device) {
   // (without them the ids that use them run kernels that need none)
   (void)g_stream_scratch.reserve(StreamBlock::grow);
   (void)g_parts_scratch.reserve(StreamBlock::grow);
+  (void)g_pages_scratch.reserve(StreamBlock::grow);
   return QMM_OK;
 }
 
