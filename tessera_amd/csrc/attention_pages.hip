@@ -1024,7 +1024,7 @@ PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
   const uint64_t tiles = tiles_of(c, columns), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
   const uint64_t resident = 2 * cus, log_tile = log_tile_of(c, columns);
   const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus ? 8u : 4u};
-  if (!in_parts) return one;
+  if (!in_parts || groups * stored_of(c, columns) >= (1u << 24)) return one;      // (the merge's grid has a workgroup a column: fewer than 2^32 threads)
   if (columns < 64) {
     const uint64_t parts = (tiles + 3) / 4, of_64 = tiles >> (6 - log_tile);
     const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost, 4};

@@ -103,6 +103,27 @@ def test_many_sequences_of_all_lengths(backend, fmt, d, kv, group, most_rows, se
         assert np.all(got[at:at + rows[7]] == 7.0)
 
 
+@pytest.mark.parametrize("fmt,sequences,most", [("q8", 4096, 40), ("fp8", 257, 300), ("q8", 256, 70), ("fp8", 129, 4000)])
+def test_the_most_sequences(backend, fmt, sequences, most):
+    """Up to as many sequences as a call takes, with rows and without, written, read and attended."""
+    kv, group, d, block = 1, 2, 16, 16
+    rs = np.random.RandomState(sequences + most)
+    rows = (rs.rand(sequences) < 0.7).astype(int)
+    rows[[0, -1]] = 0, 1
+    b = Batch(backend, 61, fmt, kv, block, d, [int(n) for n in rs.randint(1, most, sequences)])
+    m = int(rows.sum())
+    k, v = queries(b.rs, m, kv * d), queries(b.rs, m, kv * d)
+    want = b.want_write([int(n) for n in rows], k, v)
+    b.write([int(n) for n in rows], k, v)
+    b.same_as(want)
+    b.pool = want
+    check(b, queries(b.rs, m, kv * group * d), [int(n) for n in rows], group, max_rows=1)
+    got = b.read(np.concatenate([[0], np.cumsum(rows)]), m)
+    wanted = [want.rows(b.table[s], np.array([int(b.lens[s]) - 1])) for s in range(sequences) if rows[s]]
+    for g, w in zip(got, zip(*wanted)):
+        assert np.array_equal(g, np.concatenate([x.reshape(1, -1) for x in w]))
+
+
 def test_rows_behind_the_last_and_what_does_not_hold(backend):
     """Rows of no sequence stay as they were; so do those of sequences that do not hold, or exceed what the launch was made for."""
     kv, group, d, block = 2, 3, 64, 16
