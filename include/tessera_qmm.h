@@ -203,7 +203,7 @@ const char* qmm_kernel_name(size_t index);
  *   - a batch of sequences in a paged cache of 8-bit keys and values, for which the reference has no ids.  A page holds
  *     `block` (16, 32, 64 or 128) positions of one sequence: keys Kp [page][kv_head][position][element], values Vp
  *     [page][kv_head][element][position], int8 codes ("_q8") or E4M3 ones ("_fp8"), an element code * scale under one
- *     fp32 scale for each page and key head (Ks, Vs: pages x kv_heads).  Page j of sequence s is Table[s * width + j]
+ *     fp32 scale, not negative, for each page and key head (Ks, Vs: pages x kv_heads).  Page j of sequence s is Table[s * width + j]
  *     (u32).  Rows Starts[s] .. Starts[s + 1] - 1 of a call (u32, sequences + 1 of them) are the last positions of
  *     sequence s, of which there are then Lens[s] (u32): one row in decode, a few with drafted tokens, many in prefill,
  *     none for a sequence that rests.  Starts, Lens and Table are read on the device, so that one recorded launch serves
@@ -227,9 +227,11 @@ const char* qmm_kernel_name(size_t index);
  *     row sees the positions up to its own; under a window (not 0) the last `window` of them and the first `sinks` of the
  *     sequence.  Positions of unknown pages are not seen; a row that sees nothing becomes zeros, and what a row does not
  *     see does not reach it.  max_rows, max_len: the most rows and positions that a sequence has (0: rows, width * block),
- *     which the launch is shaped by; a sequence with more is left out.  Scores and sums are fp32.  A query's element goes
- *     to 2^-23 of its head's largest over int8 pages, over E4M3 ones to 2^-22 of itself down to 2^-16 of that largest (2^-38
- *     of it below); a weight times its value's scale to 2^-22 of itself down to 2^-12 of the row's largest (2^-34 of that below).
+ *     which the launch is shaped by; a sequence with more is left out.  (E4M3's codes of NaN, which "pages_write_fp8" does not
+ *     write, are not looked for: in a page of Vp that is walked they reach rows that do not see them.)  Scores and sums are
+ *     fp32.  A query's element goes to 2^-23 of its head's largest over int8 pages, over E4M3 ones to 2^-22 of itself down
+ *     to 2^-16 of that largest (2^-38 of it below); a weight times its value's scale to 2^-22 of itself down to 2^-12 of the
+ *     row's largest (2^-34 of that below).
  *     How positions are shared among workgroups depends on the sizes, max_rows, max_len and Lens, and the last bits with it.
  *     "draft_verify": buffers Logits (rows x vocab floats), Tokens (rows u32), Random (rows x 2 floats in [0, 1)), Starts,
  *     Accepted, Next (sequences u32)[, DraftLogits (as Logits)]; scalars rows, vocab, sequences, temperature,

@@ -68,6 +68,18 @@ __device__ __forceinline__ UnitTiles unit_tiles(const PageAttention& a, const Pa
 }
 __device__ __forceinline__ uint32_t tile_at(const UnitTiles& w, uint32_t i) { return i < w.sink_tiles ? i : w.from_tile + (i - w.sink_tiles); }
 
+// What is loaded of a page that the pool has not: a head's keys or values at most, all 0.  (Its positions are hidden, but a code that is NaN
+// would reach the sums through a weight of 0.)
+alignas(16) __device__ const uint8_t g_no_page[256 * 128] = {};
+// (An address of global memory as such: of a choice between that and a buffer's the compiler knows no more than that it is one.)
+typedef const __attribute__((address_space(1))) uint8_t* PageBytes;
+template <class T>
+__device__ __forceinline__ T load_page(PageBytes from) {
+  typedef uint32_t words __attribute__((ext_vector_type(sizeof(T) / 4)));
+  return bit_cast<T>(*(const __attribute__((address_space(1))) words*)from);
+}
+__device__ __forceinline__ PageBytes page_bytes_of(const uint8_t* pool, bool held, uint64_t at) { return held ? (PageBytes)pool + at : (PageBytes)g_no_page; }
+
 // ---- operands ------------------------------------------------------------------------------------
 
 // Eight codes (two dwords) as fp16.  The half 0x6400 | u is 1024 + u.
@@ -121,6 +133,7 @@ __device__ __forceinline__ void scale_sums(float4_t (&o)[N], float corr) {
       o[x][e] = v;
     }
   }
+  asm volatile("s_nop 1" ::);                                       // (before a matrix instruction takes them)
 }
 
 // Weights are taken relative to a reference that follows a column's largest score only where that would leave it by 2^kSlack.
@@ -332,277 +345,276 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
     at_tile = blockIdx.x * share, last_tile = at_tile + share;
   }
   for (bool first_run = true;; first_run = false) {
-  PageUnit u;
-  UnitTiles w;
-  uint32_t kv, begin, end;
-  uint64_t slot;
-  if (a.even != 0u) {
-    if (at_tile >= last_tile || !find_unit(b, at_tile, [&](const PageSequence& q) { return even_of(a, q) * b.kv_heads; }, &u)) return;
-    const uint32_t in = u.at;
-    w = sequence_tiles(a, u.seq);
-    constexpr uint32_t EMPTY = kBegin * (64u / TILE);
-    const uint32_t wide = w.tiles + EMPTY, from = in % wide, left = last_tile - at_tile, to = wide - from < left ? wide : from + left;
-    kv = in / wide;
-    if (to <= EMPTY) return;                                       // (the next workgroup begins it)
-    begin = from > EMPTY ? from - EMPTY : 0u, end = to - EMPTY;
-    slot = 2u * static_cast<uint64_t>(blockIdx.x) + (first_run ? 0u : 1u);
-    at_tile += to - from;
-  } else {
-    const uint32_t rest = blockIdx.x / b.kv_heads, part = rest % a.parts;
-    if (!first_run || !find_unit(b, rest / a.parts, [](const PageSequence&) { return 1u; }, &u)) return;
-    w = sequence_tiles(a, u.seq);
-    kv = blockIdx.x % b.kv_heads, begin = part * a.part_tiles;
-    if (begin >= w.tiles) return;
-    end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
-    slot = (static_cast<uint64_t>(rest / a.parts) * b.kv_heads + kv) * a.parts + part;
-  }
-  const uint32_t past = u.seq.len - u.seq.rows;
-
-  // Page numbers of a tile's quarters r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
-  const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
-  const uint32_t last_slot = (u.seq.len - 1u) >> b.log_block;
-  auto slot_of = [&](uint32_t position) {
-    const uint32_t s = position >> b.log_block;
-    return s < last_slot ? s : last_slot;
-  };
-  struct Numbers {
-    uint32_t k, v;
-  };
-  auto numbers = [&](uint32_t i) {
-    const uint32_t p0 = tile_at(w, i) * TILE;
-    return Numbers{table[slot_of(p0 + (r >> 2) * OWN)], table[slot_of(p0 + g * OWN)]};
-  };
-  uint4 kr[NT][KL];
-  std::conditional_t<OWN == 16, uint4, uint2> vr[VL];
-  float ks, vs;
-  bool known;
-  const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
-  // Where a lane's runs of a tile begin.  (Elements past head_dim meet zeros of the queries, or are not stored.)
-  const uint32_t past_end = 16u * g < D % 64u ? 0u : 16u * g - (D % 64u == 0u ? 0u : D % 64u - 16u);       // in a run of 64 that is not whole
-  auto keys_at = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i) * TILE + (r >> 2) * OWN) & (block - 1u);
-    return a.k + page * page_bytes + (kv * block + at + (r & 3u)) * D + 16u * g;
-  };
-  auto values_at = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i) * TILE + g * OWN) & (block - 1u);
-    return a.v + page * page_bytes + (kv * D + r) * block + at;
-  };
-  auto fetch_keys = [&](const uint8_t* from, int y, int x) {
-    const uint8_t* at = 64u * x + 64u <= D ? from : from - past_end;
-    kr[y][x] = load_u4(at + (4u * y * D + (64u * x < D ? 64u * x : 0u)));
-  };
-  auto fetch_values = [&](const uint8_t* from, int x) {
-    const uint8_t* at = from + (16u * x < D ? 16u * x * block : 0u);   // (uniform: no register of its own)
-    if constexpr (OWN == 16) vr[x] = load_u4(at);
-    else vr[x] = *reinterpret_cast<const uint2*>(at);
-  };
-  auto fetch_scales = [&](const Numbers& n) {
-    known = n.v < b.pages;
-    const uint64_t at = static_cast<uint64_t>(known ? n.v : 0u) * b.kv_heads + kv;
-    ks = a.k_scale[at], vs = a.v_scale[at];
-  };
-
-  // This lane's columns; past the last one, the last.  Their loads are before the tile's, behind whose numbers they need not wait.
-  // (No branches: where they meet again everything would be waited for.  A wavefront without a tile loads the last one.)
-  uint32_t i = begin + wave;
-  const uint32_t own = i < end ? i : end - 1u;
-  const Numbers now = numbers(own);
-  Numbers next = numbers(i + NW < end ? i + NW : own);
-  uint32_t pos[CG];
-  float q_scale[CG], raw[CG][DP / 64][16];
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const uint32_t at = cg * 16u + r, col = at < w.columns ? at : w.columns - 1u, row = col / a.group;
-    pos[cg] = past + row;
-    query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw[cg]);
-  }
-  {
-    const uint8_t *from_k = keys_at(own, now), *from_v = values_at(own, now);
-    fetch_scales(now);
-#pragma unroll
-    for (int y = 0; y < NT; ++y) {
-#pragma unroll
-      for (int x = 0; x < KL; ++x) fetch_keys(from_k, y, x);
+    PageUnit u;
+    UnitTiles w;
+    uint32_t kv, begin, end;
+    uint64_t slot;
+    if (a.even != 0u) {
+      if (at_tile >= last_tile || !find_unit(b, at_tile, [&](const PageSequence& q) { return even_of(a, q) * b.kv_heads; }, &u)) return;
+      const uint32_t in = u.at;
+      w = sequence_tiles(a, u.seq);
+      constexpr uint32_t EMPTY = kBegin * (64u / TILE);
+      const uint32_t wide = w.tiles + EMPTY, from = in % wide, left = last_tile - at_tile, to = wide - from < left ? wide : from + left;
+      kv = in / wide;
+      if (to <= EMPTY) return;                                       // (the next workgroup begins it)
+      begin = from > EMPTY ? from - EMPTY : 0u, end = to - EMPTY;
+      slot = 2u * static_cast<uint64_t>(blockIdx.x) + (first_run ? 0u : 1u);
+      at_tile += to - from;
+    } else {
+      const uint32_t rest = blockIdx.x / b.kv_heads, part = rest % a.parts;
+      if (!first_run || !find_unit(b, rest / a.parts, [](const PageSequence&) { return 1u; }, &u)) return;
+      w = sequence_tiles(a, u.seq);
+      kv = blockIdx.x % b.kv_heads, begin = part * a.part_tiles;
+      if (begin >= w.tiles) return;
+      end = w.tiles - begin < a.part_tiles ? w.tiles : begin + a.part_tiles;
+      slot = (static_cast<uint64_t>(rest / a.parts) * b.kv_heads + kv) * a.parts + part;
     }
-#pragma unroll
-    for (int x = 0; x < VL; ++x) fetch_values(from_v, x);
-  }
-  // Each wavefront makes a share of the operands.
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) q_scale[cg] = query_terms<KIND, DP>(raw[cg], D, sh.q[cg], wave, NW);
-  lds_barrier();
+    const uint32_t past = u.seq.len - u.seq.rows;
 
-  Column col[CG];
-  float4_t o[CG][VL];
+    // Page numbers of a tile's quarters r / 4 (keys) and g (values, scores).  Positions behind the last are the last page's.
+    const uint32_t* table = b.table + static_cast<uint64_t>(u.s) * b.width;
+    const uint32_t last_slot = (u.seq.len - 1u) >> b.log_block;
+    auto slot_of = [&](uint32_t position) {
+      const uint32_t s = position >> b.log_block;
+      return s < last_slot ? s : last_slot;
+    };
+    struct Numbers {
+      uint32_t k, v;
+    };
+    auto numbers = [&](uint32_t i) {
+      const uint32_t p0 = tile_at(w, i) * TILE;
+      return Numbers{table[slot_of(p0 + (r >> 2) * OWN)], table[slot_of(p0 + g * OWN)]};
+    };
+    uint4 kr[NT][KL];
+    std::conditional_t<OWN == 16, uint4, uint2> vr[VL];
+    float ks, vs;
+    bool known;
+    const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
+    // Where a lane's runs of a tile begin.  (Elements past head_dim meet zeros of the queries, or are not stored.)
+    const uint32_t past_end = 16u * g < D % 64u ? 0u : 16u * g - (D % 64u == 0u ? 0u : D % 64u - 16u);       // in a run of 64 that is not whole
+    auto keys_at = [&](uint32_t i, const Numbers& n) {
+      const uint32_t at = (tile_at(w, i) * TILE + (r >> 2) * OWN) & (block - 1u);
+      return page_bytes_of(a.k, n.k < b.pages, n.k * page_bytes + kv * block * D) + ((at + (r & 3u)) * D + 16u * g);
+    };
+    auto values_at = [&](uint32_t i, const Numbers& n) {
+      const uint32_t at = (tile_at(w, i) * TILE + g * OWN) & (block - 1u);
+      return page_bytes_of(a.v, n.v < b.pages, n.v * page_bytes + kv * block * D) + (r * block + at);
+    };
+    auto fetch_keys = [&](PageBytes from, int y, int x) {
+      const PageBytes at = 64u * x + 64u <= D ? from : from - past_end;
+      kr[y][x] = load_page<uint4>(at + (4u * y * D + (64u * x < D ? 64u * x : 0u)));
+    };
+    auto fetch_values = [&](PageBytes from, int x) {
+      const PageBytes at = from + (16u * x < D ? 16u * x * block : 0u);   // (uniform: no register of its own)
+      vr[x] = load_page<std::remove_reference_t<decltype(vr[x])>>(at);
+    };
+    auto fetch_scales = [&](const Numbers& n) {
+      known = n.v < b.pages;
+      const uint64_t at = static_cast<uint64_t>(known ? n.v : 0u) * b.kv_heads + kv;
+      ks = a.k_scale[at], vs = a.v_scale[at];
+    };
+
+    // This lane's columns; past the last one, the last.  Their loads are before the tile's, behind whose numbers they need not wait.
+    // (No branches: where they meet again everything would be waited for.  A wavefront without a tile loads the last one.)
+    uint32_t i = begin + wave;
+    const uint32_t own = i < end ? i : end - 1u;
+    const Numbers now = numbers(own);
+    Numbers next = numbers(i + NW < end ? i + NW : own);
+    uint32_t pos[CG];
+    float q_scale[CG], raw[CG][DP / 64][16];
 #pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
+    for (int cg = 0; cg < CG; ++cg) {
+      const uint32_t at = cg * 16u + r, col = at < w.columns ? at : w.columns - 1u, row = col / a.group;
+      pos[cg] = past + row;
+      query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw[cg]);
+    }
+    {
+      const PageBytes from_k = keys_at(own, now), from_v = values_at(own, now);
+      fetch_scales(now);
 #pragma unroll
-    for (int x = 0; x < VL; ++x) o[cg][x] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  auto tile = [&](auto last) {
-    constexpr bool MORE = !decltype(last)::value;
-    const uint32_t first = tile_at(w, i) * TILE;
-    const float k_scale = ks, v_scale = vs;
-    const bool in_pool = known;
-    const uint8_t *from_k = nullptr, *from_v = nullptr;
-    if constexpr (MORE) from_k = keys_at(i + NW, next), from_v = values_at(i + NW, next);
-    float4_t acc[CG][NT];
-    if constexpr (KIND == PageKind::Q8) {
-      constexpr int YB = CG == 2 ? 1 : 2;                            // key operands that share a query operand's way from LDS
+      for (int y = 0; y < NT; ++y) {
 #pragma unroll
-      for (int y0 = 0; y0 < NT; y0 += YB) {
-        uint32_t from = lane;
-        if constexpr (YB == 1) asm volatile("" : "+v"(from));         // (the queries are read once more, not held)
-        int4_t sum[CG][YB][3];
+        for (int x = 0; x < KL; ++x) fetch_keys(from_k, y, x);
+      }
 #pragma unroll
-        for (int cg = 0; cg < CG; ++cg) {
+      for (int x = 0; x < VL; ++x) fetch_values(from_v, x);
+    }
+    // Each wavefront makes a share of the operands.
 #pragma unroll
-          for (int y = 0; y < YB; ++y) sum[cg][y][0] = sum[cg][y][1] = sum[cg][y][2] = int4_t{0, 0, 0, 0};
-        }
+    for (int cg = 0; cg < CG; ++cg) q_scale[cg] = query_terms<KIND, DP>(raw[cg], D, sh.q[cg], wave, NW);
+    lds_barrier();
+
+    Column col[CG];
+    float4_t o[CG][VL];
 #pragma unroll
-        for (int x = 0; x < KL; ++x) {
+    for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+      for (int x = 0; x < VL; ++x) o[cg][x] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto tile = [&](auto last) {
+      constexpr bool MORE = !decltype(last)::value;
+      const uint32_t first = tile_at(w, i) * TILE;
+      const float k_scale = ks, v_scale = vs;
+      const bool in_pool = known;
+      PageBytes from_k = nullptr, from_v = nullptr;
+      if constexpr (MORE) from_k = keys_at(i + NW, next), from_v = values_at(i + NW, next);
+      float4_t acc[CG][NT];
+      if constexpr (KIND == PageKind::Q8) {
+        constexpr int YB = CG == 2 ? 1 : 2;                            // key operands that share a query operand's way from LDS
+#pragma unroll
+        for (int y0 = 0; y0 < NT; y0 += YB) {
+          uint32_t from = lane;
+          if constexpr (YB == 1) asm volatile("" : "+v"(from));         // (the queries are read once more, not held)
+          int4_t sum[CG][YB][3];
 #pragma unroll
           for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-            for (int n = 0; n < 3; ++n) {
-              const int4_t q = bit_cast<int4_t>(sh.q[cg][3 * x + n][from]);
+            for (int y = 0; y < YB; ++y) sum[cg][y][0] = sum[cg][y][1] = sum[cg][y][2] = int4_t{0, 0, 0, 0};
+          }
 #pragma unroll
-              for (int y = 0; y < YB; ++y) {
-                sum[cg][y][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bit_cast<int4_t>(kr[y0 + y][x]), q, sum[cg][y][n], 0, 0, 0);
+          for (int x = 0; x < KL; ++x) {
+#pragma unroll
+            for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+              for (int n = 0; n < 3; ++n) {
+                const int4_t q = bit_cast<int4_t>(sh.q[cg][3 * x + n][from]);
+#pragma unroll
+                for (int y = 0; y < YB; ++y) {
+                  sum[cg][y][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(bit_cast<int4_t>(kr[y0 + y][x]), q, sum[cg][y][n], 0, 0, 0);
+                }
+              }
+            }
+            if constexpr (MORE) {
+#pragma unroll
+              for (int y = 0; y < YB; ++y) fetch_keys(from_k, y0 + y, x);
+            }
+          }
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+            for (int y = 0; y < YB; ++y) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                // (the lower two together are below 2^31)
+                const float low = static_cast<float>((sum[cg][y][1][e] << 8) + sum[cg][y][0][e]);
+                acc[cg][y0 + y][e] = fmaf(static_cast<float>(sum[cg][y][2][e]), 65536.0f, low);
               }
             }
           }
-          if constexpr (MORE) {
-#pragma unroll
-            for (int y = 0; y < YB; ++y) fetch_keys(from_k, y0 + y, x);
-          }
         }
+      } else {
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-          for (int y = 0; y < YB; ++y) {
+          for (int y = 0; y < NT; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              // (the lower two together are below 2^31)
-              const float low = static_cast<float>((sum[cg][y][1][e] << 8) + sum[cg][y][0][e]);
-              acc[cg][y0 + y][e] = fmaf(static_cast<float>(sum[cg][y][2][e]), 65536.0f, low);
+        for (int x = 0; x < 2 * KL; ++x) {
+          half8_t hi[CG], lo[CG];
+#pragma unroll
+          for (int cg = 0; cg < CG; ++cg) hi[cg] = bit_cast<half8_t>(sh.q[cg][2 * x][lane]), lo[cg] = bit_cast<half8_t>(sh.q[cg][2 * x + 1][lane]);
+#pragma unroll
+          for (int y = 0; y < NT; ++y) {
+            const uint4 run = kr[y][x / 2];
+            const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
+#pragma unroll
+            for (int cg = 0; cg < CG; ++cg) {
+              acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, lo[cg], acc[cg][y], 0, 0, 0);
+              acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, hi[cg], acc[cg][y], 0, 0, 0);
+            }
+            if constexpr (MORE) {
+              if (x % 2 == 1) fetch_keys(from_k, y, x / 2);
             }
           }
         }
       }
-    } else {
+      if constexpr (MORE) {
+        fetch_scales(next);
+        if (i + 2 * NW < end) next = numbers(i + 2 * NW);
+      }
+      // Every column sees every position of the tile, or it goes by bits.
+      const bool all = first + (TILE - 1u) <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
+      half8_t p_hi[CG][OWN / 8], p_lo[CG][OWN / 8];
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
+        float s[OWN], corr;
 #pragma unroll
-        for (int y = 0; y < NT; ++y) acc[cg][y] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      }
+        for (uint32_t e = 0; e < OWN; ++e) s[e] = acc[cg][e / 4][e % 4];
+        bool moves;
+        if (all) {
+          moves = weigh<true>(col[cg], s, q_scale[cg] * k_scale, 0u, v_scale, p_hi[cg], p_lo[cg], &corr);
+        } else {
+          const uint32_t p0 = first + OWN * g;
+          uint32_t shown = 0u;
 #pragma unroll
-      for (int x = 0; x < 2 * KL; ++x) {
-        half8_t hi[CG], lo[CG];
-#pragma unroll
-        for (int cg = 0; cg < CG; ++cg) hi[cg] = bit_cast<half8_t>(sh.q[cg][2 * x][lane]), lo[cg] = bit_cast<half8_t>(sh.q[cg][2 * x + 1][lane]);
-#pragma unroll
-        for (int y = 0; y < NT; ++y) {
-          const uint4 run = kr[y][x / 2];
-          const half8_t key = x % 2 == 0 ? operand<KIND>(run.x, run.y) : operand<KIND>(run.z, run.w);
-#pragma unroll
-          for (int cg = 0; cg < CG; ++cg) {
-            acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, lo[cg], acc[cg][y], 0, 0, 0);
-            acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key, hi[cg], acc[cg][y], 0, 0, 0);
+          for (uint32_t e = 0; e < OWN; ++e) {
+            const uint32_t p = p0 + e;
+            const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & in_pool;
+            shown |= (sees ? 1u : 0u) << e;
           }
-          if constexpr (MORE) {
-            if (x % 2 == 1) fetch_keys(from_k, y, x / 2);
-          }
+          moves = weigh<false>(col[cg], s, q_scale[cg] * k_scale, shown, v_scale, p_hi[cg], p_lo[cg], &corr);
         }
+        if (moves) scale_sums(o[cg], corr);
       }
-    }
-    if constexpr (MORE) {
-      fetch_scales(next);
-      if (i + 2 * NW < end) next = numbers(i + 2 * NW);
-    }
-    // Every column sees every position of the tile, or it goes by bits.
-    const bool all = first + (TILE - 1u) <= w.low && (a.window == 0u || first + a.window > w.high) && __all(in_pool);
-    half8_t p_hi[CG][OWN / 8], p_lo[CG][OWN / 8];
+#pragma unroll
+      for (int x = 0; x < VL; ++x) {
+        half8_t value[OWN / 8];
+        value[0] = operand<KIND>(vr[x].x, vr[x].y);
+        if constexpr (OWN == 16) value[1] = operand<KIND>(vr[x].z, vr[x].w);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg) {
+#pragma unroll
+          for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_lo[cg][n], o[cg][x], 0, 0, 0);
+#pragma unroll
+          for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_hi[cg][n], o[cg][x], 0, 0, 0);
+        }
+        if constexpr (MORE) fetch_values(from_v, x);
+      }
+    };
+    for (; i + NW < end; i += NW) tile(std::false_type{});
+    if (i < end) tile(std::true_type{});
+
+    // Merge of the wavefronts under the largest reference.
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
-      float s[OWN], corr;
+      const float total = groups_sum(col[cg].sum);
+      if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = total;
+    }
+    __syncthreads();                                                  // (no wavefront reads the queries any more)
 #pragma unroll
-      for (uint32_t e = 0; e < OWN; ++e) s[e] = acc[cg][e / 4][e % 4];
-      bool moves;
-      if (all) {
-        moves = weigh<true>(col[cg], s, q_scale[cg] * k_scale, 0u, v_scale, p_hi[cg], p_lo[cg], &corr);
+    for (int cg = 0; cg < CG; ++cg) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][cg * 16u + r]);
+      const float factor = __builtin_amdgcn_exp2f(col[cg].ref - from_reference(top)) / col[cg].up;
+#pragma unroll
+      for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * factor;
+    }
+    __syncthreads();
+    const bool whole = begin == 0u && end == w.tiles;                 // no other part has tiles
+    slot *= a.stored;
+    for (uint32_t e = t; e < w.columns * (D / 4u); e += NW * 64u) {
+      const uint32_t c = e / (D / 4u), d = e % (D / 4u) * 4u;
+      float top = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][c]);
+      float total = 0.0f;
+      float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int n = 0; n < NW; ++n) {
+        total = fmaf(__builtin_amdgcn_exp2f(sh.ref[n][c] - from_reference(top)), sh.sum[n][c], total);
+        x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]);
+      }
+      if (whole) {
+        const uint32_t pair = c;
+        float* to = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
+        *reinterpret_cast<float4_t*>(to) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
       } else {
-        const uint32_t p0 = first + OWN * g;
-        uint32_t shown = 0u;
-#pragma unroll
-        for (uint32_t e = 0; e < OWN; ++e) {
-          const uint32_t p = p0 + e;
-          const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & in_pool;
-          shown |= (sees ? 1u : 0u) << e;
-        }
-        moves = weigh<false>(col[cg], s, q_scale[cg] * k_scale, shown, v_scale, p_hi[cg], p_lo[cg], &corr);
+        *reinterpret_cast<float4_t*>(a.part_sum + (slot + c) * D + d) = x;
+        if (d == 0u) a.part_most[slot + c] = top, a.part_total[slot + c] = total;
       }
-      if (moves) scale_sums(o[cg], corr);
     }
-#pragma unroll
-    for (int x = 0; x < VL; ++x) {
-      half8_t value[OWN / 8];
-      value[0] = operand<KIND>(vr[x].x, vr[x].y);
-      if constexpr (OWN == 16) value[1] = operand<KIND>(vr[x].z, vr[x].w);
-#pragma unroll
-      for (int cg = 0; cg < CG; ++cg) {
-#pragma unroll
-        for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_lo[cg][n], o[cg][x], 0, 0, 0);
-#pragma unroll
-        for (uint32_t n = 0; n < OWN / 8; ++n) o[cg][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[n], p_hi[cg][n], o[cg][x], 0, 0, 0);
-      }
-      if constexpr (MORE) fetch_values(from_v, x);
-    }
-  };
-  for (; i + NW < end; i += NW) tile(std::false_type{});
-  if (i < end) tile(std::true_type{});
-
-  // Merge of the wavefronts under the largest reference.
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const float total = groups_sum(col[cg].sum);
-    if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = total;
-  }
-  __syncthreads();                                                  // (no wavefront reads the queries any more)
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][cg * 16u + r]);
-    const float factor = __builtin_amdgcn_exp2f(col[cg].ref - from_reference(top)) / col[cg].up;
-#pragma unroll
-    for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * factor;
-  }
-  __syncthreads();
-  const bool whole = begin == 0u && end == w.tiles;                 // no other part has tiles
-  slot *= a.stored;
-  for (uint32_t e = t; e < w.columns * (D / 4u); e += NW * 64u) {
-    const uint32_t c = e / (D / 4u), d = e % (D / 4u) * 4u;
-    float top = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][c]);
-    float total = 0.0f;
-    float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int n = 0; n < NW; ++n) {
-      total = fmaf(__builtin_amdgcn_exp2f(sh.ref[n][c] - from_reference(top)), sh.sum[n][c], total);
-      x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]);
-    }
-    if (whole) {
-      const uint32_t pair = c;
-      float* to = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
-      *reinterpret_cast<float4_t*>(to) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
-    } else {
-      *reinterpret_cast<float4_t*>(a.part_sum + (slot + c) * D + d) = x;
-      if (d == 0u) a.part_most[slot + c] = top, a.part_total[slot + c] = total;
-    }
-  }
-  lds_barrier();                                                    // the next run's queries go where these sums are
+    lds_barrier();                                                    // the next run's queries go where these sums are
   }
 }
 
@@ -671,21 +683,21 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
   const uint64_t page_bytes = static_cast<uint64_t>(b.kv_heads) * block * D;
   auto key_run = [&](int x) { return (WAVES / 4u) * x + wave / 4u; };
   auto fetch_keys = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.k < b.pages ? n.k : 0u, at = (tile_at(w, i < end ? i : end - 1u) * 64u + (r >> 2) * 16u) & (block - 1u);
-    const uint8_t* from = a.k + page * page_bytes + (kv * block + at + (r & 3u) + 4u * (wave & 3u)) * D;
+    const uint32_t at = (tile_at(w, i < end ? i : end - 1u) * 64u + (r >> 2) * 16u) & (block - 1u);
+    const PageBytes from = page_bytes_of(a.k, n.k < b.pages, n.k * page_bytes + kv * block * D) + (at + (r & 3u) + 4u * (wave & 3u)) * D;
 #pragma unroll
     for (int x = 0; x < KOWN; ++x) {
       const uint32_t d = 64u * key_run(x) + 16u * g;
-      kr[x] = load_u4(from + (d < D ? d : 0u));
+      kr[x] = load_page<uint4>(from + (d < D ? d : 0u));
     }
   };
   auto fetch_values = [&](uint32_t i, const Numbers& n) {
-    const uint32_t page = n.v < b.pages ? n.v : 0u, at = (tile_at(w, i < end ? i : end - 1u) * 64u + g * 16u) & (block - 1u);
-    const uint8_t* from = a.v + page * page_bytes + static_cast<uint64_t>(kv) * block * D + at;
+    const uint32_t at = (tile_at(w, i < end ? i : end - 1u) * 64u + g * 16u) & (block - 1u);
+    const PageBytes from = page_bytes_of(a.v, n.v < b.pages, n.v * page_bytes + kv * block * D) + at;
 #pragma unroll
     for (int x = 0; x < VOWN; ++x) {
       const uint32_t d = 16u * (WAVES * x + wave) + r;
-      vr[x] = load_u4(from + (d < D ? d : r) * block);
+      vr[x] = load_page<uint4>(from + (d < D ? d : r) * block);
     }
   };
   auto fetch_scales = [&](const Numbers& n) {

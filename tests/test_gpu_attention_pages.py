@@ -156,6 +156,20 @@ def test_unknown_pages(backend, window, sinks, rows):
     assert np.all(got[rows:2 * rows] == 0.0)
 
 
+@pytest.mark.parametrize("rows,past,d", [(1, 160, 64), (1, 5000, 128), (5, 900, 256), (40, 200, 96)])
+def test_unknown_pages_beside_codes_of_nan(backend, rows, past, d):
+    """What is walked in place of an unknown page is no page of the pool: there may be anything in those that no table names."""
+    kv, group, block = 2, 4, 16
+    b = Batch(backend, 44, "fp8", kv, block, d, [past + rows, 70 + rows])
+    unused = np.setdiff1d(np.arange(b.pool.pages), np.concatenate([b.table[s, :-(-int(n) // block)] for s, n in enumerate(b.lens)]))
+    assert len(unused)
+    b.table[b.table == 0], b.pool.kp[0], b.pool.vp[0] = unused[0], 0x7F, 0xFF
+    b.table[0, [0, 3, -(-past // block) - 1]] = [b.pool.pages, 0xFFFFFFFF, 0x80000000]
+    b.table[1, 2] = b.pool.pages + 5
+    b.upload()
+    check(b, queries(b.rs, 2 * rows, kv * group * d), [rows] * 2, group)
+
+
 @pytest.mark.parametrize("rows", [1, 4, 40])
 def test_not_finite_where_hidden(backend, rows):
     """Pages that are NaN, where no row sees them, or some: others' results are as if they were zeros."""
