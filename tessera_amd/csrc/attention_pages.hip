@@ -203,12 +203,9 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
 // ---- an even split -------------------------------------------------------------------------------
 //
 // Of units that are a sequence each: all their tiles, a sequence's heads one behind the other, in runs of equal cost, one a workgroup.
-// To begin a head costs what kBegin tiles do: so many lie before its first, with nothing in them (2, 4, 6, 9, 12 of them: 35.4, 33.4, 31.2,
-// 33.7, 36.4 us for windows of 4096 in 8 sequences, and within 2 % for 48 sequences of all lengths).  A run that covers a head whole
-// gives its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second
-// those of a later one.
-constexpr uint32_t kBegin = 6;                                      // of 64 positions
-__host__ __device__ constexpr uint32_t begin_tiles(uint32_t log_tile) { return kBegin << (6u - log_tile); }
+// To begin a head costs what begin_tiles do: so many lie before its first, with nothing in them.  A run that covers a head whole gives
+// its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second those of
+// a later one.
 __device__ __forceinline__ uint32_t even_of(const PageAttention& a, const PageSequence& seq) {
   return seq.rows == 0u ? 0u : sequence_tiles(a, seq).tiles + begin_tiles(a.log_tile);
 }
@@ -240,8 +237,6 @@ __device__ __forceinline__ uint32_t even_share(const PageAttention& a, uint32_t 
 // 48 sequences of up to 8000 positions, 24 heads over 4 of 256, int8, 395 MB: 82 us, 4.8 TB/s; 5 rows on 65000, 32 over 8 of 128, E4M3, 133 MB:
 // 33 us, of which 5 pass until the first tile is there and 4 until the last workgroup has begun; 1 row on 1187, 16 over 4 of 64: 9 us,
 // of which 2.2 go by before the sequence is found, 2 before its tiles are there, 1.5 a tile for the longest wavefront.
-// Positions of a tile: 64, or 32 where a tile's codes and the sums together are more registers than two wavefronts a SIMD have.
-constexpr uint32_t few_tile(uint64_t head_dim, uint64_t columns) { return head_dim <= 128 && columns == 16 ? 64 : 32; }
 constexpr int query_operands(PageKind kind, int dp) { return kind == PageKind::Q8 ? 3 * (dp / 64) : 2 * (dp / 32); }
 
 template <PageKind KIND, int DP, int CG, int NW>
@@ -333,7 +328,7 @@ typedef int int4_t __attribute__((ext_vector_type(4)));
 template <PageKind KIND, int DP, int CG, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAttention a) {
   constexpr int KL = DP / 64, VL = DP / 16, C = 16 * CG;
-  constexpr uint32_t TILE = few_tile(DP, C), OWN = TILE / 4;      // positions of a tile, and of a lane's
+  constexpr uint32_t TILE = 1u << pages_log_tile(DP, C), OWN = TILE / 4;      // positions of a tile, and of a lane's
   constexpr int NT = TILE / 16;                                     // key operands
   __shared__ FewShared<KIND, DP, CG, NW> sh;
   const PageBatch& b = a.batch;
@@ -353,7 +348,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
       if (at_tile >= last_tile || !find_unit(b, at_tile, [&](const PageSequence& q) { return even_of(a, q) * b.kv_heads; }, &u)) return;
       const uint32_t in = u.at;
       w = sequence_tiles(a, u.seq);
-      constexpr uint32_t EMPTY = kBegin * (64u / TILE);
+      constexpr uint32_t EMPTY = begin_tiles(TILE == 32 ? 5 : 6);
       const uint32_t wide = w.tiles + EMPTY, from = in % wide, left = last_tile - at_tile, to = wide - from < left ? wide : from + left;
       kv = in / wide;
       if (to <= EMPTY) return;                                       // (the next workgroup begins it)
@@ -920,7 +915,6 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 // ---- the parts' merge ----------------------------------------------------------------------------
 
 // A workgroup a column: its parts' sums under the largest of their references, the first parts' loads under way at once.
-constexpr uint32_t kPagePartsMost = 1024;
 template <int C>
 __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttention a) {
   __shared__ float of_wave[2][4], weight[kPagePartsMost];
@@ -994,67 +988,14 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   *reinterpret_cast<float4_t*>(out) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
 }
 
-uint64_t units_of(const PageAttentionCall& c, uint64_t columns) {
-  const uint64_t group = c.heads / c.page.kv_heads;
-  const uint64_t some = c.page.rows * group / columns + c.page.sequences, each = c.page.sequences * ((c.max_rows * group + columns - 1) / columns);
-  return some < each ? some : each;
-}
-
 }  // namespace
 
-// Positions of a tile, and tiles that a unit walks at most.
-static uint32_t log_tile_of(const PageAttentionCall& c, uint64_t columns) {
-  return columns < 64 && few_tile(c.page.head_dim, columns) == 32 ? 5u : 6u;
+static PagesCall sizes_of(const PageAttentionCall& c) {
+  return PagesCall{c.page.rows, c.page.sequences, c.heads / c.page.kv_heads, c.page.kv_heads, c.page.head_dim, c.max_rows, c.max_len, c.window, c.sinks};
 }
-static uint64_t tiles_of(const PageAttentionCall& c, uint64_t columns) {
-  const uint64_t tile = uint64_t{1} << log_tile_of(c, columns), all = (c.max_len + tile - 1) / tile;
-  if (c.window == 0) return all;
-  const uint64_t some = (c.sinks + tile - 1) / tile + (c.window + c.max_rows + tile - 1) / tile + 1;
-  return some < all ? some : all;
-}
-
-// Columns of a unit that can be there.
-static uint64_t stored_of(const PageAttentionCall& c, uint64_t columns) {
-  const uint64_t pairs = c.max_rows * (c.heads / c.page.kv_heads);
-  return pairs < columns ? pairs : columns;
-}
-
-size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape& shape) {
-  const uint64_t places = shape.even != 0 ? 2 * shape.even : shape.parts < 2 ? 0 : units_of(c, shape.columns) * c.page.kv_heads * shape.parts;
-  return static_cast<size_t>(places * stored_of(c, shape.columns) * (c.page.head_dim + 2) * 4);
-}
-
-// Few columns: one workgroup a head of a sequence, or parts of four tiles where all of those are on the chip at once, or an even split.
-// A split costs the merge and its launch, each of its runs a start; one workgroup has the longest sequence's time.  us, one
-// workgroup / parts: a sequence of 4 heads of 64, 500 positions 7.3 / 11.3, 1500 11.0 / 11.4, 2000 13 / 12; 8 heads of 128, 400 10.4 / 13.2,
-// 1000 13.7 / 13.2; 4 heads of 256, 250 11.8 / 14.0, 500 14.9 / 14.0.  One / even split, sequences of all lengths up to the stated one: 40
-// of 8 heads of 128, 2000 29 / 32, 3000 51 / 41, 128 of them, 3000 92 / 99, 5000 142 / 141, 8000 215 / 205; 48 of 4 heads of 256, 1500
-// 27 / 31, 3000 52 / 46, 8000 124 / 88, 200 of them, 3000 147 / 151, 5000 225 / 211.
-// Many columns: parts only where the units are fewer than two a CU.
+size_t attention_pages_parts_bytes(const PageAttentionCall& c, const PagesShape& shape) { return pages_bytes(sizes_of(c), shape); }
 PagesShape attention_pages_shape(const PageAttentionCall& c, bool in_parts) {
-  const uint64_t D = c.page.head_dim, pairs = c.max_rows * (c.heads / c.page.kv_heads), columns = pairs <= 16 ? 16 : pairs <= 32 && D <= 128 ? 32 : 64;
-  const uint64_t tiles = tiles_of(c, columns), cus = static_cast<uint64_t>(num_cus()), groups = units_of(c, columns) * c.page.kv_heads;
-  const uint64_t resident = 2 * cus, log_tile = log_tile_of(c, columns);
-  const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus ? 8u : 4u};
-  if (!in_parts || groups * stored_of(c, columns) >= (1u << 24)) return one;      // (the merge's grid has a workgroup a column: fewer than 2^32 threads)
-  if (columns < 64) {
-    const uint64_t parts = (tiles + 3) / 4, of_64 = tiles >> (6 - log_tile);
-    const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident < kPagePartsMost ? resident : kPagePartsMost, 4};
-    if (groups * parts <= resident) {
-      return parts < 2 || of_64 <= (D <= 64 ? 24 : D <= 128 ? 12 : 6) || attention_pages_parts_bytes(c, each) > kAttentionPartsMost ? one : each;
-    }
-    if (of_64 <= 32 || of_64 <= 38 * groups / resident) return one;
-    return c.page.sequences * c.page.kv_heads * (tiles + begin_tiles(5)) < (1u << 30) && attention_pages_parts_bytes(c, even) <= kAttentionPartsMost ? even : one;
-  }
-  uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
-  if (parts > 256) parts = 256;
-  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
-  for (; parts > 1; --parts) {
-    const uint64_t each = (tiles + parts - 1) / parts;
-    const PagesShape shape{columns, (tiles + each - 1) / each, each, 0, 4};
-    if (attention_pages_parts_bytes(c, shape) <= kAttentionPartsMost) return shape;
-  }
-  return one;
+  return pages_rule(sizes_of(c), static_cast<uint64_t>(num_cus()), in_parts ? kAttentionPartsMost : 0);
 }
 
 hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const PagesShape& shape, const float* q, const uint8_t* k, const uint8_t* v,
@@ -1069,8 +1010,8 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   a.window = c.window >= c.max_len ? 0u : static_cast<uint32_t>(c.window);
   a.sinks = static_cast<uint32_t>(c.sinks < c.max_len ? c.sinks : c.max_len);
   a.parts = static_cast<uint32_t>(shape.parts), a.part_tiles = static_cast<uint32_t>(shape.part_tiles);
-  a.stored = static_cast<uint32_t>(stored_of(c, shape.columns)), a.log_tile = log_tile_of(c, shape.columns);
-  const uint64_t groups = units_of(c, shape.columns) * c.page.kv_heads;
+  a.stored = static_cast<uint32_t>(pages_stored(sizes_of(c), shape.columns)), a.log_tile = pages_log_tile(c.page.head_dim, shape.columns);
+  const uint64_t groups = pages_units(sizes_of(c), shape.columns) * c.page.kv_heads;
   a.even = static_cast<uint32_t>(shape.even);
   const bool split = shape.parts > 1 || shape.even != 0;
   if (split) {

@@ -329,11 +329,75 @@ constexpr LogprobPlan logprob_plan(uint64_t rows, uint64_t vocab, uint64_t top_k
 }
 
 // ---- "attention_pages" -----------------------------------------------------------------------------------------------
+// A unit is `columns` (row, head) pairs of a key head in a sequence: one unit a sequence where 16 or 32 hold all, else 64 each.
+struct PagesCall {
+  uint64_t rows, sequences, group, kv_heads, head_dim, max_rows, max_len, window, sinks;      // group: queries' heads to a key head
+};
 struct PagesShape {
-  uint64_t columns, parts, part_tiles;                        // (row, head) pairs a workgroup; parts of the positions, tiles of 64 each
+  uint64_t columns, parts, part_tiles;                        // parts of a unit's positions, tiles each
   uint64_t even;                                              // workgroups that share all tiles evenly; 0: a workgroup a part
   uint64_t waves;                                             // wavefronts a workgroup, where columns are few
 };
+constexpr uint32_t kPagePartsMost = 1024;                     // that the merge takes
+// Positions of a tile, as a power of two: 64, or 32 where a tile's codes and the sums are more registers together than a
+// wavefront has with another on its SIMD (heads of 256, as the register limit has it: 48 sequences 91 us with 64 and one
+// wavefront, 88 with 32 and two).
+constexpr uint32_t pages_log_tile(uint64_t head_dim, uint64_t columns) {
+  return columns >= 64 || (columns == 16 && head_dim <= 128) ? 6 : 5;
+}
+// To begin a head in an even split costs what so many tiles do (of 64 positions 2, 4, 6, 9, 12: 35.4, 33.4, 31.2, 33.7, 36.4
+// us for windows of 4096 in 8 sequences of 8 heads, and within 2 % for 48 sequences of all lengths).
+constexpr uint32_t begin_tiles(uint32_t log_tile) { return 6u << (6u - log_tile); }
+constexpr uint64_t pages_units(const PagesCall& c, uint64_t columns) {
+  const uint64_t of_row = (c.group + columns - 1) / columns, of_sequence = (c.max_rows * c.group + columns - 1) / columns;
+  uint64_t most = c.rows * c.group / columns + c.sequences;
+  for (const uint64_t other : {c.rows * of_row, c.sequences * of_sequence}) most = other < most ? other : most;
+  return most;
+}
+// Columns of a unit that can be there; tiles that it walks at most.
+constexpr uint64_t pages_stored(const PagesCall& c, uint64_t columns) { return c.max_rows * c.group < columns ? c.max_rows * c.group : columns; }
+constexpr uint64_t pages_tiles(const PagesCall& c, uint64_t columns) {
+  const uint64_t tile = uint64_t{1} << pages_log_tile(c.head_dim, columns), all = (c.max_len + tile - 1) / tile;
+  const uint64_t some = (c.sinks + tile - 1) / tile + (c.window + c.max_rows + tile - 1) / tile + 1;
+  return c.window == 0 || all < some ? all : some;
+}
+// What the parts leave for the merge: for each column its sums, their reference and the weights' sum.
+constexpr size_t pages_bytes(const PagesCall& c, const PagesShape& shape) {
+  const uint64_t places = shape.even != 0 ? 2 * shape.even : shape.parts < 2 ? 0 : pages_units(c, shape.columns) * c.kv_heads * shape.parts;
+  return static_cast<size_t>(places * pages_stored(c, shape.columns) * (c.head_dim + 2) * 4);
+}
+// Few columns: one workgroup a head of a sequence, or parts of four tiles where all of those are on the chip at once, or an
+// even split.  A split costs the merge and its launch, each of its runs a start; one workgroup has the longest sequence's time.
+// us, one workgroup / parts: a sequence of 4 heads of 64, 500 positions 7.3 / 11.3, 1500 11.0 / 11.4, 2000 13 / 12; 8 heads of
+// 128, 400 10.4 / 13.2, 1000 13.7 / 13.2; 4 heads of 256, 250 11.8 / 14.0, 500 14.9 / 14.0.  One / even split, sequences of all
+// lengths up to the stated one: 40 of 8 heads of 128, 2000 29 / 32, 3000 51 / 41; 128 of them, 3000 92 / 99, 5000 142 / 141, 8000
+// 215 / 205; 48 of 4 heads of 256, 1500 27 / 31, 3000 52 / 46, 8000 124 / 88; 200 of them, 3000 147 / 151, 5000 225 / 211.
+// Many columns: parts only where the units are fewer than two a CU.  (`most`: bytes that the parts may take.)
+constexpr PagesShape pages_rule(const PagesCall& c, uint64_t cus, size_t most) {
+  const uint64_t pairs = c.max_rows * c.group, columns = pairs <= 16 ? 16 : pairs <= 32 && c.head_dim <= 128 ? 32 : 64;
+  const uint64_t tiles = pages_tiles(c, columns), groups = pages_units(c, columns) * c.kv_heads, log_tile = pages_log_tile(c.head_dim, columns);
+  const uint64_t resident = 2 * cus < kPagePartsMost ? 2 * cus : kPagePartsMost;
+  const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus ? 8u : 4u};
+  if (groups * pages_stored(c, columns) >= (1u << 24)) return one;      // (the merge has a workgroup a column: a grid of fewer than 2^32 threads)
+  if (columns < 64) {
+    const uint64_t parts = (tiles + 3) / 4, of_64 = tiles >> (6 - log_tile);
+    const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident, 4};
+    if (groups * parts <= resident) {
+      return parts < 2 || of_64 <= (c.head_dim <= 64 ? 24 : c.head_dim <= 128 ? 12 : 6) || pages_bytes(c, each) > most ? one : each;
+    }
+    if (of_64 <= 32 || of_64 <= 38 * groups / resident) return one;
+    return c.sequences * c.kv_heads * (tiles + begin_tiles(5)) < (1u << 30) && pages_bytes(c, even) <= most ? even : one;      // (32-bit sums)
+  }
+  uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
+  if (parts > 256) parts = 256;
+  if (parts > (tiles + 3) / 4) parts = (tiles + 3) / 4;
+  for (; parts > 1; --parts) {
+    const uint64_t each = (tiles + parts - 1) / parts;
+    const PagesShape shape{columns, (tiles + each - 1) / each, each, 0, 4};
+    if (shape.parts > 1 && pages_bytes(c, shape) <= most) return shape;
+  }
+  return one;
+}
 
 // ---- "attention_combine" ---------------------------------------------------------------------------------------------
 // Wavefronts of a (row, head): sixteen where there are few and many parts, four where the rows fill the chip by themselves or
