@@ -228,7 +228,7 @@ __device__ __forceinline__ bool sequence_rows(const DraftArgs& a, uint32_t s, ui
   return begin < end && end <= a.rows;
 }
 // Row `at` of a sequence, by a wavefront, from its chunks' statistics; `draft` those of the draft's row, unless `of_draft` is `known`.
-__device__ __forceinline__ Verdict judge(const DraftArgs& a, const ChunkStats* target, const ChunkStats* draft, uint32_t first, uint32_t rows, uint32_t at,
+__device__ __forceinline__ Verdict verdict_of(const DraftArgs& a, const ChunkStats* target, const ChunkStats* draft, uint32_t first, uint32_t rows, uint32_t at,
                                          bool known, RowStats of_draft) {
   Verdict v;
   v.draft = of_draft;
@@ -394,7 +394,7 @@ __device__ __forceinline__ Verdict find_end(const DraftArgs& a, uint32_t first, 
     __syncthreads();
     if (base + wave < rows) {
       const uint64_t at = static_cast<uint64_t>(first + base + wave) * a.chunks;
-      const Verdict v = judge(a, a.stats + at, a.stats + static_cast<uint64_t>(a.rows) * a.chunks + at, first, rows, base + wave, false, RowStats{0.0, 0.0f, 0u});
+      const Verdict v = verdict_of(a, a.stats + at, a.stats + static_cast<uint64_t>(a.rows) * a.chunks + at, first, rows, base + wave, false, RowStats{0.0, 0.0f, 0u});
       if (lane == 0u) sh.of[wave] = v;
     } else if (lane == 0u) {
       sh.of[wave].is = 0u;
@@ -461,7 +461,7 @@ __global__ __launch_bounds__(kThreads) void draft_alone_kernel(DraftArgs a) {
       draft = row_stats(hold(sh.stats, a.chunks, 0u), sh.stats, a.chunks, a.draft_scale);
     }
     gather(a.logits, first + at, a.scale);
-    v = judge(a, sh.stats, nullptr, first, rows, at, true, draft);
+    v = verdict_of(a, sh.stats, nullptr, first, rows, at, true, draft);
   }
   if (a.draft != nullptr && (v.is & kRefused) != 0u) {
     for (uint32_t c = wave; c < a.chunks; c += kWaves) {
