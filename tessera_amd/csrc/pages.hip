@@ -42,7 +42,7 @@ __device__ __forceinline__ float decode(uint32_t four, int i) {
 struct PageWork {
   PageUnit unit;
   uint32_t kv, page, from, to, first_row;   // first_row: the call's row at place `from`
-  bool values, held;                        // held: the page's number is one of the pool's
+  bool values;
 };
 __device__ __forceinline__ bool page_work(const PageBatch& b, PageWork* w) {
   const uint32_t which = blockIdx.x % (2u * b.kv_heads);
@@ -53,8 +53,10 @@ __device__ __forceinline__ bool page_work(const PageBatch& b, PageWork* w) {
   w->from = past > base ? past - base : 0u;
   w->to = q.len - base < block ? q.len - base : block;
   w->first_row = q.first + (base + w->from - past);
-  w->page = b.table[static_cast<uint64_t>(w->unit.s) * b.width + slot];
-  w->held = w->page < b.pages;
+  // (a vector load, so that what comes before its use is not kept waiting as by a scalar one)
+  uint32_t here = 0u;
+  asm("" : "+v"(here));
+  w->page = b.table[static_cast<uint64_t>(w->unit.s) * b.width + slot + here];
   return true;
 }
 
@@ -70,14 +72,10 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
                                                                    uint64_t v_stride, uint8_t* kp, uint8_t* vp, float* ks, float* vs) {
   __shared__ uint32_t most_of[kPageThreads / 64];
   PageWork w;
-  if (!page_work(b, &w) || !w.held) return;               // workgroup-uniform
+  if (!page_work(b, &w)) return;                          // workgroup-uniform
   const uint32_t t = threadIdx.x, D = b.head_dim, block = 1u << b.log_block, runs = D / 16u;
   const uint64_t stride = w.values ? v_stride : k_stride;
   const float* rows = (w.values ? v : k) + static_cast<uint64_t>(w.first_row) * stride + w.kv * D;   // of place `from`
-  const uint64_t head = static_cast<uint64_t>(w.page) * b.kv_heads + w.kv;
-  float* scale_at = (w.values ? vs : ks) + head;
-  uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
-  const float before = w.from == 0u ? 0.0f : *scale_at;
 
   // A thread's n-th run: of a key's elements d .. d + 15 at `place`, or of an element d at places place .. place + 15.
   const uint32_t count = block * runs, of_row = (1u << 20) / (w.values ? D : runs) + 1u;      // (i < 2048 is divided by its product)
@@ -97,7 +95,7 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) x[n][e] = 0.0f;
     if (!w.values) {
-      if (r.i < count && r.place >= w.from && r.place < w.to) {
+      if (r.i < count && r.place - w.from < rows_here) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const float4 four = *reinterpret_cast<const float4*>(rows + (r.place - w.from) * stride + r.d + e);
@@ -114,6 +112,16 @@ __global__ __launch_bounds__(kPageThreads) void pages_write_kernel(PageBatch b, 
 #pragma unroll
       for (uint32_t e = 0; e < 16u; ++e) x[n][e] = r.place + e - w.from < rows_here ? x[n][e] : 0.0f;
     }
+  }
+  // (the page's number is asked for before the rows and looked at behind them)
+  const uint32_t page = __builtin_amdgcn_readfirstlane(w.page);
+  if (page >= b.pages) return;                             // workgroup-uniform
+  const uint64_t head = static_cast<uint64_t>(page) * b.kv_heads + w.kv;
+  float* scale_at = (w.values ? vs : ks) + head;
+  uint8_t* codes = (w.values ? vp : kp) + head * (static_cast<uint64_t>(block) * D);
+  const float before = w.from == 0u ? 0.0f : *scale_at;
+#pragma unroll
+  for (int n = 0; n < ITEMS; ++n) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) most = max(most, bit_cast<uint32_t>(x[n][e]) & 0x7FFFFFFFu);
   }
