@@ -625,23 +625,24 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
 // The tile's operands lie in LDS, made once for all columns: keys' as few_kernel's (int8 codes as they are), values' as fp16,
 // each operand's 64 lanes side by side, so that every write and read is whole lines.  While a tile is multiplied the next one goes to the
 // other half of the LDS and the one after that is under way.
-template <PageKind KIND, int DP>
+template <PageKind KIND, int DP, int HALVES>
 struct TileShared {
   static constexpr int KEYS = (KIND == PageKind::Q8 ? 4 : 8) * (DP / 64), VALUES = 2 * (DP / 16);   // operands of a tile
   static constexpr int QUERIES = query_operands(KIND, DP);
   union {
     uint4 stage[2][KEYS + VALUES][64];
-    uint4 q[4][QUERIES][64];                                        // of four groups of 16 columns, before the first tile
-    float4_t o[4][DP / 16][64];                                     // of the second half, behind the last
+    uint4 q[8 / HALVES][QUERIES][64];                               // of groups of 16 columns, before the first tile
+    float4_t o[4][DP / 16][HALVES == 2 ? 64 : 1];                   // of the second half, behind the last
   };
-  float scale[64], ref[2][64], sum[2][64];
+  float scale[128 / HALVES], ref[HALVES][128 / HALVES], sum[HALVES][128 / HALVES];
 };
 
-template <PageKind KIND, int DP, int CG>
+template <PageKind KIND, int DP, int CG, int HALVES>
 __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageAttention a) {
-  constexpr int KL = DP / 64, VL = DP / 16, C = 64, WAVES = 8 / CG, GROUPS = 4 / CG;
+  constexpr int KL = DP / 64, VL = DP / 16, C = 128 / HALVES, WAVES = 8 / CG, GROUPS = WAVES / HALVES;
+  constexpr int OWN = 16 / HALVES, NT = 4 / HALVES, SETS = C / 16;  // places of a tile that are a lane's; key operands; groups of 16 columns
   constexpr int KOWN = 4 * KL / WAVES, VOWN = VL / WAVES;           // a thread's runs of a tile
-  using Shared = TileShared<KIND, DP>;
+  using Shared = TileShared<KIND, DP, HALVES>;
   __shared__ Shared sh;
   const PageBatch& b = a.batch;
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = __builtin_amdgcn_readfirstlane(t >> 6), r = lane & 15u, g = lane >> 4;
@@ -727,10 +728,10 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
     return col / a.group;
   };
   {
-    const uint32_t own = wave & 3u, at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
+    const uint32_t own = wave % SETS, at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
     float raw[DP / 64][16];
     query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw);
-    const float scale = query_terms<KIND, DP>(raw, D, sh.q[own], wave / 4u, WAVES / 4u);
+    const float scale = query_terms<KIND, DP>(raw, D, sh.q[own], wave / SETS, WAVES / SETS);
     if (g == 0u) sh.scale[own * 16u + r] = scale;
   }
   lds_barrier();
@@ -766,22 +767,22 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
     const Scales after = fetch_scales(next);
     const Numbers further = numbers(i + 3u);
     // Scores of the key operands 2 half, 2 half + 1.
-    float s[CG][8];
+    float s[CG][OWN];
     if constexpr (KIND == PageKind::Q8) {
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < NT; ++y) {
         int4_t sum[CG][3];
 #pragma unroll
         for (int cg = 0; cg < CG; ++cg) sum[cg][0] = sum[cg][1] = sum[cg][2] = int4_t{0, 0, 0, 0};
 #pragma unroll
         for (int x = 0; x < KL; ++x) {
-          const int4_t key = bit_cast<int4_t>(sh.stage[buf][(2u * half + y) * KL + x][lane]);
+          const int4_t key = bit_cast<int4_t>(sh.stage[buf][(NT * half + y) * KL + x][lane]);
 #pragma unroll
           for (int n = 0; n < 3; ++n) {
 #pragma unroll
             for (int cg = 0; cg < CG; ++cg) sum[cg][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(key, bit_cast<int4_t>(q[cg][3 * x + n]), sum[cg][n], 0, 0, 0);
           }
-          constexpr int EACH = 2 * KL / KOWN;
+          constexpr int EACH = NT * KL / KOWN;
           if ((KL * y + x) % EACH == EACH - 1) stash_keys(buf ^ 1u, (KL * y + x) / EACH);
         }
 #pragma unroll
@@ -793,18 +794,18 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
         }
       }
     } else {
-      float4_t acc[CG][2];
+      float4_t acc[CG][NT];
 #pragma unroll
-      for (int cg = 0; cg < CG; ++cg) acc[cg][0] = acc[cg][1] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int y = 0; y < CG * NT; ++y) acc[y / NT][y % NT] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int x = 0; x < 2 * KL; ++x) {
-        half8_t key[2];
+        half8_t key[NT];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) key[y] = bit_cast<half8_t>(sh.stage[buf][(2u * half + y) * (2 * KL) + x][lane]);
+        for (int y = 0; y < NT; ++y) key[y] = bit_cast<half8_t>(sh.stage[buf][(NT * half + y) * (2 * KL) + x][lane]);
 #pragma unroll
         for (int term = 1; term >= 0; --term) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
+          for (int y = 0; y < NT; ++y) {
 #pragma unroll
             for (int cg = 0; cg < CG; ++cg) acc[cg][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(key[y], bit_cast<half8_t>(q[cg][2 * x + term]), acc[cg][y], 0, 0, 0);
           }
@@ -814,21 +815,23 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 #pragma unroll
       for (int cg = 0; cg < CG; ++cg) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[cg][e] = acc[cg][e / 4][e % 4];
+        for (int e = 0; e < OWN; ++e) s[cg][e] = acc[cg][e / 4][e % 4];
       }
     }
     fetch_keys(i + 2u, next);
     // The first values' operands are on their way while the weights are formed.  (Not where that costs the third wavefront a SIMD.)
     constexpr bool EARLY = DP > 64;
-    constexpr int EACH = 4 / CG;
+    constexpr int EACH = 4 / CG, STEPS = 2 * VL / HALVES / EACH;    // value operands of a step
     half8_t ahead[EACH];
-    auto read_values = [&](int x) {
+    auto element = [](int step) { return HALVES == 2 ? step * EACH : step / 2 * EACH; };      // its first set of sixteen elements
+    auto read_values = [&](int step) {
+      const uint32_t eights = HALVES == 2 ? half : static_cast<uint32_t>(step) % 2u;          // of the places
 #pragma unroll
-      for (int y = 0; y < EACH; ++y) ahead[y] = bit_cast<half8_t>(sh.stage[buf][Shared::KEYS + 2 * (x + y) + half][lane]);
+      for (int y = 0; y < EACH; ++y) ahead[y] = bit_cast<half8_t>(sh.stage[buf][Shared::KEYS + 2 * (element(step) + y) + eights][lane]);
     };
     if constexpr (EARLY) read_values(0);
     const bool all = first + 63u <= w.low && (a.window == 0u || first + a.window > w.high) && __all(scales.known != 0u);
-    half8_t p_hi[CG][1], p_lo[CG][1];
+    half8_t p_hi[CG][OWN / 8], p_lo[CG][OWN / 8];
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
       float corr;
@@ -836,10 +839,10 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       if (all) {
         moves = weigh<true>(col[cg], s[cg], q_scale[cg] * scales.k, 0u, scales.v, p_hi[cg], p_lo[cg], &corr);
       } else {
-        const uint32_t p0 = first + 16u * g + 8u * half;
+        const uint32_t p0 = first + 16u * g + OWN * half;
         uint32_t shown = 0u;
 #pragma unroll
-        for (uint32_t e = 0; e < 8u; ++e) {
+        for (uint32_t e = 0; e < OWN; ++e) {
           const uint32_t p = p0 + e;
           const bool sees = (p <= pos[cg]) & ((a.window == 0u) | (pos[cg] - p < a.window) | (p < a.sinks)) & (scales.known != 0u);
           shown |= (sees ? 1u : 0u) << e;
@@ -849,21 +852,24 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       if (moves) scale_sums(o[cg], corr);
     }
 #pragma unroll
-    for (int x = 0; x < VL; x += EACH) {
-      if constexpr (!EARLY) read_values(x);
+    for (int step = 0; step < STEPS; ++step) {
+      if constexpr (!EARLY) read_values(step);
       half8_t value[EACH];
 #pragma unroll
       for (int y = 0; y < EACH; ++y) value[y] = ahead[y];
-      if (EARLY && x + EACH < VL) read_values(x + EACH);
+      if (EARLY && step + 1 < STEPS) read_values(step + 1);
+      const int x = element(step), of = HALVES == 2 ? 0 : step % 2, done = element(step + 1);
 #pragma unroll
       for (int term = 1; term >= 0; --term) {                       // (the same sum's products four apart)
 #pragma unroll
         for (int y = 0; y < EACH; ++y) {
 #pragma unroll
-          for (int cg = 0; cg < CG; ++cg) o[cg][x + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[y], term == 1 ? p_lo[cg][0] : p_hi[cg][0], o[cg][x + y], 0, 0, 0);
+          for (int cg = 0; cg < CG; ++cg) {
+            o[cg][x + y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(value[y], term == 1 ? p_lo[cg][of] : p_hi[cg][of], o[cg][x + y], 0, 0, 0);
+          }
         }
       }
-      if ((x + EACH) % WAVES == 0) stash_values(buf ^ 1u, x / WAVES);
+      if (done != x && done % WAVES == 0) stash_values(buf ^ 1u, done / WAVES - 1);
     }
     fetch_values(i + 2u, next);
     scales = of_next, of_next = after, next = further;
@@ -871,28 +877,33 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
   }
 
   // Merge of the halves.
-#pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const float total = groups_sum(col[cg].sum);
-    if (g == 0u) sh.ref[half][(group * CG + cg) * 16u + r] = col[cg].ref, sh.sum[half][(group * CG + cg) * 16u + r] = total;
-  }
-  lds_barrier();
   float factor[CG], top[CG], total[CG];
+  if constexpr (HALVES == 1) {
 #pragma unroll
-  for (int cg = 0; cg < CG; ++cg) {
-    const uint32_t at = (group * CG + cg) * 16u + r;
-    const float ref0 = sh.ref[0][at], ref1 = sh.ref[1][at];
-    top[cg] = fmaxf(ref0, ref1);
-    const float to = from_reference(top[cg]);
-    total[cg] = fmaf(__builtin_amdgcn_exp2f(ref1 - to), sh.sum[1][at], __builtin_amdgcn_exp2f(ref0 - to) * sh.sum[0][at]);
-    factor[cg] = __builtin_amdgcn_exp2f(col[cg].ref - to) / col[cg].up;
-    if (half == 1u) {
+    for (int cg = 0; cg < CG; ++cg) top[cg] = col[cg].ref, total[cg] = groups_sum(col[cg].sum), factor[cg] = 1.0f / col[cg].up;
+  } else {
 #pragma unroll
-      for (int x = 0; x < VL; ++x) sh.o[group * CG + cg][x][lane] = o[cg][x] * factor[cg];
+    for (int cg = 0; cg < CG; ++cg) {
+      const float total = groups_sum(col[cg].sum);
+      if (g == 0u) sh.ref[half][(group * CG + cg) * 16u + r] = col[cg].ref, sh.sum[half][(group * CG + cg) * 16u + r] = total;
     }
+    lds_barrier();
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      const uint32_t at = (group * CG + cg) * 16u + r;
+      const float ref0 = sh.ref[0][at], ref1 = sh.ref[1][at];
+      top[cg] = fmaxf(ref0, ref1);
+      const float to = from_reference(top[cg]);
+      total[cg] = fmaf(__builtin_amdgcn_exp2f(ref1 - to), sh.sum[1][at], __builtin_amdgcn_exp2f(ref0 - to) * sh.sum[0][at]);
+      factor[cg] = __builtin_amdgcn_exp2f(col[cg].ref - to) / col[cg].up;
+      if (half == 1u) {
+#pragma unroll
+        for (int x = 0; x < VL; ++x) sh.o[group * CG + cg][x][lane] = o[cg][x] * factor[cg];
+      }
+    }
+    lds_barrier();
+    if (half == 1u) return;
   }
-  lds_barrier();
-  if (half == 1u) return;
   const bool whole = w.tiles <= a.part_tiles;                       // no other part has tiles
   const uint64_t slot = ((static_cast<uint64_t>(unit) * b.kv_heads + kv) * a.parts + part) * a.stored;
 #pragma unroll
@@ -906,7 +917,9 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 #pragma unroll
     for (int x = 0; x < VL; ++x) {
       const uint32_t d = 16u * x + 4u * g;
-      const float4_t v = (o[cg][x] * factor[cg] + sh.o[group * CG + cg][x][lane]) * scale;
+      float4_t v = o[cg][x] * factor[cg];
+      if constexpr (HALVES == 2) v += sh.o[group * CG + cg][x][lane];
+      v *= scale;
       if (d < D) *reinterpret_cast<float4_t*>(to + d) = v;
     }
   }
@@ -923,7 +936,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   const uint32_t c = blockIdx.x % a.stored, rest = blockIdx.x / a.stored, kv = rest % b.kv_heads, unit = rest / b.kv_heads, t = threadIdx.x;
   PageUnit u;
   if (!find_unit(b, unit, [&](const PageSequence& q) { return C < 64 ? 1u : (q.rows * a.group + C - 1u) / C; }, &u)) return;
-  if constexpr (C == 64) u.at = (u.seq.rows * a.group + C - 1u) / C - 1u - u.at;      // as the tiles' kernel has it
+  if constexpr (C >= 64) u.at = (u.seq.rows * a.group + C - 1u) / C - 1u - u.at;      // as the tiles' kernel has it
   const UnitTiles w = C < 64 ? sequence_tiles(a, u.seq) : unit_tiles(a, u, C);
   if (c >= w.columns) return;                                       // workgroup-uniform, as the next ones
   // Places of the parts: the first one's, then from `then` on, `step` apart.
@@ -1022,8 +1035,14 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   }
   auto tile = [&](auto kind, auto dim) {
     constexpr int CG = decltype(dim)::value == 256 ? 1 : 2;
-    hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, decltype(dim)::value, CG>), dim3(static_cast<uint32_t>(groups * shape.parts)),
-                       dim3(512 / CG), 0, stream, a);
+    const dim3 grid(static_cast<uint32_t>(groups * shape.parts));
+    if constexpr (CG == 1) {
+      if (shape.columns == 128) {
+        hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, 256, 1, 1>), grid, dim3(512), 0, stream, a);
+        return;
+      }
+    }
+    hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, decltype(dim)::value, CG, 2>), grid, dim3(512 / CG), 0, stream, a);
   };
   auto few = [&](auto kind, auto dim, auto cg) {
     constexpr int DP = decltype(dim)::value, CG = decltype(cg)::value;
@@ -1032,7 +1051,7 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
     else hipLaunchKernelGGL((attention_pages_few_kernel<decltype(kind)::value, DP, CG, 4>), grid, dim3(256), 0, stream, a);
   };
   auto with_columns = [&](auto kind, auto dim) {
-    if (shape.columns == 64) return tile(kind, dim);
+    if (shape.columns >= 64) return tile(kind, dim);
     if constexpr (decltype(dim)::value <= 128) {
       if (shape.columns == 32) return few(kind, dim, std::integral_constant<int, 2>{});
     }
@@ -1047,7 +1066,8 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || !split) return e;
   auto merge = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups * a.stored)), dim3(256), 0, stream, a); };
-  shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : shape.columns == 32 ? merge(attention_pages_merge_kernel<32>) : merge(attention_pages_merge_kernel<64>);
+  shape.columns == 16 ? merge(attention_pages_merge_kernel<16>) : shape.columns == 32 ? merge(attention_pages_merge_kernel<32>)
+  : shape.columns == 64 ? merge(attention_pages_merge_kernel<64>) : merge(attention_pages_merge_kernel<128>);
   return hipGetLastError();
 }
 
