@@ -727,11 +727,13 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
     const uint32_t col = w.first_col + (at < w.columns ? at : w.columns - 1u);
     return col / a.group;
   };
-  {
-    const uint32_t own = wave % SETS, at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
+  constexpr uint32_t SHARE = WAVES > SETS ? WAVES / SETS : 1;
+#pragma unroll
+  for (uint32_t own = wave % SETS; own < SETS; own += WAVES) {
+    const uint32_t at = own * 16u + r, col = w.first_col + (at < w.columns ? at : w.columns - 1u), row = col / a.group;
     float raw[DP / 64][16];
     query_load<DP>(a.q + (static_cast<uint64_t>(u.seq.first + row) * a.heads + kv * a.group + col % a.group) * D, D, raw);
-    const float scale = query_terms<KIND, DP>(raw, D, sh.q[own], wave / SETS, WAVES / SETS);
+    const float scale = query_terms<KIND, DP>(raw, D, sh.q[own], wave / SETS, SHARE);
     if (g == 0u) sh.scale[own * 16u + r] = scale;
   }
   lds_barrier();
@@ -1036,11 +1038,10 @@ hipError_t launch_attention_pages(bool fp8, const PageAttentionCall& c, const Pa
   auto tile = [&](auto kind, auto dim) {
     constexpr int CG = decltype(dim)::value == 256 ? 1 : 2;
     const dim3 grid(static_cast<uint32_t>(groups * shape.parts));
-    if constexpr (CG == 1) {
-      if (shape.columns == 128) {
-        hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, 256, 1, 1>), grid, dim3(512), 0, stream, a);
-        return;
-      }
+    constexpr int TALL = decltype(dim)::value == 64 ? 2 : 1;
+    if (shape.columns == 128) {
+      hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, decltype(dim)::value, TALL, 1>), grid, dim3(512 / TALL), 0, stream, a);
+      return;
     }
     hipLaunchKernelGGL((attention_pages_tile_kernel<decltype(kind)::value, decltype(dim)::value, CG, 2>), grid, dim3(512 / CG), 0, stream, a);
   };

@@ -374,7 +374,7 @@ constexpr size_t pages_bytes(const PagesCall& c, const PagesShape& shape) {
 // 215 / 205; 48 of 4 heads of 256, 1500 27 / 31, 3000 52 / 46, 8000 124 / 88; 200 of them, 3000 147 / 151, 5000 225 / 211.
 // Many columns: parts only where the units are fewer than two a CU.  (`most`: bytes that the parts may take.)
 constexpr PagesShape pages_rule(const PagesCall& c, uint64_t cus, size_t most) {
-  const uint64_t pairs = c.max_rows * c.group, columns = pairs <= 16 ? 16 : pairs <= 32 && c.head_dim <= 128 ? 32 : pairs <= 64 || c.head_dim <= 128 ? 64 : 128;
+  const uint64_t pairs = c.max_rows * c.group, columns = pairs <= 16 ? 16 : pairs <= 32 && c.head_dim <= 128 ? 32 : pairs <= 64 ? 64 : 128;
   const uint64_t tiles = pages_tiles(c, columns), groups = pages_units(c, columns) * c.kv_heads, log_tile = pages_log_tile(c.head_dim, columns);
   const uint64_t resident = 2 * cus < kPagePartsMost ? 2 * cus : kPagePartsMost;
   const PagesShape one{columns, 1, tiles, 0, columns < 64 && groups <= cus ? 8u : 4u};

@@ -16,7 +16,7 @@ def test_pages_rule(tmp_path):
       const size_t most = size_t{16} << 20;
       const PagesShape s = pages_rule(c, cus, most);
       const uint64_t units = pages_units(c, s.columns), groups = units * kv, tiles = pages_tiles(c, s.columns), stored = pages_stored(c, s.columns);
-      CHECK(s.columns == 16 || s.columns == 64 || (s.columns == 32 ? d <= 128 : s.columns == 128 && d > 128), "%zu columns", static_cast<size_t>(s.columns));
+      CHECK(s.columns == 16 || s.columns == 64 || s.columns == 128 || (s.columns == 32 && d <= 128), "%zu columns", static_cast<size_t>(s.columns));
       CHECK(s.columns >= 64 || c.max_rows * group <= s.columns, "a sequence is one unit");
       CHECK(units >= sequences * ((each * group + s.columns - 1) / s.columns), "%zu units", static_cast<size_t>(units));      // (all have as many rows)
       CHECK(stored >= 1 && stored <= s.columns, "stored");
