@@ -324,9 +324,10 @@ __device__ __forceinline__ uint32_t draw_token(const DraftArgs& a, Verdict v, co
   }
   // (a number outside [0, 1) is the nearest in it)
   const double goal = (u >= 0.0f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0) * whole;
-  // The first whose running sum exceeds the goal; where rounding leaves none, the last that has something.
+  // The first with something whose running sum exceeds the goal; where rounding leaves none, the last with something.  (Running sums of
+  // lanes are not of one order of additions: by a rounding that of a lane with nothing may exceed the goal where the one before does not.)
   auto first_over = [](bool over, bool any) {
-    const uint64_t some = __ballot(over), last = __ballot(any);
+    const uint64_t some = __ballot(over && any), last = __ballot(any);
     return some != 0u ? static_cast<uint32_t>(__ffsll(static_cast<unsigned long long>(some)) - 1)
                       : 63u - static_cast<uint32_t>(__clzll(static_cast<unsigned long long>(last | 1u)));
   };
