@@ -28,7 +28,7 @@ struct PageAttention {
   const uint8_t *k, *v;
   const float *k_scale, *v_scale;
   float* out;
-  float *part_sum, *part_most, *part_total;   // (unit, key head, part, one of `stored` columns): head_dim sums; the reference in powers of two; the weights' sum
+  float *part_sum, *part_most, *part_total;   // (unit, key head, part, one of `stored` columns): the part's result; its reference in powers of two; its weights' sum
   uint32_t heads, group, window, sinks;       // window 0: every position
   uint32_t log_tile, parts, part_tiles, stored, even;   // positions a tile; tiles a part; columns of a unit that a part has room for; workgroups of an even split, or 0
 };
@@ -136,6 +136,10 @@ __device__ __forceinline__ void scale_sums(float4_t (&o)[N], float corr) {
   asm volatile("s_nop 1" ::);                                       // (before a matrix instruction takes them)
 }
 
+// What a sum of weights times values is multiplied by, of weights that are `total` together.  Before all else: a result is no larger than
+// its values are, where their sum could be past fp32's range.
+__device__ __forceinline__ float share_of(float total) { return total == 0.0f ? 0.0f : 1.0f / total; }
+
 // Weights are taken relative to a reference that follows a column's largest score only where that would leave it by 2^kSlack.
 constexpr float kSlack = 3.0f;
 
@@ -204,7 +208,7 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
 //
 // Of units that are a sequence each: all their tiles, a sequence's heads one behind the other, in runs of equal cost, one a workgroup.
 // To begin a head costs what begin_tiles do: so many lie before its first, with nothing in them.  A run that covers a head whole gives
-// its result, else it leaves the sums for the merge: in the workgroup's first place those of its first head, in its second those of
+// its result, else it leaves its own for the merge: in the workgroup's first place that of its first head, in its second that of
 // a later one.
 __device__ __forceinline__ uint32_t even_of(const PageAttention& a, const PageSequence& seq) {
   return seq.rows == 0u ? 0u : sequence_tiles(a, seq).tiles + begin_tiles(a.log_tile);
@@ -569,21 +573,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
     for (; i + NW < end; i += NW) tile(std::false_type{});
     if (i < end) tile(std::true_type{});
 
-    // Merge of the wavefronts under the largest reference.
+    // Merge of the wavefronts' results by the weights that they have under the largest reference.
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
-      const float total = groups_sum(col[cg].sum);
-      if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = total;
+      col[cg].sum = groups_sum(col[cg].sum);
+      if (g == 0u) sh.ref[wave][cg * 16u + r] = col[cg].ref, sh.sum[wave][cg * 16u + r] = col[cg].sum;
     }
     __syncthreads();                                                  // (no wavefront reads the queries any more)
 #pragma unroll
     for (int cg = 0; cg < CG; ++cg) {
-      float top = -INFINITY;
+      const float share = share_of(col[cg].sum), factor = 1.0f / col[cg].up;
 #pragma unroll
-      for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][cg * 16u + r]);
-      const float factor = __builtin_amdgcn_exp2f(col[cg].ref - from_reference(top)) / col[cg].up;
-#pragma unroll
-      for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * factor;
+      for (int x = 0; x < VL; ++x) *reinterpret_cast<float4_t*>(&sh.o[wave][cg * 16u + r][16 * x + 4 * g]) = o[cg][x] * share * factor;
     }
     __syncthreads();
     const bool whole = begin == 0u && end == w.tiles;                 // no other part has tiles
@@ -593,17 +594,18 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
       float top = -INFINITY;
 #pragma unroll
       for (int n = 0; n < NW; ++n) top = fmaxf(top, sh.ref[n][c]);
-      float total = 0.0f;
+      float weight[NW], total = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NW; ++n) weight[n] = __builtin_amdgcn_exp2f(sh.ref[n][c] - from_reference(top)) * sh.sum[n][c], total += weight[n];
+      const float share = share_of(total);
       float4_t x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int n = 0; n < NW; ++n) {
-        total = fmaf(__builtin_amdgcn_exp2f(sh.ref[n][c] - from_reference(top)), sh.sum[n][c], total);
-        x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]);
-      }
+      for (int n = 0; n < NW; ++n) x += *reinterpret_cast<const float4_t*>(&sh.o[n][c][d]) * (weight[n] * share);
+      if (total == 0.0f) x = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
       if (whole) {
         const uint32_t pair = c;
         float* to = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
-        *reinterpret_cast<float4_t*>(to) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
+        *reinterpret_cast<float4_t*>(to) = x;
       } else {
         *reinterpret_cast<float4_t*>(a.part_sum + (slot + c) * D + d) = x;
         if (d == 0u) a.part_most[slot + c] = top, a.part_total[slot + c] = total;
@@ -900,7 +902,7 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       factor[cg] = __builtin_amdgcn_exp2f(col[cg].ref - to) / col[cg].up;
       if (half == 1u) {
 #pragma unroll
-        for (int x = 0; x < VL; ++x) sh.o[group * CG + cg][x][lane] = o[cg][x] * factor[cg];
+        for (int x = 0; x < VL; ++x) sh.o[group * CG + cg][x][lane] = o[cg][x] * share_of(total[cg]) * factor[cg];
       }
     }
     lds_barrier();
@@ -914,14 +916,14 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
     if (c >= w.columns) continue;
     const uint32_t at = w.first_col + c;
     float* to = whole ? a.out + (static_cast<uint64_t>(u.seq.first + at / a.group) * a.heads + kv * a.group + at % a.group) * D : a.part_sum + (slot + c) * D;
-    const float scale = !whole ? 1.0f : total[cg] == 0.0f ? 0.0f : 1.0f / total[cg];
+    const float share = share_of(total[cg]);
     if (!whole && g == 0u) a.part_most[slot + c] = top[cg], a.part_total[slot + c] = total[cg];
 #pragma unroll
     for (int x = 0; x < VL; ++x) {
       const uint32_t d = 16u * x + 4u * g;
-      float4_t v = o[cg][x] * factor[cg];
+      float4_t v = o[cg][x] * share * factor[cg];
       if constexpr (HALVES == 2) v += sh.o[group * CG + cg][x][lane];
-      v *= scale;
+      if (total[cg] == 0.0f) v = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
       if (d < D) *reinterpret_cast<float4_t*>(to + d) = v;
     }
   }
@@ -929,7 +931,8 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
 
 // ---- the parts' merge ----------------------------------------------------------------------------
 
-// A workgroup a column: its parts' sums under the largest of their references, the first parts' loads under way at once.
+// A workgroup a column: its parts' results by the weights that they have under the largest of their references, the first parts' loads under
+// way at once.
 template <int C>
 __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttention a) {
   __shared__ float of_wave[2][4], weight[kPagePartsMost];
@@ -957,7 +960,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   if (parts == 1u) return;
   const uint32_t D = b.head_dim, runs = D / 4u;
   auto column = [&](uint32_t p) { return (p == 0u ? place : then + (p - 1u) * step) * a.stored + c; };
-  // 256 / runs threads a run of four elements; the first parts' sums are asked for before their weights are there
+  // 256 / runs threads a run of four elements; the first parts' results are asked for before their weights are there
   constexpr uint32_t AHEAD = 8, OWN = kPagePartsMost / 256u;
   float own[OWN], sum[OWN], most = -INFINITY;
 #pragma unroll
@@ -978,21 +981,21 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   float all = 0.0f;
 #pragma unroll
   for (uint32_t i = 0; i < OWN; ++i) {
-    const float f = t + 256u * i < parts ? __builtin_amdgcn_exp2f(own[i] - from_reference(top)) : 0.0f;
+    const float f = t + 256u * i < parts ? __builtin_amdgcn_exp2f(own[i] - from_reference(top)) * sum[i] : 0.0f;
     weight[t + 256u * i] = f;
-    all = fmaf(f, sum[i], all);
+    all += f;
   }
   all = wave_sum(all);
   if ((t & 63u) == 0u) of_wave[1][t >> 6] = all;
   __syncthreads();
-  const float total = (of_wave[1][0] + of_wave[1][1]) + (of_wave[1][2] + of_wave[1][3]);
+  const float total = (of_wave[1][0] + of_wave[1][1]) + (of_wave[1][2] + of_wave[1][3]), share = share_of(total);
 #pragma unroll
   for (uint32_t i = 0; i < AHEAD; ++i) {
-    if (mine + i * lanes < parts) x += early[i] * weight[mine + i * lanes];
+    if (mine + i * lanes < parts) x += early[i] * (weight[mine + i * lanes] * share);
   }
 #pragma unroll 4
   for (uint32_t p = mine + AHEAD * lanes; p < parts; p += lanes) {
-    if (mine < lanes) x += *reinterpret_cast<const float4_t*>(a.part_sum + column(p) * D + d) * weight[p];
+    if (mine < lanes) x += *reinterpret_cast<const float4_t*>(a.part_sum + column(p) * D + d) * (weight[p] * share);
   }
   piece[t] = x;
   __syncthreads();
@@ -1000,7 +1003,7 @@ __global__ __launch_bounds__(256) void attention_pages_merge_kernel(PageAttentio
   for (uint32_t n = 1; n < lanes; ++n) x += piece[n * runs + t];
   const uint32_t pair = w.first_col + c;
   float* out = a.out + (static_cast<uint64_t>(u.seq.first + pair / a.group) * a.heads + kv * a.group + pair % a.group) * D + d;
-  *reinterpret_cast<float4_t*>(out) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / total);
+  *reinterpret_cast<float4_t*>(out) = total == 0.0f ? float4_t{0.0f, 0.0f, 0.0f, 0.0f} : x;
 }
 
 }  // namespace

@@ -361,7 +361,7 @@ constexpr uint64_t pages_tiles(const PagesCall& c, uint64_t columns) {
   const uint64_t some = (c.sinks + tile - 1) / tile + (c.window + c.max_rows + tile - 1) / tile + 1;
   return c.window == 0 || all < some ? all : some;
 }
-// What the parts leave for the merge: for each column its sums, their reference and the weights' sum.
+// What the parts leave for the merge: for each column their result, its reference and its weights' sum.
 constexpr size_t pages_bytes(const PagesCall& c, const PagesShape& shape) {
   const uint64_t places = shape.even != 0 ? 2 * shape.even : shape.parts < 2 ? 0 : pages_units(c, shape.columns) * c.kv_heads * shape.parts;
   return static_cast<size_t>(places * pages_stored(c, shape.columns) * (c.head_dim + 2) * 4);
