@@ -172,7 +172,11 @@ __device__ __forceinline__ bool weigh(Column& c, float (&s)[COUNT], float scale,
     c.ref = fmaxf(c.ref, groups_max(most));
     float by = before == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(before - c.ref);
     c.sum *= by;
-    c.most = fmaxf(c.most * by, __builtin_amdgcn_exp2f(most - from_reference(c.ref)) * v_scale);
+    // A weight counts as 2^-116 at least, so that v_scale * up is finite (the least is 2^-126: their terms begin 2^10 lower at most);
+    // without any the scale may be as large as it likes, and nothing is weighed under it.  (NaN stays.)
+    const float weight = __builtin_amdgcn_exp2f(most - from_reference(c.ref));
+    c.most = fmaxf(c.most * by, (weight > 0.0f ? fmaxf(weight, 0x1p-116f) : 0.0f) * v_scale);
+    v_scale = weight == 0.0f && v_scale < INFINITY ? 0.0f : v_scale;
     const float largest = groups_max(c.most), scaled = largest * c.up;
     if (largest > 0.0f && !(scaled >= 0x1p9f && scaled < 0x1p12f)) {
       const float up = power_to(largest, 10);
