@@ -381,12 +381,16 @@ constexpr PagesShape pages_rule(const PagesCall& c, uint64_t cus, size_t most) {
   if (groups * pages_stored(c, columns) >= (1u << 24)) return one;      // (the merge has a workgroup a column: a grid of fewer than 2^32 threads)
   if (columns < 64) {
     const uint64_t parts = (tiles + 3) / 4, of_64 = tiles >> (6 - log_tile);
-    const PagesShape each{columns, parts, 4, 0, 4}, even{columns, 1, tiles, resident, 4};
+    const PagesShape each{columns, parts, 4, 0, 4};
     if (groups * parts <= resident) {
       return parts < 2 || of_64 <= (c.head_dim <= 64 ? 24 : c.head_dim <= 128 ? 12 : 6) || pages_bytes(c, each) > most ? one : each;
     }
     if (of_64 <= 32 || of_64 <= 38 * groups / resident) return one;
-    return c.sequences * c.kv_heads * (tiles + begin_tiles(5)) < (1u << 30) && pages_bytes(c, even) <= most ? even : one;      // (32-bit sums)
+    // As many workgroups as are on the chip at once, or as leave no more than there is room for: of 16 MB 504 of 512 where all of 32 columns
+    // of 128, 508 where all of 16 of 256 are there.
+    const PagesShape even{columns, 1, tiles, 1, 4};
+    const uint64_t room = most / pages_bytes(c, even), runs = room < resident ? room : resident;
+    return c.sequences * c.kv_heads * (tiles + begin_tiles(5)) < (1u << 30) && runs != 0 ? PagesShape{columns, 1, tiles, runs, 4} : one;      // (32-bit sums)
   }
   uint64_t parts = groups >= 2 * cus ? 1 : 2 * cus / groups;
   if (parts > 256) parts = 256;
