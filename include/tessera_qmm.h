@@ -229,10 +229,14 @@ const char* qmm_kernel_name(size_t index);
  *     see does not reach it.  max_rows, max_len: the most rows and positions that a sequence has (0: rows, width * block),
  *     which the launch is shaped by; a sequence with more is left out.  (E4M3's codes of NaN, which "pages_write_fp8" does not
  *     write, are not looked for: in a page of Vp that is walked they reach rows that do not see them.)  Scores and sums are
- *     fp32.  A query's element goes to 2^-23 of its head's largest over int8 pages, over E4M3 ones to 2^-22 of itself down
+ *     fp32, a result no larger than its values.  A query's element goes to 2^-23 of its head's largest over int8 pages, over E4M3 ones to 2^-22 of itself down
  *     to 2^-16 of that largest (2^-38 of it below); a weight times its value's scale to 2^-22 of itself down to 2^-12 of the
- *     row's largest (2^-34 of that below).
+ *     row's largest (2^-34 of that below; 2^10 coarser where weights lie 2^116 and more below their row's largest, and from 2^-126
+ *     of it on a weight is 0).
  *     How positions are shared among workgroups depends on the sizes, max_rows, max_len and Lens, and the last bits with it.
+ *     The launch is shaped by max_rows alone, so that a prompt makes a batch's other sequences slow (60 of one row on 3000 beside
+ *     500 rows on 1000: 160 to 240 us, in two calls 110 to 165).  Put prompts first and make two calls over the same buffers: of the
+ *     prompts alone (`sequences`), and of all with a max_rows that leaves the prompts out.
  *     "draft_verify": buffers Logits (rows x vocab floats), Tokens (rows u32), Random (rows x 2 floats in [0, 1)), Starts,
  *     Accepted, Next (sequences u32)[, DraftLogits (as Logits)]; scalars rows, vocab, sequences, temperature,
  *     draft_temperature (fp32 bits).  Row i of a sequence holds the target's logits behind Tokens[i]; Tokens[i + 1] was
@@ -240,8 +244,9 @@ const char* qmm_kernel_name(size_t index);
  *     With p = softmax(logits / temperature), q the draft's: a draft x stands where Random[i][0] q(x) < p(x).  Accepted:
  *     how many stand before the first that does not; Next: the token behind them, the first whose running sum of
  *     max(p - q, 0) there (without DraftLogits: of p but for x; where nothing is left, or behind the last row: of p)
- *     exceeds Random[i][1] (outside [0, 1): the nearest in it) of the whole.  All in fp64.  temperature 0: a draft stands where it is the row's largest logit,
- *     the lowest of equals, and Next is that.  -infinity is a token of probability 0.  A row that holds NaN or +infinity or
+ *     exceeds Random[i][1] (outside [0, 1): the nearest in it) of the whole.  All in fp64, the exponentials to 2^-39 of themselves; a
+ *     token without a probability is never drawn.  temperature 0: a draft stands where it is the row's largest logit, the lowest
+ *     of equals, and Next is that.  -infinity is a token of probability 0.  A row that holds NaN or +infinity or
  *     nothing but -infinity (the draft's likewise, where it is needed) ends the draft there, with Next 0xFFFFFFFF.  A token
  *     of vocab or more never stands.  vocab is at most 2^21.
  *   - "mfma_probe": buffer Out (workgroups * 256 floats); scalars kind (0 fp16 32x32x16, 1 scaled

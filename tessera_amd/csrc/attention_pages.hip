@@ -8,8 +8,8 @@
 // largest element, in three int8 limbs: an element is carried to 2^-23 of the largest, products and sums are exact.  Else it is two fp16
 // terms, x = hi + lo, hi = RN16(x), lo = RN16(x - hi), under a power of two that brings a query's largest element to 2^13 .. 2^14 (an
 // element is carried to 2^-22 of itself down to 2^-16 of the largest, below to 2^-38 of that), the largest of a row's weights times their
-// values' scales so far to 2^9 .. 2^15 (to 2^-22 of itself down to 2^-12 of the largest, below to 2^-34 of that).  Codes enter exactly; a
-// key's scale multiplies its fp32 score.  Scores, references, sums and results are fp32.
+// values' scales so far to 2^9 .. 2^15 (to 2^-22 of itself down to 2^-12 of the largest, below to 2^-34 of that; 2^10 coarser where weights
+// are below 2^-116).  Codes enter exactly; a key's scale multiplies its fp32 score.  Scores, references, sums and results are fp32.
 
 #include <type_traits>
 
@@ -35,8 +35,8 @@ struct PageAttention {
 
 // ---- which positions a unit walks ----------------------------------------------------------------
 //
-// A unit is COLUMNS (row, head) pairs of a key head in one sequence, `group` pairs to a row.  It walks tiles of 64 positions: those with
-// sinks that lie before its windows, then those from the first row's window to the last row's position.
+// A unit is COLUMNS (row, head) pairs of a key head in one sequence, `group` pairs to a row.  It walks tiles of 64 positions, or of 32 where
+// pages_log_tile says so: those with sinks that lie before its windows, then those from the first row's window to the last row's position.
 struct UnitTiles {
   uint32_t columns;               // that there are
   uint32_t first_col;             // its first among the sequence's
@@ -621,13 +621,15 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_pages_few_kernel(PageAtt
 
 // ---- many columns --------------------------------------------------------------------------------
 //
-// Bound by the matrix instructions and the vector instructions beside them.  64 columns a workgroup, 4 / CG groups of 16 CG times two halves
-// of a tile of 64 positions: of each page's sixteen positions of the tile a wavefront takes the first or the last eight.  (CG 2 reads half as
-// much of the LDS; of heads of 256 its sums are more registers than there are.)  2 x 1500 rows over up to 2000 more, 24 heads over 4 of 256,
-// 137 GFLOP: 320 us (int8), 300 (E4M3); 48 over 8 of 128: 310, 297; 32 over 8 of 64: 160, 123.  As the terms have it that is 3.5 and 4 times
-// as many products as one fp16 product would be: 0.75 and 0.9 PFLOP/s.  The matrix instructions are busy in a third of the cycles, the
-// vector instructions (200 beside 56 of the others) in another, both wavefronts of a SIMD between the same barriers.  (Halves
-// that take turns at them, with barriers between, were slower: their registers did not suffice.  So were priorities by half or by phase.)
+// Bound by the matrix instructions and the vector instructions beside them.  A workgroup takes 128 columns, a wavefront 16 CG of them and all
+// of a tile of 64 positions (HALVES 1); or, where 64 are enough, those, 4 / CG groups of 16 CG times two halves of a tile: of each page's
+// sixteen positions of the tile a wavefront takes the first or the last eight, and the halves are merged in the end.  (CG 2 reads half as much
+// of the LDS; of heads of 256, and of 128 with all of a tile, its sums are more registers than there are.)  2 x 1500 rows over up to 2000
+// more, 24 heads over 4 of 256, 137 GFLOP: 244 us (E4M3 248); 48 over 8 of 128: 281, 282; 32 over 8 of 64: 143, 127 (pages_rule has those of 64
+// columns).  As the terms have it, int8 products at twice the rate, that is 1.75 and 2 times the work of fp16 products: 1.0 and 1.1, 0.85 and
+// 1.0, 0.55 and 0.7 PFLOP/s.  Of heads of 256 over int8 pages the matrix instructions are busy in two fifths of the cycles, the vector instructions
+// (three beside each of the others) in another third, the wavefronts of a SIMD between the same barriers.  (Halves that take turns at
+// them, with barriers between, were slower: their registers did not suffice.  So were priorities by half or by phase.)
 // The tile's operands lie in LDS, made once for all columns: keys' as few_kernel's (int8 codes as they are), values' as fp16,
 // each operand's 64 lanes side by side, so that every write and read is whole lines.  While a tile is multiplied the next one goes to the
 // other half of the LDS and the one after that is under way.
@@ -827,7 +829,8 @@ __global__ __launch_bounds__(512 / CG, 2) void attention_pages_tile_kernel(PageA
       }
     }
     fetch_keys(i + 2u, next);
-    // The first values' operands are on their way while the weights are formed.  (Not where that costs the third wavefront a SIMD.)
+    // The first values' operands are on their way while the weights are formed.  (Not of heads of 64, which with 64 columns of E4M3 are three
+    // wavefronts a SIMD without.)
     constexpr bool EARLY = DP > 64;
     constexpr int EACH = 4 / CG, STEPS = 2 * VL / HALVES / EACH;    // value operands of a step
     half8_t ahead[EACH];

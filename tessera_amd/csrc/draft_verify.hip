@@ -12,8 +12,8 @@
 //
 // Two launches: the statistics of all rows, a wavefront a chunk; then a workgroup a sequence, or where drafts have probabilities as
 // many as fill the chip, of which the last to arrive draws.  Without scratch a workgroup takes a sequence, with the same bits.
-// The first is bound by the fp64 instructions, some twenty a logit (100 rows of 131072 of target and draft each: 28 us, 3.7 TB/s), the
-// second by one way to memory after the other (8 us without the draft's probabilities, 13 with them, 18 for 32 sequences): nothing is to
+// The first is bound by the fp64 instructions, some twenty a logit (100 rows of 131072 of target and draft each: 29 us, 3.6 TB/s), the
+// second by one way to memory after the other (8 us without the draft's probabilities, 13 with them, 20 for 32 sequences): nothing is to
 // keep it waiting besides, above all no array or struct with padding that the compiler would put into LDS by the dispatch packet's sizes,
 // which lies in the host's memory (22 us of 32).
 

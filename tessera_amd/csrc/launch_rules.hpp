@@ -329,7 +329,7 @@ constexpr LogprobPlan logprob_plan(uint64_t rows, uint64_t vocab, uint64_t top_k
 }
 
 // ---- "attention_pages" -----------------------------------------------------------------------------------------------
-// A unit is `columns` (row, head) pairs of a key head in a sequence: one unit a sequence where 16 or 32 hold all, else 64 each.
+// A unit is `columns` (row, head) pairs of a key head in a sequence: one unit a sequence where 16, 32 or 64 hold all, else 128 each.
 struct PagesCall {
   uint64_t rows, sequences, group, kv_heads, head_dim, max_rows, max_len, window, sinks;      // group: queries' heads to a key head
 };
@@ -372,7 +372,13 @@ constexpr size_t pages_bytes(const PagesCall& c, const PagesShape& shape) {
 // 128, 400 10.4 / 13.2, 1000 13.7 / 13.2; 4 heads of 256, 250 11.8 / 14.0, 500 14.9 / 14.0.  One / even split, sequences of all
 // lengths up to the stated one: 40 of 8 heads of 128, 2000 29 / 32, 3000 51 / 41; 128 of them, 3000 92 / 99, 5000 142 / 141, 8000
 // 215 / 205; 48 of 4 heads of 256, 1500 27 / 31, 3000 52 / 46, 8000 124 / 88; 200 of them, 3000 147 / 151, 5000 225 / 211.
-// Many columns: parts only where the units are fewer than two a CU.  (`most`: bytes that the parts may take.)
+// Many columns: 64 where they hold all, else 128 (though 65 pairs fill half of those).  us, 64 / 128 columns, int8, heads of 64, 128 and 256 (8, 8 and
+// 4 key heads; E4M3 within 8 % but for 190 / 182 of the first): 2 x 1500 rows of 6 queries on 1000 positions 254 / 199, 321 / 299, 298 / 263; 4 x
+// 512 of 4 on 4000 258 / 207, 319 / 273, 273 / 231; 64 x 13 of 5 on 1000 77 / 60, 96 / 82, 93 / 70; 8 x 15 of 6 on 3000 53 / 48, 70 / 66, 55 / 50.  They
+// cost where units of 128 leave CUs idle and parts of theirs do not fit or do not pay: 8 x 50 of 4 on 3000 93 / 92, 102 / 98, 96 / 141; 32 x 15 of
+// 6 on 2000 72 / 108, 90 / 77, 78 / 104; 400 of 4 alone 34 / 36, 38 / 37, 31 / 37.
+// Parts only where the units are fewer than two a CU, as if two workgroups were on a CU at once.  So they are of 256 threads; of 512 threads (heads
+// over 64 in 128 columns, over 128 in 64) it is one.  (`most`: bytes that the parts may take.)
 constexpr PagesShape pages_rule(const PagesCall& c, uint64_t cus, size_t most) {
   const uint64_t pairs = c.max_rows * c.group, columns = pairs <= 16 ? 16 : pairs <= 32 && c.head_dim <= 128 ? 32 : pairs <= 64 ? 64 : 128;
   const uint64_t tiles = pages_tiles(c, columns), groups = pages_units(c, columns) * c.kv_heads, log_tile = pages_log_tile(c.head_dim, columns);
